@@ -44,6 +44,10 @@ extern "C" {
 #define HS_DTYPE_F32 0
 #define HS_DTYPE_F16 1
 #define HS_DTYPE_BF16 2
+/* Element codes of a quantised KV pool (hs_append_quantized): signed 8-bit integers, and
+ * 8-bit floats of four significand bits (largest 448, no infinity) */
+#define HS_DTYPE_I8 3
+#define HS_DTYPE_E4M3 4
 
 typedef struct ihipStream_t* hs_stream_t;
 
@@ -405,6 +409,61 @@ int hs_attend_window(const void* query, int64_t q_stride_h, const void* pool, in
                      void* workspace, int64_t workspace_bytes, hs_stream_t stream);
 
 /*
+ * Attention of one new token per request over page tables; no counterpart in the
+ * reference (its page layout attends one request's windows one by one,
+ * reference/attention.py:42-128).
+ *   query    [batch, heads, head_dim] in query_dtype (strides in elements, head_dim
+ *            contiguous)
+ *   pool     [blocks, 2, P, Hkv, D]: float32, float16 or bfloat16 (then query_dtype is
+ *            pool_code and scales is null), or the codes of hs_append_quantized with their
+ *            scales [blocks, 2, P, Hkv] (any query_dtype)
+ *   tables   int32 [batch, pages] (t_stride_k = 0) or [batch, kv_heads, pages]: token t of
+ *            a request sits in row t % P of block table[t / P]; an entry below 0 or at or
+ *            past `blocks` is an absent page, whose tokens are masked
+ *   lengths  int32 [batch] on the device: tokens of each request (clamped to 0 ..
+ *            pages * P); rows past them are never used
+ *   out      [batch, heads, head_dim] in query_dtype; 0 for a request without a token
+ * Scores, softmax statistics and sums are fp32.  The workspace
+ * (hs_attend_pages_workspace_bytes of the same sizes, 8-byte aligned) may hold anything
+ * before a call; calls that share one must run in order.  Nothing is read on the host, so
+ * a captured call replays with the tables and lengths of the moment.
+ */
+int64_t hs_attend_pages_workspace_bytes(int32_t query_dtype, int32_t pool_code, int64_t batch, int64_t heads,
+                                        int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t pages);
+int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_stride_h, int32_t query_dtype,
+                    const void* pool, const float* scales, int32_t pool_code, int64_t blocks, int64_t page_size,
+                    int64_t kv_heads, int64_t head_dim, const int32_t* tables, int64_t t_stride_b,
+                    int64_t t_stride_k, int64_t pages, const int32_t* lengths, int64_t batch, int64_t heads,
+                    void* out, int64_t o_stride_b, int64_t o_stride_h, void* workspace, int64_t workspace_bytes,
+                    hs_stream_t stream);
+
+/* ------------------------------------------------------- quantised KV rows */
+
+/*
+ * 8-bit K/V rows of a paged pool; no counterpart in the reference.  The pool is codes
+ * [blocks, 2, P, Hkv, D] (code HS_DTYPE_I8 or HS_DTYPE_E4M3) and scales [blocks, 2, P, Hkv]
+ * float32.  Per head vector of largest magnitude a: scale = a / top rounded to float32 (top
+ * 127 or 448), each code the nearest to the exact quotient by the scale (ties to even);
+ * zeros give scale 0; a vector with a NaN or infinity gets scale NaN and codes 0, and so
+ * reads back as NaN.
+ *   rows   int64 on the device: physical rows (block * P + offset).  hs_append_quantized
+ *          skips a row outside [0, pool_rows); rows of one call must differ (of two equal
+ *          ones the codes and the scale may come from different tokens).  hs_read_quantized
+ *          gives zeros for a row outside the pool.
+ *   k, v   hs_append_quantized: [tokens, Hkv, D] in `dtype`, element strides per token and
+ *          head; hs_read_quantized: [n, Hkv, D] contiguous out, code * scale rounded to
+ *          `dtype`
+ * pool_rows = blocks * P; head_dim at most 512; tokens or n may be 0.
+ */
+int hs_append_quantized(const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                        int64_t v_stride_h, int32_t dtype, const int64_t* rows, int64_t tokens, void* codes,
+                        float* scales, int32_t code, int64_t pool_rows, int64_t page_size, int64_t kv_heads,
+                        int64_t head_dim, hs_stream_t stream);
+int hs_read_quantized(const void* codes, const float* scales, int32_t code, int64_t pool_rows, int64_t page_size,
+                      int64_t kv_heads, int64_t head_dim, const int64_t* rows, int64_t n, void* k, void* v,
+                      int32_t dtype, hs_stream_t stream);
+
+/*
  * Diagnostic (no reference counterpart): read, without computing, n segment
  * pairs of a device region -- segment i at byte offset offsets[i] (device
  * array) and its partner plane_bytes further, segment_bytes each -- with
@@ -443,6 +502,10 @@ int hs_attend_time_next(void* start_event, void* stop_event);
  *   kv_heads, kv_heads head vectors of head_dim); writes rotated q [rows, heads,
  *   head_dim], rotated k and copied v [rows, kv_heads, head_dim] at the row's
  *   position positions[row] (device int64) with base `theta`.
+ * hs_norm_rotary_split: hs_rotary_split with a per-head RMSNorm of q and k before the
+ *   rotation (weights q_weight and k_weight [head_dim], `eps` added to the mean square; no
+ *   counterpart in the reference, whose heads are not normed).  Computed in fp32 with the
+ *   angles position * theta^(-2i/D) reduced in 64 bits, and rounded once.  head_dim <= 512.
  * hs_silu_mul: out[row, j] = silu(g[row, j]) * u[row, j] where a gate_up row
  *   holds g (width) then u (width).
  */
@@ -452,6 +515,9 @@ int hs_add_rms_norm(const void* x, const void* delta, void* x_out, void* y, cons
 int hs_rotary_split(const void* qkv, int64_t qkv_stride, void* q, void* k, void* v, const int64_t* positions,
                     int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, float theta, int32_t dtype,
                     hs_stream_t stream);
+int hs_norm_rotary_split(const void* qkv, int64_t qkv_stride, const void* q_weight, const void* k_weight, float eps,
+                         void* q, void* k, void* v, const int64_t* positions, int64_t rows, int64_t heads,
+                         int64_t kv_heads, int64_t head_dim, double theta, int32_t dtype, hs_stream_t stream);
 int hs_silu_mul(const void* gate_up, int64_t gu_stride, void* out, int64_t out_stride, int64_t rows,
                 int64_t width, int32_t dtype, hs_stream_t stream);
 

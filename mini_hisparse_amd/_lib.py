@@ -6,13 +6,14 @@ no fallback: when the library is missing every kernel call raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
-from ctypes import c_uint64, POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import c_uint64, POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
 from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libhisparse_hip.so"
 
-HS_DTYPE_F32, HS_DTYPE_F16, HS_DTYPE_BF16 = 0, 1, 2
+HS_DTYPE_F32, HS_DTYPE_F16, HS_DTYPE_BF16, HS_DTYPE_I8, HS_DTYPE_E4M3 = 0, 1, 2, 3, 4
 
 
 class HipLibraryError(RuntimeError):
@@ -130,6 +131,30 @@ SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
          c_float, c_int32, c_void_p],
     ),
+    "hs_norm_rotary_split": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+         c_int64, c_int64, c_double, c_int32, c_void_p],
+    ),
+    "hs_append_quantized": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p,
+         c_int32, c_int64, c_int64, c_int64, c_int64, c_void_p],
+    ),
+    "hs_read_quantized": (
+        c_int,
+        [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+         c_int32, c_void_p],
+    ),
+    "hs_attend_pages_workspace_bytes": (
+        c_int64, [c_int32, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64],
+    ),
+    "hs_attend_pages": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64,
+         c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+         c_int64, c_void_p],
+    ),
     "hs_silu_mul": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p]),
     "hs_uniform_pages": (
         c_int, [c_uint64, c_uint64, POINTER(c_int64), c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p],
@@ -217,6 +242,16 @@ def dtype_code(dtype) -> int:
     return codes[dtype]
 
 
+def cache_code(dtype) -> int:
+    """Element code of a quantised pool's codes."""
+    import torch
+
+    codes = {torch.int8: HS_DTYPE_I8, torch.float8_e4m3fn: HS_DTYPE_E4M3}
+    if dtype not in codes:
+        raise ValueError("cache codes must be int8 or float8_e4m3fn")
+    return codes[dtype]
+
+
 def ptr(tensor) -> int:
     return 0 if tensor is None else tensor.data_ptr()
 
@@ -236,3 +271,14 @@ def stream_handle(device=None) -> int:
     if index is None:
         index = torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which ``device`` (a tensor's) is the current device: a kernel is launched
+    on a stream of the current device only.  Free where it is current already."""
+    import torch
+
+    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)

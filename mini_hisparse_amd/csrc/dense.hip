@@ -11,12 +11,14 @@
 //   add_rms_norm   x <- x + delta (in the model dtype), y = RMSNorm(x)
 //   rotary_split   fused q|k|v projection output -> rotated q, rotated k, v
 //   silu_mul       fused gate|up projection output -> silu(gate) * up
+//   norm_rotary_split  rotary_split with a per-head RMSNorm of q and k before the rotation
 //
 // Rounding follows the PyTorch ops they replace: the residual add rounds to
 // the model dtype; RMSNorm squares and averages in fp32, rounds x * rsqrt to
 // the model dtype and multiplies by the weight in that dtype; rotary rounds
 // cos/sin, each product and the sum to the model dtype; SiLU rounds its fp32
-// result before the product with `up`.  Only the fp32 sum order of the norm
+// result before the product with `up`; norm_rotary_split has no chain of ops to follow
+// and rounds its fp32 result once.  Only the fp32 sum order of the norm
 // and the device's transcendental functions differ from PyTorch's.
 #include <math.h>
 
@@ -170,6 +172,138 @@ __global__ __launch_bounds__(DN_T) void rotary_split_kernel(const void* qkv, int
   }
 }
 
+// Per-head RMS norm of q and k, then the rotary embedding, with the split of a packed
+// q|k|v row: for a q or k head vector x with norm weight w,
+//
+//   n_d = x_d rsqrt(mean(x^2) + eps) w_d,
+//   (y_i, y_{i+D/2}) = (n_i cos a - n_{i+D/2} sin a, n_{i+D/2} cos a + n_i sin a),
+//   a = position * theta^(-2i/D),
+//
+// in fp32, rounded once.  The angle is reduced to a part of one turn in 64 bits: at
+// position 10^5 an fp32 angle is off by up to 4e-3, more than a bf16 step of the result.
+// A head vector is held by `lanes` lanes of NH_E pairs each (D = 128: 16 lanes of 4), so
+// both halves of a pair meet in one lane and the norm's sum is a butterfly within the
+// lanes.  A workgroup takes `brows` rows: its threads first fill the rows' cos/sin table in
+// LDS (one 64-bit reduction per row and pair, shared by all heads), then walk the rows' heads.
+constexpr int NH_E = 4;      // rotation pairs per lane
+constexpr int NH_TAB = 512;  // cos/sin pairs of a workgroup's table
+
+struct NormRotaryArgs {
+  const void *qkv, *wq, *wk;
+  void *q, *k, *v;
+  const int64_t* positions;
+  int64_t qkv_stride, rows, heads, kv_heads;
+  double log2_theta;
+  float eps;
+  int D, lanes_log2, brows;
+};
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void load_pairs(const void* base, int64_t at, int lane, int lanes, int half,
+                                           float (&x)[NH_E]) {
+  if constexpr (VEC) {
+    const bool in = lane * NH_E < half;
+    const int64_t i = at + (in ? lane * NH_E : 0);
+    if constexpr (DT == HS_DTYPE_F32) {
+      const f32x4 w = *reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + i);
+#pragma unroll
+      for (int e = 0; e < NH_E; ++e) x[e] = in ? w[e] : 0.f;
+    } else {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const unsigned short*>(base) + i);
+#pragma unroll
+      for (int e = 0; e < NH_E; ++e) {
+        const unsigned short b = static_cast<unsigned short>((in ? w[e >> 1] : 0u) >> (16 * (e & 1)));
+        x[e] = DT == HS_DTYPE_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < NH_E; ++e) {
+      const int i = lane + lanes * e;
+      x[e] = i < half ? load_elem<DT>(base, at + i) : 0.f;
+    }
+  }
+}
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void store_pairs(void* base, int64_t at, int lane, int lanes, int half,
+                                            const float (&x)[NH_E]) {
+  if constexpr (VEC) {
+    if (lane * NH_E >= half) return;
+    const int64_t i = at + lane * NH_E;
+    if constexpr (DT == HS_DTYPE_F32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(base) + i) = f32x4{x[0], x[1], x[2], x[3]};
+    } else {
+      u32x2 w;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        w[e] = DT == HS_DTYPE_BF16
+                   ? f32_to_bf16_bits(x[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(x[2 * e + 1])) << 16
+                   : f32_to_f16_bits(x[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(x[2 * e + 1])) << 16;
+      *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(base) + i) = w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < NH_E; ++e) {
+      const int i = lane + lanes * e;
+      if (i < half) store_elem<DT>(base, at + i, x[e]);
+    }
+  }
+}
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(DN_T) void norm_rotary_split_kernel(NormRotaryArgs a) {
+  __shared__ float s_cos[NH_TAB], s_sin[NH_TAB];
+  const int half = a.D / 2, lanes = 1 << a.lanes_log2;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.brows;
+  const int nrows = static_cast<int>(a.rows - row0 < a.brows ? a.rows - row0 : a.brows);
+  for (int t = threadIdx.x; t < nrows * half; t += DN_T) {
+    const int r = t / half, i = t - r * half;
+    // turns = position * theta^(-2i/D) / 2 pi
+    const double turns = static_cast<double>(a.positions[row0 + r]) *
+                         (exp2(-(2.0 * i / a.D) * a.log2_theta) * 0.15915494309189535);
+    float s, c;
+    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+    s_cos[t] = c;
+    s_sin[t] = s;
+  }
+  __syncthreads();
+  const int64_t H = a.heads, K = a.kv_heads, total = H + 2 * K;
+  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> a.lanes_log2, groups = DN_T >> a.lanes_log2;
+  const int64_t tasks = nrows * total;
+  for (int64_t t = static_cast<int64_t>(blockIdx.y) * groups + group; t < tasks;
+       t += static_cast<int64_t>(gridDim.y) * groups) {
+    const int64_t r = t / total, h = t - r * total;
+    const int64_t row = row0 + r;
+    const int64_t src = row * a.qkv_stride + h * a.D;
+    float lo[NH_E], hi[NH_E];
+    load_pairs<DT, VEC>(a.qkv, src, lane, lanes, half, lo);
+    load_pairs<DT, VEC>(a.qkv, src + half, lane, lanes, half, hi);
+    void* dst = h < H ? a.q : (h < H + K ? a.k : a.v);
+    const int64_t to = (h < H ? row * H + h : (h < H + K ? row * K + h - H : row * K + h - H - K)) * a.D;
+    if (h < H + K) {  // one condition for all lanes of the head
+      float wl[NH_E], wh[NH_E], sq = 0.f;
+      const void* w = h < H ? a.wq : a.wk;
+      load_pairs<DT, VEC>(w, 0, lane, lanes, half, wl);
+      load_pairs<DT, VEC>(w, half, lane, lanes, half, wh);
+#pragma unroll
+      for (int e = 0; e < NH_E; ++e) sq += lo[e] * lo[e] + hi[e] * hi[e];
+      for (int off = lanes >> 1; off > 0; off >>= 1) sq += __shfl_xor(sq, off, 64);
+      const float norm = rsqrtf(sq / static_cast<float>(a.D) + a.eps);
+#pragma unroll
+      for (int e = 0; e < NH_E; ++e) {
+        const int i = VEC ? lane * NH_E + e : lane + lanes * e;
+        const int at = i < half ? static_cast<int>(r) * half + i : 0;
+        const float x = lo[e] * norm * wl[e], y = hi[e] * norm * wh[e], c = s_cos[at], s = s_sin[at];
+        lo[e] = x * c - y * s;
+        hi[e] = y * c + x * s;
+      }
+    }
+    store_pairs<DT, VEC>(dst, to, lane, lanes, half, lo);
+    store_pairs<DT, VEC>(dst, to + half, lane, lanes, half, hi);
+  }
+}
+
 // out[row, j] = silu(gate[row, j]) * up[row, j] with gate = gate_up[row, :width],
 // up = gate_up[row, width:].
 template <int DT>
@@ -220,6 +354,54 @@ extern "C" int hs_rotary_split(const void* qkv, int64_t qkv_stride, void* q, voi
   HS_DENSE_DISPATCH(dtype, rotary_split_kernel, dim3(static_cast<unsigned>(heads + 2 * kv_heads), static_cast<unsigned>(rows)),
                     dim3(threads), stream, qkv, qkv_stride, q, k, v, positions, heads, kv_heads, head_dim, theta);
   HS_CHECK_LAUNCH("rotary_split");
+  return HS_OK;
+}
+
+extern "C" int hs_norm_rotary_split(const void* qkv, int64_t qkv_stride, const void* q_weight, const void* k_weight,
+                                    float eps, void* q, void* k, void* v, const int64_t* positions, int64_t rows,
+                                    int64_t heads, int64_t kv_heads, int64_t head_dim, double theta, int32_t dtype,
+                                    hipStream_t stream) {
+  HS_CHECK_ARG(valid_dtype(dtype), "invalid dtype code %d", dtype);
+  HS_CHECK_ARG(rows >= 1 && heads >= 1 && kv_heads >= 1 && head_dim >= 2 && head_dim % 2 == 0 && head_dim <= 512,
+               "invalid normed rotary shape");
+  HS_CHECK_ARG(rows <= 0x7fffffff && heads <= 0xffff && kv_heads <= 0xffff, "too many rows or heads in one call");
+  HS_CHECK_ARG(qkv_stride >= (heads + 2 * kv_heads) * head_dim, "q|k|v row stride below its width");
+  HS_CHECK_ARG(qkv && q_weight && k_weight && q && k && v && positions, "null normed rotary pointer");
+  HS_CHECK_ARG(theta > 0.0 && isfinite(theta) && eps >= 0.f, "theta must be positive and eps not negative");
+  const int half = static_cast<int>(head_dim / 2);
+  const uintptr_t bytes = NH_E * elem_bytes(dtype);  // a lane's vector
+  const uintptr_t all = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_weight) |
+                        reinterpret_cast<uintptr_t>(k_weight) | reinterpret_cast<uintptr_t>(q) |
+                        reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
+  const bool vec = half % NH_E == 0 && qkv_stride % NH_E == 0 && all % bytes == 0;
+  NormRotaryArgs a{qkv, q_weight, k_weight, q, k, v, positions, qkv_stride, rows, heads, kv_heads, log2(theta), eps,
+                   static_cast<int>(head_dim), 6, 1};
+  if (vec) {
+    a.lanes_log2 = 0;
+    while ((NH_E << a.lanes_log2) < half) ++a.lanes_log2;
+  }
+  const int64_t groups = DN_T >> a.lanes_log2, total = heads + 2 * kv_heads;
+  // Rows per workgroup: as many as give every thread one cos/sin pair, once that still
+  // leaves two workgroups per CU; fewer rows go one to a workgroup, their heads spread.
+  const int64_t fill = DN_T / half > 1 ? DN_T / half : 1;
+  a.brows = rows >= 512 * fill ? static_cast<int>(fill) : 1;
+  int64_t spread = 1;
+  if (rows < 512) {
+    spread = (total + groups - 1) / groups;
+    const int64_t most = (512 + rows - 1) / rows;
+    if (spread > most) spread = most;
+  }
+  const dim3 grid(static_cast<unsigned>((rows + a.brows - 1) / a.brows), static_cast<unsigned>(spread));
+  if (vec) {
+    if (dtype == HS_DTYPE_BF16) hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_BF16, true>), grid, dim3(DN_T), 0, stream, a);
+    else if (dtype == HS_DTYPE_F16) hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_F16, true>), grid, dim3(DN_T), 0, stream, a);
+    else hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_F32, true>), grid, dim3(DN_T), 0, stream, a);
+  } else {
+    if (dtype == HS_DTYPE_BF16) hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_BF16, false>), grid, dim3(DN_T), 0, stream, a);
+    else if (dtype == HS_DTYPE_F16) hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_F16, false>), grid, dim3(DN_T), 0, stream, a);
+    else hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_F32, false>), grid, dim3(DN_T), 0, stream, a);
+  }
+  HS_CHECK_LAUNCH("norm_rotary_split");
   return HS_OK;
 }
 

@@ -9,6 +9,8 @@ RMSNorm (with the residual add before it), the rotary embedding of q and k
 (over a packed gate|up projection) of the Qwen2 layer that ``MiniModel``
 implements (model.py:53-57 RMSNorm, the rotary and MLP of this package's
 ``model.py``; the reference's model.py:183-226).  One launch each for B rows.
+``norm_rotary_split`` (``hs_norm_rotary_split``) is ``rotary_split`` with a per-head
+RMSNorm of q and k before the rotation.
 """
 
 from __future__ import annotations
@@ -321,6 +323,61 @@ def prepare_rotary_split(qkv, positions, heads, kv_heads, head_dim, theta, out):
     if out is None:
         raise ValueError("prepare_rotary_split writes into a given out")
     return _rotary_launch(qkv, positions, heads, kv_heads, head_dim, theta, *out)
+
+
+def _norm_rotary_check(qkv, q_weight, k_weight, positions, heads, kv_heads, head_dim, out):
+    if heads < 1 or kv_heads < 1 or head_dim < 2 or head_dim % 2 or head_dim > 512:
+        raise ValueError("norm_rotary_split takes positive head counts and an even head_dim of at most 512")
+    if qkv.dim() != 2 or qkv.shape[0] < 1:
+        raise ValueError("qkv must be [rows, (heads + 2 kv_heads) head_dim] with at least one row")
+    if qkv.stride(0) < qkv.shape[1] and qkv.shape[0] > 1:
+        raise ValueError("qkv rows must not overlap")
+    _rotary_check(qkv, positions, heads, kv_heads, head_dim, out)
+    if not positions.is_contiguous():
+        raise ValueError("positions must be contiguous")
+    for name, weight in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if (weight.shape != (head_dim,) or weight.dtype != qkv.dtype or weight.device != qkv.device
+                or not weight.is_contiguous()):
+            raise ValueError(f"{name} must be [head_dim] contiguous in the dtype and on the device of qkv")
+    if qkv.device.type != "cuda":
+        raise ValueError("norm_rotary_split needs ROCm device tensors (HIP kernels only)")
+
+
+def _norm_rotary_launch(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, q, k, v):
+    return Launch(_lib.load().hs_norm_rotary_split,
+                  (qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), q_weight.data_ptr(), k_weight.data_ptr(),
+                   float(eps), q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), qkv.shape[0], heads,
+                   kv_heads, head_dim, float(theta), _lib.dtype_code(qkv.dtype)),
+                  "hs_norm_rotary_split")
+
+
+def norm_rotary_split(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, out=None):
+    """:func:`rotary_split` for decoders that norm their heads: every q and k head vector is
+    RMS-normed over ``head_dim`` (``eps``, weights ``q_weight`` / ``k_weight`` [head_dim]),
+    then rotated; v is copied.  Any number of rows (a prompt or a decode batch).  Computed
+    in float32, angles in 64 bits, and rounded once (``rotary_split`` rounds after every op
+    of the model's chain, and its angles are float32)."""
+    _norm_rotary_check(qkv, q_weight, k_weight, positions, heads, kv_heads, head_dim, out)
+    rows = qkv.shape[0]
+    if out is None:
+        q = torch.empty((rows, heads, head_dim), dtype=qkv.dtype, device=qkv.device)
+        k = torch.empty((rows, kv_heads, head_dim), dtype=qkv.dtype, device=qkv.device)
+        v = torch.empty_like(k)
+    else:
+        q, k, v = out
+    with _lib.on_device(qkv.device):
+        _norm_rotary_launch(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, q, k,
+                            v)(_stream(qkv))
+    return q, k, v
+
+
+def prepare_norm_rotary_split(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, out):
+    """:func:`norm_rotary_split` into ``out`` = (q, k, v), bound once (``positions`` is read
+    when the launch runs)."""
+    _norm_rotary_check(qkv, q_weight, k_weight, positions, heads, kv_heads, head_dim, out)
+    if out is None:
+        raise ValueError("prepare_norm_rotary_split writes into a given out")
+    return _norm_rotary_launch(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, *out)
 
 
 def _silu_check(gate_up, out):

@@ -1,0 +1,395 @@
+"""Attention over page tables (attend_pages) against softmax attention in 64 bits, with every
+row it may not use filled with NaN, and the calls it refuses."""
+
+import ctypes
+
+import pytest
+import torch
+
+from mini_hisparse_amd import _lib
+from mini_hisparse_amd.quantized import QuantizedPool, append_quantized
+from mini_hisparse_amd.row_kernels import attend_pages, attend_rows
+
+PLAIN = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+CODES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+def rows_of(values, code):
+    """(codes or plain values, scales or None) of random rows [blocks, 2, P, Hkv, D]."""
+    if code in PLAIN:
+        return values.to(PLAIN[code]), None
+    top = 127.0 if code == "int8" else 448.0
+    scales = values.abs().amax(-1) / top
+    q = values / scales[..., None]
+    return (q.round() if code == "int8" else q).clamp(-top, top).to(CODES[code]), scales
+
+
+def case(batch, heads, kv, dim, page, lengths, code, dtype, device, seed=0, absent=0.0, per_head=False, spare=3,
+         amplitude=1.0):
+    """A batch whose tables are scattered over the pool.  Rows no request may use -- past a
+    length, of blocks in no table -- are NaN (for int8 codes: NaN scales and any codes)."""
+    gen = torch.Generator().manual_seed(seed + dim + page + sum(lengths))
+    lists = kv if per_head else 1
+    pages = [-(-n // page) for n in lengths]
+    width = max(1, max(pages)) + 2
+    blocks = lists * sum(pages) + spare
+    order = torch.randperm(blocks, generator=gen)
+    tables = torch.randint(-3, blocks + 3, (batch, lists, width), generator=gen)  # past the pages: anything
+    values = torch.randn(blocks, 2, page, kv, dim, generator=gen)
+    values[..., : max(1, dim // 50)] *= 8
+    values[:, 1] *= amplitude
+    used = torch.zeros(blocks, page, kv, dtype=torch.bool)
+    taken = 0
+    for b, n in enumerate(lengths):
+        for h in range(lists):
+            mine = order[taken : taken + pages[b]]
+            taken += pages[b]
+            tables[b, h, : pages[b]] = mine
+            for i, block in enumerate(mine.tolist()):
+                gone = absent and torch.rand((), generator=gen).item() < absent
+                if gone:
+                    tables[b, h, i] = [-1, blocks, -(2**31), 2**31 - 1][i % 4]
+                elif per_head:
+                    used[block, : n - i * page, h] = True
+                else:
+                    used[block, : n - i * page] = True
+    stored, scales = rows_of(values, code)
+    junk = ~used[:, None].expand(-1, 2, -1, -1)
+    if scales is None:
+        stored[junk] = float("nan")
+    else:
+        scales[junk] = float("nan")
+        raw = stored.view(torch.int8)
+        raw[junk] = 0x7F  # e4m3's NaN, int8's 127
+    query = torch.randn(batch, heads, dim, generator=gen).to(PLAIN[dtype])
+    tables = tables.to(torch.int32) if per_head else tables[:, 0].to(torch.int32)
+    pool = stored.to(device) if scales is None else QuantizedPool(stored.to(device), scales.to(device))
+    return query.to(device), pool, tables.to(device), torch.tensor(lengths, dtype=torch.int32, device=device)
+
+
+def store_of(pool):
+    """The pool's values in 64 bits."""
+    if not isinstance(pool, QuantizedPool):
+        return pool.cpu().double()
+    return pool.codes.cpu().float().double() * pool.scales.cpu().double()[..., None]
+
+
+def formula(query, pool, tables, lengths):
+    """(out, weighted sum of |V|, largest sum of |q K| D^-1/2, largest |score|, tokens) in 64 bits."""
+    store = store_of(pool)
+    query, tables, lengths = query.cpu().double(), tables.cpu().long(), lengths.cpu().tolist()
+    blocks, _, page, kv, dim = store.shape
+    batch, heads, _ = query.shape
+    group = heads // kv
+    out, weight, size, top, count = (torch.zeros(batch, heads, n, dtype=torch.float64) for n in (dim, dim, 1, 1, 1))
+    for b, n in enumerate(lengths):
+        n = max(0, min(n, tables.shape[-1] * page))
+        token = torch.arange(n)
+        for h in range(kv):
+            table = tables[b, h] if tables.dim() == 3 else tables[b]
+            block = table[token // page]
+            keep = (block >= 0) & (block < blocks)
+            if not keep.any():
+                continue
+            k, v = (store[block[keep], plane, (token % page)[keep], h] for plane in (0, 1))
+            rows = slice(h * group, (h + 1) * group)
+            q = query[b, rows]
+            scores = q @ k.T * dim**-0.5
+            p = torch.softmax(scores, -1)
+            out[b, rows], weight[b, rows] = p @ v, p @ v.abs()
+            size[b, rows] = (q.abs() @ k.abs().T).amax(-1, keepdim=True) * dim**-0.5
+            top[b, rows] = scores.abs().amax(-1, keepdim=True)
+            count[b, rows] = float(keep.sum())
+    return out, weight, size, top, count
+
+
+def check(got, args):
+    """|error| <= half a step of the dtype, and before that rounding the weights' error times
+    the weighted |V| twice (numerator and sum): with u = 2^-24, a score is off by at most
+    D u of its sum of magnitudes, three roundings of the score and 4 u of its size again in
+    the exponential's argument; the exponential by 4 u; the sums of n tokens and their
+    rescalings by (n + 16) u; a weight held in 16 bits by half a step of its type.  A
+    quantised pool's weights are held in two bf16 parts (2^-17), three for float32."""
+    query, pool = args[0], args[1]
+    want, weight, size, top, count = formula(*args)
+    u, dim = 2.0**-24, query.shape[-1]
+    quantized = isinstance(pool, QuantizedPool)
+    held = 2.0**-17 if quantized else 0.0
+    if not quantized and query.dtype != torch.float32:
+        held = torch.finfo(query.dtype).eps / 2
+    if quantized and query.dtype == torch.float32:
+        held = 2.0**-24
+    weights = (dim + 4) * u * size + 8 * u * top + 4 * u + (count + 16) * u + held
+    tol = torch.finfo(query.dtype).eps / 2 * want.abs() + 2 * weights * weight
+    # float32 has no normal value below 2^-126 and no value below 2^-149: a weight smaller
+    # than 2^-126 of the largest may be held as 0, so each of the n tokens may miss 2^-126 of
+    # the largest |V| (q of 1000 sigma: the true output is 1e-45 where the winner's V is 0)
+    largest = (store_of(pool).nan_to_num(0.0).abs().amax()).item()
+    tol = tol + count * 2.0**-126 * largest
+    if query.dtype == torch.float16:
+        tol = tol + 2.0**-25
+    error = (got.double().cpu() - want).abs()
+    over = error > tol
+    assert not over.any(), (error[over].max().item(), tol[over].max().item())
+
+
+SHAPES = [(28, 4, 128), (14, 2, 64), (4, 2, 32), (8, 8, 128), (16, 1, 128), (20, 1, 64), (36, 1, 128), (12, 3, 96),
+          (5, 5, 80), (3, 1, 256), (2, 2, 512), (2, 1, 20), (3, 3, 7), (1, 1, 1), (22, 11, 64)]
+POOLS = [("int8", "bf16"), ("e4m3", "bf16"), ("int8", "f16"), ("e4m3", "f16"), ("int8", "f32"), ("e4m3", "f32"),
+         ("bf16", "bf16"), ("f16", "f16"), ("f32", "f32")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", POOLS)
+@pytest.mark.parametrize("heads,kv,dim", SHAPES)
+def test_matches_the_formula(gpu, heads, kv, dim, code, dtype):
+    args = case(3, heads, kv, dim, 16, [333, 1, 97], code, dtype, gpu)
+    check(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("e4m3", "f32"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("page", [1, 3, 8, 12, 16, 32, 48, 64, 256])
+def test_page_sizes(gpu, page, code, dtype):
+    args = case(2, 14, 2, 64, page, [401, 256], code, dtype, gpu)
+    check(attend_pages(*args), args)
+    args = case(1, 8, 4, 128, page, [63], code, dtype, gpu)
+    check(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("e4m3", "f16"), ("f16", "f16"), ("f32", "f32")])
+def test_lengths_around_the_tiles(gpu, code, dtype):
+    """Lengths on both sides of a page, a tile and a split, and none at all."""
+    for lengths in ([0], [1], [2], [15, 16, 17], [31, 32, 33], [63, 64, 65, 0, 127, 128, 129], [255, 0, 256, 257],
+                    [511, 512, 513], [2047, 2048, 2049], [4000, 3, 0]):
+        args = case(len(lengths), 8, 2, 128, 16, lengths, code, dtype, gpu)
+        got = attend_pages(*args)
+        check(got, args)
+        for b, n in enumerate(lengths):
+            assert n or (got[b] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("e4m3", "bf16"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("page", [16, 5])
+def test_absent_pages_and_tables_per_head(gpu, page, code, dtype):
+    for per_head in (False, True):
+        for absent in (0.0, 0.4, 1.0):
+            args = case(3, 14, 2, 64, page, [700, 33, 16], code, dtype, gpu, absent=absent, per_head=per_head)
+            got = attend_pages(*args)
+            check(got, args)
+            assert absent < 1.0 or (got == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", ["int8", "bf16"])
+def test_uneven_batches(gpu, code):
+    """One long history among many short ones, and the other way round."""
+    for lengths in ([9000] + [5] * 20, [3000] * 5 + [0, 1], [40] * 70):
+        args = case(len(lengths), 14, 2, 64, 16, lengths, code, "bf16", gpu)
+        check(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("int8", "f16"), ("e4m3", "f32")])
+def test_small_and_large_values(gpu, code, dtype):
+    """V rows of any size: the weights times a scale keep their precision (float16 queries too)."""
+    for amplitude in (1e-6, 1e-3, 2000.0):
+        args = case(2, 8, 2, 128, 16, [300, 1], code, dtype, gpu, amplitude=amplitude)
+        check(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+def test_sharp_and_flat_scores(gpu):
+    for size in (0.0, 30.0, 1000.0):
+        args = case(2, 28, 4, 128, 16, [500, 77], "int8", "f32", gpu)
+        args = (args[0] * size, *args[1:])
+        check(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", POOLS)
+def test_nan_in_a_used_row_reaches_its_heads_alone(gpu, code, dtype):
+    for dim in (64, 96):
+        query, pool, tables, lengths = case(2, 4, 2, dim, 16, [40, 40], code, dtype, gpu)
+        block = tables[0, 1].item()
+        (pool.scales if code in CODES else pool)[block, 0, 3, 1] = float("nan")  # a key of request 0, KV head 1
+        got = attend_pages(query, pool, tables, lengths)
+        assert got[0, 2:].isnan().all() and got[0, :2].isfinite().all() and got[1].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_lengths_past_the_tables_and_below_zero(gpu):
+    query, pool, tables, lengths = case(2, 4, 2, 64, 16, [64, 48], "int8", "bf16", gpu, spare=1)
+    tables = tables[:, :3].contiguous()  # 48 tokens at most
+    want = attend_pages(query, pool, tables, torch.tensor([48, 48], dtype=torch.int32, device=gpu))
+    got = attend_pages(query, pool, tables, torch.tensor([2**31 - 1, 49], dtype=torch.int32, device=gpu))
+    assert torch.equal(got, want)
+    none = attend_pages(query, pool, tables, torch.tensor([-1, -(2**31)], dtype=torch.int32, device=gpu))
+    assert (none == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("bf16", "bf16"), ("f32", "f32")])
+def test_strides_outputs_and_misaligned_buffers(gpu, code, dtype):
+    query, pool, tables, lengths = case(3, 8, 2, 64, 16, [100, 7, 50], code, dtype, gpu)
+    want = attend_pages(query, pool, tables, lengths)
+    wide = torch.zeros(3, 8, 100, dtype=query.dtype, device=gpu)
+    wide[..., 3:67] = query
+    assert torch.equal(attend_pages(wide[..., 3:67], pool, tables, lengths), want)
+    turned = query.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(attend_pages(turned, pool, tables, lengths), want)
+    assert torch.equal(attend_pages(query.repeat_interleave(2, 2)[..., ::2], pool, tables, lengths), want)
+    spread = torch.full((3, 2 * tables.shape[1]), 7, dtype=torch.int32, device=gpu)
+    spread[:, : tables.shape[1]] = tables
+    assert torch.equal(attend_pages(query, pool, spread[:, : tables.shape[1]], lengths), want)
+    shared = tables[:, None].expand(-1, 2, -1)  # the same list for both KV heads
+    assert torch.equal(attend_pages(query, pool, shared, lengths), want)
+    guarded = torch.full((5, 8, 64), 9.0, dtype=query.dtype, device=gpu)
+    got = attend_pages(query, pool, tables, lengths, out=guarded[1:4])
+    assert got.data_ptr() == guarded[1].data_ptr() and torch.equal(got, want)
+    assert (guarded[0] == 9).all() and (guarded[4] == 9).all()
+    # a pool that starts at an odd element: same result from the element-wise kernel
+    store = pool.codes if code in CODES else pool
+    room = torch.empty(store.numel() + 1, dtype=torch.int8 if code in CODES else store.dtype, device=gpu)
+    moved = room[1:].view(store.shape)
+    moved.copy_(store.view(room.dtype))
+    moved = QuantizedPool(moved.view(store.dtype), pool.scales) if code in CODES else moved
+    args = (query, moved, tables, lengths)
+    check(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("f32", "f32")])
+def test_one_request_of_a_batch_does_not_change_another(gpu, code, dtype):
+    """The same request gives the same bits twice, alone or beside others of its length."""
+    args = case(4, 14, 2, 64, 16, [900, 900, 900, 900], code, dtype, gpu)
+    first, again = attend_pages(*args), attend_pages(*args)
+    assert torch.equal(first, again)
+
+
+@pytest.mark.gpu
+def test_pool_past_32_bit_offsets(gpu):
+    blocks, page, kv, dim = 140_000, 16, 8, 128  # 4.6e9 codes
+    pool = QuantizedPool.empty(blocks, page, kv, dim, torch.int8, gpu)
+    tables = torch.tensor([[blocks - 1, 70_000], [65_537, 131_073]], dtype=torch.int32, device=gpu)
+    lengths = torch.tensor([29, 32], dtype=torch.int32, device=gpu)
+    rows = (tables.long()[:, :, None] * page + torch.arange(page, device=gpu)).flatten()
+    k, v = (torch.randn(len(rows), kv, dim, device=gpu) for _ in range(2))
+    append_quantized(k, v, rows, pool)
+    query = torch.randn(2, 16, dim, device=gpu).to(torch.bfloat16)
+    got = attend_pages(query, pool, tables, lengths)
+    order = torch.tensor([[2, 1], [0, 3]], dtype=torch.int32, device=gpu)  # the same rows in a small pool
+    small = QuantizedPool(*(t[tables.long()[[1, 0, 0, 1], [0, 1, 0, 1]]].contiguous()
+                            for t in (pool.codes, pool.scales)))
+    args = (query, small, order, lengths)
+    check(got, args)
+
+
+@pytest.mark.gpu
+def test_agrees_with_attend_rows(gpu):
+    """The same rows by page table and by row list, over one plain pool."""
+    from mini_hisparse_amd.config import CacheConfig
+
+    query, pool, tables, lengths = case(2, 28, 4, 128, 16, [320, 320], "bf16", "bf16", gpu)
+    config = CacheConfig(gpu_pages=pool.shape[0], page_size=16, kv_heads=4, head_dim=128, device=gpu,
+                         dtype=torch.bfloat16)
+    rows = (tables.long()[:, :20, None] * 16 + torch.arange(16, device=gpu)).flatten(1)
+    by_rows = attend_rows(query, pool, rows, config)
+    args = (query, pool, tables, lengths)
+    check(by_rows, args)
+    check(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("bf16", "bf16"), ("f32", "f32")])
+def test_streams_and_captured_replays(gpu, code, dtype):
+    """Calls at once on two streams, and captured calls replayed with other tables, lengths and
+    queries, with eager calls between the replays; two graphs replayed at once."""
+    a = case(3, 14, 2, 64, 16, [2000, 1300, 5], code, dtype, gpu)
+    b = case(2, 14, 2, 64, 16, [1500, 900], code, dtype, gpu, seed=1)
+    want_a, want_b = attend_pages(*a), attend_pages(*b)
+    main = torch.cuda.current_stream(torch.device(gpu))
+    streams = [torch.cuda.Stream(torch.device(gpu)) for _ in range(2)]
+    for s in streams:
+        s.wait_stream(main)
+    results = []
+    for _ in range(4):
+        for s, args in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                results.append(attend_pages(*args))
+    for s in streams:
+        main.wait_stream(s)
+    for i, r in enumerate(results):
+        assert torch.equal(r, (want_a, want_b)[i % 2])
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for graph, args in zip(graphs, (a, b)):
+        with torch.cuda.graph(graph):
+            outs.append(attend_pages(*args))
+    for step in range(4):
+        a[3][0] -= 301 * step  # shorter histories
+        b[0].normal_()
+        want_a, want_b = attend_pages(*a), attend_pages(*b)
+        for s in streams:
+            s.wait_stream(main)
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        for s in streams:
+            main.wait_stream(s)
+        assert torch.equal(outs[0], want_a) and torch.equal(outs[1], want_b)
+
+
+def test_refusals_without_a_gpu():
+    pool = QuantizedPool.empty(4, 16, 2, 8, torch.int8, "cpu")
+    plain = torch.zeros(4, 2, 16, 2, 8)
+    query = torch.zeros(3, 4, 8)
+    tables, lengths = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    bad = [
+        ("query", (query[0], pool, tables, lengths)),
+        ("query", (query, pool.codes[0], tables, lengths)),
+        ("head_dim", (query[..., :4], pool, tables, lengths)),
+        ("multiple", (query[:, :3], pool, tables, lengths)),
+        ("query", (query[:0], pool, tables[:0], lengths[:0])),
+        ("dtype", (query.double(), pool, tables, lengths)),
+        ("query dtype", (query.half(), plain, tables, lengths)),
+        ("contiguous", (query, plain.transpose(2, 3).contiguous().transpose(2, 3), tables, lengths)),
+        ("tables", (query, pool, tables.long(), lengths)),
+        ("tables", (query, pool, tables[:2], lengths)),
+        ("tables", (query, pool, tables[:, :0], lengths)),
+        ("tables", (query, pool, tables.repeat(1, 2)[:, ::2], lengths)),
+        ("tables", (query, pool, tables[:, None].expand(-1, 3, -1), lengths)),
+        ("lengths", (query, pool, tables, lengths.long())),
+        ("lengths", (query, pool, tables, lengths[:2])),
+        ("lengths", (query, pool, tables, lengths.repeat(2)[::2])),
+        ("ROCm", (query, pool, tables, lengths)),
+    ]
+    for match, args in bad:
+        with pytest.raises(ValueError, match=match):
+            attend_pages(*args)
+    with pytest.raises(ValueError, match="out"):
+        attend_pages(query, pool, tables, lengths, out=torch.zeros(3, 4, 16)[..., ::2])
+
+
+def test_entry_point_refusals_without_a_gpu():
+    lib = _lib.load()
+    buffer = ctypes.create_string_buffer(256)
+    at = ctypes.addressof(buffer)
+    at += -at % 16
+
+    def call(q=at, qd=2, pool=at, scales=at, code=3, blocks=4, page=16, kv=1, dim=64, tables=at, pages=1, lengths=at,
+             batch=1, heads=2, out=at, ws=at, nbytes=1 << 40):
+        return lib.hs_attend_pages(q, heads * dim, dim, qd, pool, scales, code, blocks, page, kv, dim, tables, pages,
+                                   0, pages, lengths, batch, heads, out, heads * dim, dim, ws, nbytes, None)
+
+    for bad in (dict(q=None), dict(qd=3), dict(pool=None), dict(scales=None), dict(code=2), dict(code=5), dict(code=0),
+                dict(blocks=0), dict(blocks=2**31), dict(page=0), dict(kv=0), dict(kv=3), dict(dim=0), dict(dim=513),
+                dict(tables=None), dict(pages=0), dict(pages=2**31), dict(page=2**20, pages=2**12), dict(lengths=None),
+                dict(batch=0), dict(batch=70_000), dict(heads=0), dict(out=None), dict(ws=None), dict(nbytes=16),
+                dict(ws=at + 4)):
+        assert call(**bad) == -1, bad
+        assert lib.hs_last_error()
+    size = lib.hs_attend_pages_workspace_bytes
+    assert size(2, 3, 0, 1, 1, 64, 16, 1) == 256 and size(2, 3, 4, 14, 2, 64, 16, 100) > 0
