@@ -17,6 +17,9 @@
 // factor log2(e), so every exponential is a power of two.
 #include <math.h>
 
+#include <type_traits>
+
+#include "arrive.h"
 #include "codes.h"
 
 namespace hs {
@@ -43,8 +46,13 @@ struct PagesArgs {
   float *part_m, *part_l, *part_o;  // [slots, Hq], [slots, Hq], [slots, Hq, D]
   SlotRange* ranges;                // [B] written by the MFMA kernel; null: `splits` slots a request
   int units, waves_units, subs;     // MFMA kernel: (KV head, 16 heads) units, of a workgroup, waves of one
-  int64_t target, min_tiles;
+  int64_t target, min_tiles;        // long: workgroups aimed at; both: the fewest tiles of a part
   int q_vec;
+  // short: tagged partial words [B, max_parts, Hq] m and l, [B, max_parts, Hq, D] o, and the
+  // arrival counters [B, units] (arrive.h)
+  unsigned long long *word_m, *word_l, *word_o, *arrivals;
+  unsigned long long epoch;
+  int max_parts;
   void* out;
   int64_t o_sb, o_sh;
 };
@@ -272,7 +280,7 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
 }
 
 // ---- the matrix-core kernel ---------------------------------------------------------------
-// 8- and 16-bit pools with a head dim of 32, 64 or 128.  A wave owns one unit (a KV head and
+// Head dims of 32, 64 and 128.  A wave owns one unit (a KV head and
 // up to 16 of its query heads) and walks tiles of 32 tokens, with no shared memory:
 //
 //   S^T = K Q^T   A: K rows (lane (j, c): row c, 8 of the head dim), B: the heads' queries;
@@ -285,12 +293,14 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
 // with (j, c) = (lane / 16, lane % 16).  Codes widen to bf16 in registers (exact); queries and
 // weights go in as sums of bf16 parts: as many of the query as its type has significand (1
 // for bf16, 2 for float16, 3 for float32) and of the weights two (2^-16 of a weight; three
-// for float32 queries).  float16 pools use float16 products.  A tile's scales are one dword a
+// for float32 queries).  float16 pools use float16 products, float32 pools float32 ones (four
+// of the head dim, or four tokens, at a time; the same lanes hold the same values).  A tile's scales are one dword a
 // lane, spread over the group by the broadcast of the multiply itself.
 // The running maximum moves only when a score passes it by more than SLACK (the sums then
 // hold weights up to 2^SLACK, no less precise): no cross-lane step in most tiles.
 
 constexpr int PM_TILE = 32;
+constexpr int PM_PARTS = 8;  // parts of a short request
 constexpr float PM_SLACK = 6.f;
 
 template <int S>
@@ -364,33 +374,58 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
 struct Share {
   int64_t b;
   int32_t slot, part, parts;  // this workgroup's slot; its part of the request's
+  int32_t n;                  // the request's tokens
 };
+
+// Inclusive sum over the wave's lanes on the vector unit (no LDS permutes: this runs before
+// the first load of a workgroup).
+template <typename T>
+__device__ __forceinline__ T scan_lanes(T v) {
+  auto step = [&](auto ctrl, auto rows) {
+    const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, decltype(rows)::value,
+                                              0xf, true);
+    v += __builtin_bit_cast(T, o);
+  };
+  step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // from 1, 2, 4, 8 lanes below
+  step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // a row's last lane to the next row
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // lane 31 to the upper half
+  return v;
+}
 
 // The request and part of workgroup w: every wave derives the same schedule from the lengths.
 // Parts are of `per` tiles, the fewest for which all requests together need at most `target`
 // workgroups (sum ceil(n_b / per) <= sum n_b / per + B); an empty request has one part.
 __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& out) {
   const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int64_t b0 = 0; b0 < a.B; b0 += 64)
-    if (b0 + lane < a.B) total += (request_length(a, b0 + lane) + PM_TILE - 1) / PM_TILE;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(static_cast<long long>(total), off, 64);
-  const int64_t room = a.target - (a.B < a.target / 2 ? a.B : a.target / 2);
-  int64_t per = (total + room - 1) / room;
-  if (per < a.min_tiles) per = a.min_tiles;
+  const int64_t limit = a.pages * a.P;
+  auto length_at = [&](int64_t b) {
+    const int64_t n = a.lengths[b < a.B ? b : 0];
+    return b < a.B && n > 0 ? static_cast<int32_t>(n < limit ? n : limit) : 0;
+  };
+  auto tiles_of = [](int32_t n) { return static_cast<int32_t>((static_cast<uint32_t>(n) + PM_TILE - 1) / PM_TILE); };
+  const int32_t first = length_at(lane);
+  float total = static_cast<float>(tiles_of(first));
+  for (int64_t b0 = 64; b0 < a.B; b0 += 64) total += static_cast<float>(tiles_of(length_at(b0 + lane)));
+  total = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scan_lanes(total)), 63));
+  const uint32_t room = static_cast<uint32_t>(a.target - (a.B < a.target / 2 ? a.B : a.target / 2));
+  // exact below 2^24 tiles; above, more than the sum's roundings can have lost
+  uint32_t per = total < 0x1p24f ? (static_cast<uint32_t>(total) + room - 1) / room
+                                 : static_cast<uint32_t>(total / static_cast<float>(room) * 1.0001f) + 1u;
+  if (per < static_cast<uint32_t>(a.min_tiles)) per = static_cast<uint32_t>(a.min_tiles);
   int32_t before = 0;
   for (int64_t b0 = 0; b0 < a.B; b0 += 64) {
-    int32_t parts = 0;
-    if (b0 + lane < a.B) {
-      const int64_t tiles = (request_length(a, b0 + lane) + PM_TILE - 1) / PM_TILE;
-      parts = tiles > per ? static_cast<int32_t>((tiles + per - 1) / per) : 1;
-    }
-    const int32_t through = before + wave_inclusive_sum(parts);
+    const int32_t n = b0 ? length_at(b0 + lane) : first;
+    const uint32_t tiles = static_cast<uint32_t>(tiles_of(n));
+    const int32_t parts = b0 + lane >= a.B ? 0 : (tiles > per ? static_cast<int32_t>((tiles + per - 1) / per) : 1);
+    const int32_t through = before + scan_lanes(parts);
     const uint64_t owners = __ballot(through > w);
     if (owners) {
       const int src = __ffsll(static_cast<unsigned long long>(owners)) - 1;
       out.b = b0 + src;
+      out.n = __builtin_amdgcn_readlane(n, src);
       out.parts = __builtin_amdgcn_readlane(parts, src);
       out.part = w - (__builtin_amdgcn_readlane(through, src) - out.parts);
       out.slot = w;
@@ -401,120 +436,211 @@ __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& o
   return false;
 }
 
-template <int S, int QD, int D, bool UNIFORM>
+// SHORT: few tokens in all.  Every unit has workgroups of its own (eight waves on its tiles), a
+// request `max_parts` at most, in a fixed grid, so that the table, the length and the query
+// load together; a part alone writes the output, several are joined by the last to arrive.
+// Else the schedule of share_of over workgroups of up to eight units (a page's rows are
+// contiguous over the KV heads), joined by pages_merge_kernel.
+template <int S, int QD, int D, bool UNIFORM, bool SHORT>
 __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
-  constexpr bool F16 = S == HS_DTYPE_F16;
+  constexpr bool F16 = S == HS_DTYPE_F16, F32 = S == HS_DTYPE_F32;
   constexpr int ES = elem_size<S>();
-  constexpr int KK = D / 32;                 // products over the head dim
+  constexpr int KK = F32 ? D / 4 : D / 32;   // products over the head dim
   constexpr int E = D / 16;                  // V elements of a lane and token
   constexpr int NQ = query_parts<S, QD>(), NP = weight_parts<S, QD>();
   constexpr int KROW = D / 4 * ES;           // K bytes of a lane and row
   constexpr int KL = KROW < 16 ? KROW : 16;  // a K load
   constexpr int KN = KROW / KL;
-  constexpr int VB = E * ES;                 // V bytes of a lane and token: one load
+  constexpr int VB = E * ES;                 // V bytes of a lane and token
+  constexpr int VL = VB < 16 ? VB : 16;      // a V load
   constexpr int VW = VB < 4 ? 1 : VB / 4;
+  constexpr int SD = D + 4;                  // row stride of the waves' sums in LDS: no bank conflicts
   extern __shared__ __attribute__((aligned(16))) float smem[];
+  __shared__ float s_m[8][16], s_l[8][16];
   const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   Share sh;
-  if (!share_of(a, static_cast<int32_t>(blockIdx.x), sh)) return;  // the same for every wave
+  if constexpr (SHORT) {
+    sh.b = blockIdx.z;
+    sh.part = static_cast<int32_t>(blockIdx.x);
+  } else {
+    if (!share_of(a, static_cast<int32_t>(blockIdx.x), sh)) return;  // the same for every wave
+    if (sh.part == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.ranges[sh.b] = SlotRange{sh.slot, sh.parts};
+  }
   const int64_t b = sh.b;
-  if (sh.part == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.ranges[b] = SlotRange{sh.slot, sh.parts};
-  const int unit = static_cast<int>(blockIdx.y) * a.waves_units + wave % a.waves_units;
-  const int sub = wave / a.waves_units;
-  const int64_t kv = unit / a.head_chunks;
-  const int h0 = unit % a.head_chunks * 16;
+  const int unit = SHORT ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * a.waves_units + wave % a.waves_units;
+  const int sub = SHORT ? wave : wave / a.waves_units;
+  const int subs = SHORT ? 8 : a.subs;
+  const int kv = unit / a.head_chunks, h0 = unit % a.head_chunks * 16;
   const int heads = static_cast<int>(a.g - h0 < 16 ? a.g - h0 : 16);
-  const int32_t n = static_cast<int32_t>(request_length(a, b));
-  const int32_t tiles = (n + PM_TILE - 1) / PM_TILE;
-  const int32_t share = (tiles + sh.parts - 1) / sh.parts;
-  const int32_t tile0 = sh.part * share;
-  const int32_t tile1 = tile0 + share < tiles ? tile0 + share : tiles;
   const int32_t* table = a.tables + b * a.t_sb + kv * a.t_sk;
-  const uint32_t P = static_cast<uint32_t>(a.P);
+  const uint32_t P = static_cast<uint32_t>(a.P), pages = static_cast<uint32_t>(a.pages);
   const char* pool = static_cast<const char*>(a.pool);
+  const uint32_t row_bytes = static_cast<uint32_t>(a.Hkv) * (D * ES);  // the host keeps 16 of them in 31 bits
+  const int64_t v_plane = a.P * static_cast<int64_t>(row_bytes);
 
-  // Q fragments of head c: part, product kk, 8 of the head dim from d0(kk)
-  auto d0_of = [&](int kk) { return ES == 1 && D >= 64 ? 64 * (kk >> 1) + 16 * j + 8 * (kk & 1) : 32 * kk + 8 * j; };
-  u32x4 qf[NQ][KK];
-  {
-    const bool in = c < heads;
-    const int64_t at = b * a.q_sb + (kv * a.g + h0 + (in ? c : 0)) * a.q_sh;
+  // Everything that needs no other load goes out first: the length, the first table entries
+  // (whatever the length: an index past the table reads its first entry, unused) and the query.
+  const int64_t limit = a.pages * a.P;
+  const int32_t length = SHORT ? a.lengths[b] : sh.n;
+  unsigned long long* counter = nullptr;
+  unsigned long long seen = 0;
+  int32_t share, tile0;
+  if constexpr (SHORT) {
+    counter = a.arrivals + b * a.units + unit;
+    seen = __hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    share = static_cast<int32_t>(a.min_tiles);
+    tile0 = sh.part * share;
+  }
+  int32_t n = 0, tiles = 0;
+  auto measure = [&]() {  // waits for the length
+    n = __builtin_amdgcn_readfirstlane(length < 0 ? 0 : (length > limit ? static_cast<int32_t>(limit) : length));
+    tiles = static_cast<int32_t>((static_cast<uint32_t>(n) + PM_TILE - 1) / PM_TILE);
+    if constexpr (SHORT) sh.parts = tiles > share ? (tiles + share - 1) / share : 1;
+  };
+  if constexpr (!SHORT) {
+    measure();
+    share = (tiles + sh.parts - 1) / sh.parts;
+    tile0 = sh.part * share;
+  }
+
+  // UNIFORM: pages of a multiple of 16 rows, so a tile's two halves lie in one page each.  A wave
+  // reads the table for 32 of its tiles at once (lane l: half l), keeps the halves' byte offsets
+  // in a register and takes each tile's from there; tiles without a page are passed over.
+  // Else lanes 0-31 find their token's row, one tile ahead, and the others take it from them.
+  int32_t entry = 0;  // table entry of this lane's half (UNIFORM: in the next batch) or token (in the next tile)
+  auto half_token = [&](int32_t batch) {  // first token of this lane's half in the batch
+    return static_cast<uint32_t>(tile0 + sub + (batch + (lane >> 1)) * subs) * 32u + 16u * (lane & 1);
+  };
+  auto token_of = [&](int32_t tile) { return static_cast<uint32_t>(tile) * 32u + (lane & 31); };
+  auto fetch = [&](uint32_t token) {
+    const uint32_t page = token / P;
+    entry = table[page < pages ? page : 0u];
+  };
+  int32_t at_tile = tile0 + sub;  // !UNIFORM: the tile `entry` belongs to
+  if constexpr (UNIFORM) fetch(half_token(0));
+  else fetch(token_of(at_tile));
+
+  // Q of head c, 8 of the head dim from d0(kk) for each product kk; or float32's one, at the dim
+  // of the lane's kk-th K word
+  auto d0_of = [&](int kk) {
+    return F32 ? 16 * (kk >> 2) + 4 * j + (kk & 3)
+               : (ES == 1 && D >= 64 ? 64 * (kk >> 1) + 16 * j + 8 * (kk & 1) : 32 * kk + 8 * j);
+  };
+  const bool live = c < heads;
+  const int64_t q_at = b * a.q_sb + (kv * a.g + h0 + (live ? c : 0)) * a.q_sh;
+  constexpr int QE = F32 ? 1 : 8;
+  constexpr int QW = QD == HS_DTYPE_F32 ? QE : 4;  // words of a product's elements
+  uint32_t qw[KK][QW];
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      float x[8];
-      if (QD != HS_DTYPE_F32 && a.q_vec) {
-        uint32_t w[4];
-        load_words<16>(static_cast<const char*>(a.q) + (at + d0_of(kk)) * 2, w);
+  for (int kk = 0; kk < KK; ++kk) {
+    if constexpr (QD == HS_DTYPE_F32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[2 * i] = low16<QD == HS_DTYPE_F16>(w[i]);
-          x[2 * i + 1] = high16<QD == HS_DTYPE_F16>(w[i]);
-        }
+      for (int i = 0; i < QE; ++i)
+        qw[kk][i] = __float_as_uint(static_cast<const float*>(a.q)[q_at + d0_of(kk) + i]);
+    } else {
+      const unsigned short* q = static_cast<const unsigned short*>(a.q) + q_at + d0_of(kk);
+      if (a.q_vec) {
+        load_words<16>(reinterpret_cast<const char*>(q), qw[kk]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = load_elem<QD>(a.q, at + d0_of(kk) + i);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = in ? x[i] : 0.f;
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          qf[q][kk][i] = pack16<F16>(x[2 * i], x[2 * i + 1]);
-          x[2 * i] -= low16<F16>(qf[q][kk][i]);
-          x[2 * i + 1] -= high16<F16>(qf[q][kk][i]);
-        }
+        for (int i = 0; i < 4; ++i) qw[kk][i] = q[2 * i] | static_cast<uint32_t>(q[2 * i + 1]) << 16;
       }
     }
   }
+  if constexpr (SHORT) measure();
+  const int32_t tile1 = tile0 + share < tiles ? tile0 + share : tiles;
+  if (SHORT && sh.part > 0 && tile0 >= tiles) return;  // past the request's tiles: the whole workgroup
 
   f32x4 acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_run = -INFINITY, l_run = 0.f;
 
-  // A tile's registers: K, V and scales.  Loads of the next tile go out as soon as the
-  // registers of this one are consumed.
+  // A tile's registers: scales, K and V.  Loads of the next tile go out as soon as the registers
+  // of this one are consumed.
   uint32_t kw[2][KN * KL / 4], vw[8][VW];
   float sc = 0.f;
-  const int64_t row_bytes = a.Hkv * D * ES;
-  const int64_t v_plane = static_cast<int64_t>(P) * row_bytes;
   // token of the scale this lane holds (lanes 0-7 of a group: keys, 8-15: values)
   const int s_token = 4 * j + (c & 3), s_half = (c >> 2) & 1;
+  float qs[F32 ? KK : 1];
+  u32x4 qf[F32 ? 1 : NQ][F32 ? 1 : KK];
+  auto split_query = [&]() {
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      if constexpr (F32) {
+        qs[kk] = live ? __uint_as_float(qw[kk][0]) : 0.f;
+      } else if constexpr (NQ == 1) {  // a 16-bit query goes in as it is
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qf[0][kk][i] = live ? qw[kk][i] : 0u;
+      } else {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (QD == HS_DTYPE_F32) x[i] = __uint_as_float(qw[kk][i]);
+          else x[i] = i & 1 ? high16<true>(qw[kk][i >> 1]) : low16<true>(qw[kk][i >> 1]);
+          x[i] = live ? x[i] : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            qf[q][kk][i] = pack16<F16>(x[2 * i], x[2 * i + 1]);
+            x[2 * i] -= low16<F16>(qf[q][kk][i]);
+            x[2 * i + 1] -= high16<F16>(qf[q][kk][i]);
+          }
+        }
+      }
+    }
+  };
 
   // One tile; bit t of `valid`: its token t counts.
   auto use_tile = [&](uint32_t valid, auto next_k, auto next_v) {
-    float sct = sc;
+    // this tile's scales leave the register that the next tile's load writes (a copy made at
+    // the end of the tile instead would wait for that load there)
+    float sct = 0.f;
+    if constexpr (quantised(S)) asm volatile("v_mov_b32 %0, %1" : "=v"(sct) : "v"(sc));
     float s[8];
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
       f32x4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        u32x4 kf;
-        if constexpr (quantised(S)) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x[4];
-            decode4<S>(kw[rt][2 * kk + h], x);
-            kf[2 * h] = pair_bf16(x[0], x[1]);
-            kf[2 * h + 1] = pair_bf16(x[2], x[3]);
-          }
+        if constexpr (F32) {
+          t = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[rt][kk]), qs[kk], t, 0, 0, 0);
         } else {
+          u32x4 kf;
+          if constexpr (quantised(S)) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) kf[i] = kw[rt][4 * kk + i];
+            for (int h = 0; h < 2; ++h) {
+              float x[4];
+              decode4<S>(kw[rt][2 * kk + h], x);
+              kf[2 * h] = pair_bf16(x[0], x[1]);
+              kf[2 * h + 1] = pair_bf16(x[2], x[3]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) kf[i] = kw[rt][4 * kk + i];
+          }
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) t = mfma_16x16x32<F16>(kf, qf[q][kk], t);
         }
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) t = mfma_16x16x32<F16>(kf, qf[q][kk], t);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * rt + i] = t[i];
     }
     next_k();
     const bool whole = valid == 0xffffffffu;
+    if (!whole) {  // a row past the end may hold anything
+      if constexpr (quantised(S)) sct = valid >> (16 * s_half + s_token) & 1 ? sct : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = valid >> (16 * (e >> 2) + 4 * j + (e & 3)) & 1;
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vw[e][w] = in ? vw[e][w] : 0u;  // its weight is 0, but 0 * NaN is not
+      }
+    }
     if constexpr (quantised(S)) {
-      if (!(valid >> (16 * s_half + s_token) & 1)) sct = 0.f;  // a row past the end may hold anything
       const float ks = sct * a.scale;
       s[0] *= group_lane<0>(ks);
       s[1] *= group_lane<1>(ks);
@@ -530,13 +656,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     }
     if (!whole) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (!(valid >> (16 * (e >> 2) + 4 * j + (e & 3)) & 1)) {
-          s[e] = -INFINITY;
-#pragma unroll
-          for (int w = 0; w < VW; ++w) vw[e][w] = 0u;  // weight 0, but 0 * NaN is none
-        }
-      }
+      for (int e = 0; e < 8; ++e) s[e] = valid >> (16 * (e >> 2) + 4 * j + (e & 3)) & 1 ? s[e] : -INFINITY;
     }
     float top = s[0];
 #pragma unroll
@@ -553,10 +673,8 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     }
     const float m_use = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      s[e] = exp2_(s[e] - m_use);
-      l_run += s[e];
-    }
+    for (int e = 0; e < 8; ++e) s[e] = exp2_(s[e] - m_use);
+    l_run += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     if constexpr (quantised(S)) {
       s[0] *= group_lane<8>(sct);
       s[1] *= group_lane<9>(sct);
@@ -567,170 +685,166 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
       s[6] *= group_lane<14>(sct);
       s[7] *= group_lane<15>(sct);
     }
-    u32x4 pf[NP];
+    if constexpr (F32) {  // four tokens a product: token slot t of the four groups
 #pragma unroll
-    for (int q = 0; q < NP; ++q) {
+      for (int t = 0; t < 8; ++t) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        pf[q][i] = pack16<F16>(s[2 * i], s[2 * i + 1]);
-        if (q + 1 < NP) {
-          s[2 * i] -= low16<F16>(pf[q][i]);
-          s[2 * i + 1] -= high16<F16>(pf[q][i]);
-        }
+        for (int e = 0; e < E; ++e)
+          acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vw[t][e]), s[t], acc[e], 0, 0, 0);
       }
-    }
-    // V^T fragments: pairs of tokens (2i, 2i + 1) at one dim
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      u32x4 even, odd;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (quantised(S)) {
-          float x[4], y[4];
-          const int shift = 8 * (e & 3);
-          decode4<S>(vw[2 * i][e >> 2], x);
-          decode4<S>(vw[2 * i + 1][e >> 2], y);
-          even[i] = pair_bf16(x[e & 3], y[e & 3]);
-          odd[i] = pair_bf16(x[(e & 3) + 1], y[(e & 3) + 1]);
-        } else {
-          even[i] = low_halves(vw[2 * i][e >> 1], vw[2 * i + 1][e >> 1]);
-          odd[i] = high_halves(vw[2 * i][e >> 1], vw[2 * i + 1][e >> 1]);
-        }
-      }
+    } else {
+      u32x4 pf[NP];
 #pragma unroll
       for (int q = 0; q < NP; ++q) {
-        acc[e] = mfma_16x16x32<F16>(even, pf[q], acc[e]);
-        acc[e + 1] = mfma_16x16x32<F16>(odd, pf[q], acc[e + 1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pf[q][i] = pack16<F16>(s[2 * i], s[2 * i + 1]);
+          if (q + 1 < NP) {
+            s[2 * i] -= low16<F16>(pf[q][i]);
+            s[2 * i + 1] -= high16<F16>(pf[q][i]);
+          }
+        }
+      }
+      // V^T fragments: pairs of tokens (2i, 2i + 1) at one dim
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        u32x4 even, odd;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (quantised(S)) {
+            float x[4], y[4];
+            decode4<S>(vw[2 * i][e >> 2], x);
+            decode4<S>(vw[2 * i + 1][e >> 2], y);
+            even[i] = pair_bf16(x[e & 3], y[e & 3]);
+            odd[i] = pair_bf16(x[(e & 3) + 1], y[(e & 3) + 1]);
+          } else {
+            even[i] = low_halves(vw[2 * i][e >> 1], vw[2 * i + 1][e >> 1]);
+            odd[i] = high_halves(vw[2 * i][e >> 1], vw[2 * i + 1][e >> 1]);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+          acc[e] = mfma_16x16x32<F16>(even, pf[q], acc[e]);
+          acc[e + 1] = mfma_16x16x32<F16>(odd, pf[q], acc[e + 1]);
+        }
       }
     }
     next_v();
   };
 
   if constexpr (UNIFORM) {
-    // Pages of a multiple of 16 rows: a tile's two halves lie in one page each.  The wave reads
-    // the table for 32 of its tiles at once (lane l: half l), keeps the byte offsets in a
-    // register and takes each tile's from there; tiles without a page are passed over.
-    const int32_t mine = tile1 - tile0 > sub ? (tile1 - tile0 - sub + a.subs - 1) / a.subs : 0;  // tiles of this wave
-    auto half_token = [&](int32_t batch) {  // first token of this lane's half in the batch
-      return 32 * (tile0 + sub + (batch + (lane >> 1)) * a.subs) + 16 * (lane & 1);
-    };
-    auto fetch = [&](int32_t batch, int32_t& block) {
-      const int32_t t = half_token(batch);
-      const bool in = batch + (lane >> 1) < mine && t < n;
-      block = table[in ? static_cast<uint32_t>(t) / P : 0u];
-      if (!in) block = -1;
-    };
-    int32_t batch = 0, block, ahead;
+    const int32_t mine = tile1 - tile0 > sub ? (tile1 - tile0 - sub + subs - 1) / subs : 0;  // tiles of this wave
+    int32_t batch = 0;
     uint64_t present = 0;
     int64_t offset = 0;  // byte offset of the half's first K row of this KV head
-    auto open = [&]() {  // the batch in `block` becomes current, the next one's table loads start
-      const int32_t t = half_token(batch);
-      const bool ok = block >= 0 && block < a.blocks;
-      const uint32_t within = static_cast<uint32_t>(t) % P;
-      offset = ok ? ((static_cast<int64_t>(block) * 2 * P + within) * a.Hkv + kv) * (D * ES) : 0;
+    auto open = [&]() {  // the batch of `entry` becomes current, and the next one's table loads start
+      const uint32_t t = half_token(batch);
+      const bool ok = batch + (lane >> 1) < mine && t < static_cast<uint32_t>(n) && entry >= 0 && entry < a.blocks;
+      offset = ok ? ((static_cast<int64_t>(entry) * 2 * P + t % P) * a.Hkv + kv) * (D * ES) : 0;
       present = __ballot(ok);
-      fetch(batch + 32, ahead);
+      if (batch + 32 < mine) fetch(half_token(batch + 32));
     };
     uint32_t valid = 0;
-    int64_t off0 = 0, off1 = 0;
+    uint64_t off0 = 0, off1 = 0;
     auto advance = [&]() {  // the next tile with a page; false at the end
-      uint64_t tilebits = (present | present >> 1) & 0x5555555555555555ull;
-      while (tilebits == 0) {
+      uint64_t some = (present | present >> 1) & 0x5555555555555555ull;
+      while (some == 0) {
         batch += 32;
         if (batch >= mine) return false;
-        block = ahead;
         open();
-        tilebits = (present | present >> 1) & 0x5555555555555555ull;
+        some = (present | present >> 1) & 0x5555555555555555ull;
       }
-      const int at = __ffsll(static_cast<unsigned long long>(tilebits)) - 1;
-      const int32_t t = 32 * (tile0 + sub + (batch + (at >> 1)) * a.subs);
-      const int left = n - t;
+      const int at = __ffsll(static_cast<unsigned long long>(some)) - 1;
+      const int32_t left = n - 32 * (tile0 + sub + (batch + (at >> 1)) * subs);
       valid = left >= PM_TILE ? 0xffffffffu : (1u << left) - 1u;
-      if (!(present >> at & 1)) valid &= 0xffff0000u;
-      if (!(present >> at & 2)) valid &= 0x0000ffffu;
+      const uint32_t has = static_cast<uint32_t>(present >> at) & 3u;
+      if (!(has & 1u)) valid &= 0xffff0000u;
+      if (!(has & 2u)) valid &= 0x0000ffffu;
       const uint32_t lo = static_cast<uint32_t>(offset), hi = static_cast<uint32_t>(offset >> 32);
-      off0 = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(hi, at))) << 32 |
-                                  static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, at)));
-      off1 = static_cast<int64_t>(
-          static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(hi, at + 1))) << 32 |
-          static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, at + 1)));
+      auto from = [&](int l) {
+        return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(hi, l))) << 32 |
+               static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, l));
+      };
+      off0 = from(at);
+      off1 = from(at + 1);
       present &= ~(3ull << at);
       return true;
     };
-    const int64_t k_lane = c * row_bytes + j * KL, v_lane = v_plane + 4 * j * row_bytes + c * VB;
+    // A load is a base every lane shares and a 32-bit offset of the lane's own.
+    const uint32_t k_lane = c * row_bytes + j * KL;
+    const uint32_t s_lane = static_cast<uint32_t>(s_token) * static_cast<uint32_t>(a.Hkv);
+    uint32_t v_lane[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v_lane[e] = (4 * j + e) * row_bytes + c * VB;
     auto load_k = [&]() {
+      if constexpr (quantised(S)) {
+        const uint64_t row = (s_half ? off1 : off0) / (D * ES) + (c >= 8 ? a.P * a.Hkv : 0);
+        sc = a.scales[row + s_lane];
+      }
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt) {
+        const char* p = pool + (rt ? off1 : off0);
 #pragma unroll
-        for (int i = 0; i < KN; ++i) load_words<KL>(pool + (rt ? off1 : off0) + k_lane + 64 * i, &kw[rt][i * (KL / 4)]);
-      }
-      if constexpr (quantised(S)) {
-        const int64_t row = (s_half ? off1 : off0) / D + (c >= 8 ? a.P * a.Hkv : 0);
-        sc = a.scales[row + s_token * a.Hkv];
+        for (int i = 0; i < KN; ++i) load_words<KL>(p + k_lane + 64 * i, &kw[rt][i * (KL / 4)]);
       }
     };
     auto load_v = [&]() {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) load_words<VB>(pool + (e < 4 ? off0 : off1) + v_lane + (e & 3) * row_bytes, vw[e]);
+      for (int e = 0; e < 8; ++e) {
+        const char* p = pool + v_plane + (e < 4 ? off0 : off1);
+#pragma unroll
+        for (int i = 0; i < VB / VL; ++i) load_words<VL>(p + v_lane[e & 3] + VL * i, &vw[e][i * 4]);
+      }
     };
     if (mine > 0) {
-      fetch(0, block);
       open();
       if (advance()) {
         load_k();
         load_v();
-        bool more = true;
-        while (more) {
+        split_query();
+        while (true) {
           const uint32_t now = valid;
-          more = advance();  // past the end the offsets stay: the last tile is read again, unused
+          const bool more = advance();  // past the end the offsets stay: the last tile is read again, unused
           use_tile(now, load_k, load_v);
+          if (!more) break;
         }
       }
     }
   } else {
-    // Any page size: lanes 0-31 find their token's row (head vectors of K from the pool's
-    // start), the others take it from them.  A masked token reads row 0.
-    int32_t tile = tile0 + sub;
-    int32_t ahead = 0;  // table entry of this lane's token, one tile ahead
-    uint32_t within = 0;
-    bool in = false;
-    int64_t row = 0;
+    int64_t row = 0;  // head vector of K of this lane's token; a masked token reads row 0
     uint32_t valid = 0;
-    auto fetch = [&](int32_t i) {
-      const int32_t t = PM_TILE * i + (lane & 31);
-      in = i < tile1 && t < n;
-      const uint32_t page = in ? static_cast<uint32_t>(t) / P : 0u;
-      within = in ? static_cast<uint32_t>(t) - page * P : 0u;
-      ahead = table[page];
-    };
     auto advance = [&]() {
-      const bool ok = in && ahead >= 0 && ahead < a.blocks;
-      row = ok ? (static_cast<int64_t>(ahead) * 2 * P + within) * a.Hkv + kv : 0;
+      const uint32_t t = token_of(at_tile);
+      const bool ok = at_tile < tile1 && t < static_cast<uint32_t>(n) && entry >= 0 && entry < a.blocks;
+      row = ok ? (static_cast<int64_t>(entry) * 2 * P + t % P) * a.Hkv + kv : 0;
       valid = static_cast<uint32_t>(__ballot(ok));
-      tile += a.subs;
-      fetch(tile);
+      at_tile += subs;
+      fetch(token_of(at_tile));
     };
     auto row_of = [&](int t) { return static_cast<int64_t>(__shfl(static_cast<long long>(row), t, 64)); };
     auto load_k = [&]() {
+      if constexpr (quantised(S)) sc = a.scales[row_of(16 * s_half + s_token) + (c >= 8 ? a.P * a.Hkv : 0)];
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt) {
         const char* p = pool + row_of(16 * rt + c) * (D * ES) + j * KL;
 #pragma unroll
         for (int i = 0; i < KN; ++i) load_words<KL>(p + 64 * i, &kw[rt][i * (KL / 4)]);
       }
-      if constexpr (quantised(S)) sc = a.scales[row_of(16 * s_half + s_token) + (c >= 8 ? a.P * a.Hkv : 0)];
     };
     auto load_v = [&]() {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        load_words<VB>(pool + row_of(16 * (e >> 2) + 4 * j + (e & 3)) * (D * ES) + v_plane + c * VB, vw[e]);
+      for (int e = 0; e < 8; ++e) {
+        const char* p = pool + row_of(16 * (e >> 2) + 4 * j + (e & 3)) * (D * ES) + v_plane + c * VB;
+#pragma unroll
+        for (int i = 0; i < VB / VL; ++i) load_words<VL>(p + VL * i, &vw[e][i * 4]);
+      }
     };
-    if (tile < tile1) {
-      fetch(tile);
+    if (at_tile < tile1) {
+      int32_t left = (tile1 - at_tile + subs - 1) / subs;
       advance();
       load_k();
       load_v();
-      int32_t left = (tile1 - tile0 - sub + a.subs - 1) / a.subs;
+      split_query();
       while (left > 0) {
         const uint32_t now = valid;
         advance();  // past the end every token is masked and reads row 0
@@ -744,10 +858,8 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
   if (l_run != l_run) m_run = 0.f;  // NaN scores set no maximum: keep the partial in the merge
-  __shared__ float s_m[8][16], s_l[8][16];
-  const int most = static_cast<int>(a.g < 16 ? a.g : 16);
-  if (a.subs == 1) {
-    if (c < heads) {
+  if (!SHORT && a.subs == 1) {
+    if (live) {
       const int64_t at = sh.slot * a.Hq + kv * a.g + h0 + c;
       if (j == 0) {
         a.part_m[at] = m_run;
@@ -761,7 +873,8 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     }
     return;
   }
-  if (c < heads) {
+  const int rows = static_cast<int>(a.g < 16 ? a.g : 16);
+  if (live) {
     if (j == 0) {
       s_m[wave][c] = m_run;
       s_l[wave][c] = l_run;
@@ -769,82 +882,261 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) smem[(wave * most + c) * D + E * (4 * j + i) + e] = acc[e][i];
+      for (int e = 0; e < E; ++e) smem[(wave * rows + c) * SD + E * (4 * j + i) + e] = acc[e][i];
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.waves_units * most * D; i += blockDim.x) {
-    const int u = i / (most * D), h = i / D % most, d = i % D;
-    const int un = static_cast<int>(blockIdx.y) * a.waves_units + u;
+  const int stride = SHORT ? 1 : a.waves_units, waves = SHORT ? 8 : a.waves_units * a.subs;
+  const uint32_t tag = SHORT ? group_tag(a.epoch, counter_round(seen, a.epoch)) : 0u;
+  constexpr int QUADS = D / 4;
+  for (int i = threadIdx.x; i < stride * rows * QUADS; i += blockDim.x) {
+    const int d = i % QUADS * 4, hu = i / QUADS;
+    const int u = SHORT ? 0 : hu / rows, h = SHORT ? hu : hu % rows;
+    const int un = SHORT ? unit : static_cast<int>(blockIdx.y) * a.waves_units + u;
     const int first = un % a.head_chunks * 16;
     if (first + h >= a.g) continue;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = u; w < a.waves_units * a.subs; w += a.waves_units) M = fmaxf(M, s_m[w][h]);
+    float M = -INFINITY, L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+      if (u + w * stride < waves) M = fmaxf(M, s_m[u + w * stride][h]);
     if (M != -INFINITY) {
-      for (int w = u; w < a.waves_units * a.subs; w += a.waves_units) {
-        const float f = s_m[w][h] == -INFINITY ? 0.f : exp2_(s_m[w][h] - M);
-        L += f * s_l[w][h];
-        O += f * smem[(w * most + h) * D + d];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const int at = u + w * stride;
+        if (at >= waves) continue;
+        const float f = exp2_(s_m[at][h] - M);  // 0 where a wave had no token
+        L += f * s_l[at][h];
+        O += f * *reinterpret_cast<const f32x4*>(smem + (at * rows + h) * SD + d);
       }
     }
-    const int64_t at = sh.slot * a.Hq + un / a.head_chunks * a.g + first + h;
-    if (d == 0) {
-      a.part_m[at] = M;
-      a.part_l[at] = L;
+    const int64_t head = static_cast<int64_t>(un / a.head_chunks) * a.g + first + h;
+    if constexpr (SHORT) {
+      if (sh.parts == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          store_any(a.out, b * a.o_sb + head * a.o_sh + d + e, L != 0.f ? O[e] / L : 0.f, a.q_dtype);
+      } else {
+        const int64_t at = (b * a.max_parts + sh.part) * a.Hq + head;
+        if (d == 0) {
+          store_partial(a.word_m + at, M, tag);
+          store_partial(a.word_l + at, L, tag);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) store_partial(a.word_o + at * D + d + e, O[e], tag);
+      }
+    } else {
+      const int64_t at = sh.slot * a.Hq + head;
+      if (d == 0) {
+        a.part_m[at] = M;
+        a.part_l[at] = L;
+      }
+      *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = O;
     }
-    a.part_o[at * D + d] = O;
+  }
+  if constexpr (SHORT) {
+    if (sh.parts == 1) return;
+    // The unit's last part joins all of them.  A slot is one (request, unit, part)'s at any
+    // length, and its words are cleared as they are taken: a replay of the launch finds no
+    // word of an earlier one, also where other work used the counters' memory in between.
+    __shared__ int s_last;
+    __shared__ float s_w[PM_PARTS][16], s_sum[16];
+    __syncthreads();  // every wave's stores are out before the arrival
+    if (threadIdx.x == 0) s_last = arrive_last(counter, seen, a.epoch, sh.parts) ? 1 : 0;
+    __syncthreads();
+    if (!s_last) return;
+    const int64_t base = b * a.max_parts * a.Hq + kv * a.g + h0;  // word of head h, part p: base + p * Hq + h
+    auto word = [&](unsigned long long* p) {
+      unsigned long long w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (static_cast<uint32_t>(w >> 32) != tag) w = partial_reread(p, tag);
+      __hip_atomic_store(p, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      return partial_value(w);
+    };
+    if (threadIdx.x < sh.parts * 16 && (threadIdx.x & 15) < heads) {
+      const int i = threadIdx.x, p = i >> 4, h = i & 15;
+      s_w[p][h] = word(a.word_m + base + p * a.Hq + h);
+      smem[i] = word(a.word_l + base + p * a.Hq + h);
+    }
+    __syncthreads();
+    if (threadIdx.x < heads) {
+      const int h = threadIdx.x;
+      float M = -INFINITY, L = 0.f;
+      for (int p = 0; p < sh.parts; ++p) M = fmaxf(M, s_w[p][h]);
+      for (int p = 0; p < sh.parts; ++p) {
+        const float f = s_w[p][h] == -INFINITY ? 0.f : exp2_(s_w[p][h] - M);
+        s_w[p][h] = f;
+        L += f * smem[p * 16 + h];
+      }
+      s_sum[h] = L;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * D; i += 512) {
+      const int h = i / D, d = i % D;
+      float O = 0.f;
+      for (int p0 = 0; p0 < sh.parts; p0 += 8) {
+        unsigned long long w[8];
+        unsigned long long* at[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int p = p0 + u < sh.parts ? p0 + u : p0;
+          at[u] = a.word_o + (base + p * a.Hq + h) * D + d;
+          w[u] = __hip_atomic_load(at[u], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (p0 + u >= sh.parts) continue;
+          if (static_cast<uint32_t>(w[u] >> 32) != tag) w[u] = partial_reread(at[u], tag);
+          __hip_atomic_store(at[u], 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          O += s_w[p0 + u][h] * partial_value(w[u]);
+        }
+      }
+      const float L = s_sum[h];
+      store_any(a.out, b * a.o_sb + (kv * a.g + h0 + h) * a.o_sh + d, L != 0.f ? O / L : 0.f, a.q_dtype);
+    }
+    if (threadIdx.x == 0)  // a replay of this launch counts from zero in the next round
+      __hip_atomic_store(counter,
+                         static_cast<unsigned long long>(counter_id(a.epoch)) << 32 |
+                             static_cast<unsigned long long>((counter_round(seen, a.epoch) + 1) & 0xffffu) << 16,
+                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 }
 
 // out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a head's slots; 0 if all are empty.
-__global__ __launch_bounds__(256) void pages_merge_kernel(PagesArgs a) {
+// One workgroup per (query head, request; and 256 C of the head dim).  The slots' weights go to LDS, one slot a thread;
+// then the sums: C elements a lane, 256 / (D / C) slots abreast and PJ_U of each in flight, so
+// that a long history's slots are a few rounds of loads (one slot after another took 66 of
+// 87 us at 128 slots of D = 64), joined over LDS in a fixed order.
+constexpr int PJ_T = 256;
+constexpr int PJ_U = 4;
+constexpr int PJ_SLOTS = 2048;  // weights held at once
+
+template <int C>
+__global__ __launch_bounds__(PJ_T) void pages_merge_kernel(PagesArgs a) {
+  __shared__ float s_w[PJ_SLOTS];
+  __shared__ float s_part[PJ_T * C];
+  __shared__ float s_red[PJ_T / 64];
   const int64_t h = blockIdx.x, b = blockIdx.y;
+  const int D = static_cast<int>(a.D);
   SlotRange r{static_cast<int32_t>(b * a.splits), static_cast<int32_t>(a.splits)};
   if (a.ranges) r = a.ranges[b];
   const int64_t base = r.first * a.Hq + h;
-  float M = -INFINITY;
-  for (int s = 0; s < r.count; ++s) M = fmaxf(M, a.part_m[base + s * a.Hq]);
-  for (int64_t d = threadIdx.x; d < a.D; d += blockDim.x) {
-    float L = 0.f, O = 0.f;
-    for (int s = 0; s < r.count; ++s) {
-      const int64_t at = base + s * a.Hq;
-      const float ms = a.part_m[at];
-      if (ms == -INFINITY) continue;
-      const float f = exp2_(ms - M);
-      L += f * a.part_l[at];
-      O += f * a.part_o[at * a.D + d];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto total = [&](float v, bool largest) {  // over the workgroup, in a fixed order
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      const float o = __shfl_xor(v, off, 64);
+      v = largest ? fmaxf(v, o) : v + o;
     }
-    store_any(a.out, b * a.o_sb + h * a.o_sh + d, L != 0.f ? O / L : 0.f, a.q_dtype);
+    __syncthreads();
+    if (lane == 0) s_red[wave] = v;
+    __syncthreads();
+    v = s_red[0];
+#pragma unroll
+    for (int w = 1; w < PJ_T / 64; ++w) v = largest ? fmaxf(v, s_red[w]) : v + s_red[w];
+    return v;
+  };
+  float M = -INFINITY;
+  for (int s = threadIdx.x; s < r.count; s += PJ_T) M = fmaxf(M, a.part_m[base + s * a.Hq]);
+  M = total(M, true);
+  const int columns = (D + C - 1) / C < PJ_T ? (D + C - 1) / C : PJ_T;  // lanes of a slot
+  const int abreast = PJ_T / columns;
+  const int g = threadIdx.x / columns, d = blockIdx.z * PJ_T * C + (threadIdx.x - g * columns) * C;
+  float L = 0.f, O[C] = {};
+  for (int s0 = 0; s0 < r.count; s0 += PJ_SLOTS) {
+    const int n = r.count - s0 < PJ_SLOTS ? r.count - s0 : PJ_SLOTS;
+    if (s0) __syncthreads();
+    for (int s = threadIdx.x; s < n; s += PJ_T) {
+      const int64_t at = base + (s0 + s) * a.Hq;
+      const float m = a.part_m[at], l = a.part_l[at];
+      const float w = m == -INFINITY ? 0.f : exp2_(m - M);
+      s_w[s] = w;
+      L += w * l;
+    }
+    __syncthreads();
+    if (g < abreast && d < D) {
+      for (int s = g; s < n; s += abreast * PJ_U) {
+        float x[PJ_U][C];
+#pragma unroll
+        for (int u = 0; u < PJ_U; ++u) {
+          const int at = s + u * abreast < n ? s + u * abreast : s;
+          const float* p = a.part_o + (base + (s0 + at) * a.Hq) * D + d;
+          if constexpr (C == 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[u][e] = v[e];
+          } else {
+            x[u][0] = *p;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < PJ_U; ++u) {
+          const float w = s + u * abreast < n ? s_w[s + u * abreast] : 0.f;
+#pragma unroll
+          for (int e = 0; e < C; ++e) O[e] += w * x[u][e];
+        }
+      }
+    }
+  }
+  L = total(L, false);
+#pragma unroll
+  for (int e = 0; e < C; ++e) s_part[threadIdx.x * C + e] = O[e];
+  __syncthreads();
+  const int first = blockIdx.z * PJ_T * C;
+  for (int i = threadIdx.x; i < columns * C && first + i < D; i += PJ_T) {
+    float sum = 0.f;
+    for (int u = 0; u < abreast; ++u) sum += s_part[u * columns * C + i];
+    store_any(a.out, b * a.o_sb + h * a.o_sh + first + i, L != 0.f ? sum / L : 0.f, a.q_dtype);
   }
 }
 
 // ---- host side ----------------------------------------------------------------
 
+static int64_t pool_elem_bytes(int code) { return code == HS_DTYPE_F32 ? 4 : (quantised(code) ? 1 : 2); }
+
 struct PagesPlan {
-  bool mfma;
+  bool mfma, brief;
   int G, head_chunks;
   int64_t splits, chunk;                 // general kernel
   int units, waves_units, subs;          // MFMA kernel
   int64_t target, min_tiles, slots;
 };
 
-static bool pages_mfma_shape(int code, int64_t D) { return code != HS_DTYPE_F32 && (D == 32 || D == 64 || D == 128); }
+static bool pages_mfma_shape(int64_t D) { return D == 32 || D == 64 || D == 128; }
 
 // Splits of the token axis: about 2048 workgroups, each with at least one tile per wave.
-static PagesPlan plan_pages(bool mfma, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t tokens) {
+static PagesPlan plan_pages(bool mfma, int64_t elem, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t tokens) {
   PagesPlan p{};
   const int64_t g = Hq / Hkv;
   p.mfma = mfma;
   if (mfma) {
     p.head_chunks = static_cast<int>((g + 15) / 16);
     p.units = static_cast<int>(Hkv * p.head_chunks);
+    const int64_t tiles = (tokens + PM_TILE - 1) / PM_TILE;
+    // Short: as many parts of a request as give every CU a workgroup, 8 at most (their join is one
+    // workgroup's work), of a tile for each of the eight waves at least.  Taken while a part is at
+    // most 32 tiles: us by this launch and by the long one, 28 query and 4 KV heads of 128 in
+    // int8, for 1 request of 256, 1024, 4096 and 16384 tokens 7.2 11.2 14.0 23.7 and 13.5 13.9
+    // 14.6 18.8, for 16 requests of 1024, 4096 and 16384 13.3 21.0 62.7 and 16.7 23.5 61.3.
+    // A unit of at most 128 KiB stays one part (14 query and 2 KV heads of 64 in int8, 64 requests
+    // of 1024 tokens: 10.4 in one part, 12.7 in two).
+    int64_t parts = 256 / (B * p.units);
+    parts = parts < 1 || tiles * 2 * PM_TILE * D * elem <= 128 * 1024 ? 1 : (parts > PM_PARTS ? PM_PARTS : parts);
+    p.min_tiles = (tiles + parts - 1) / parts;
+    if (p.min_tiles < 8) p.min_tiles = 8;
+    p.brief = p.min_tiles <= 32 && p.units <= 65535;
+    if (p.brief) {
+      p.slots = (tiles + p.min_tiles - 1) / p.min_tiles;
+      return p;
+    }
     p.waves_units = 8;
     while (p.units % p.waves_units) --p.waves_units;
     p.subs = 8 / p.waves_units;
     const int64_t groups = p.units / p.waves_units;
-    p.target = (512 + groups - 1) / groups;
-    p.min_tiles = 2 * p.subs;
-    const int64_t tiles = (tokens + PM_TILE - 1) / PM_TILE;
+    // workgroups that run at once: one of eight waves on a CU at D = 128 (registers), else two
+    // (a second round half filled cost 202 us against 191 at 8 histories of 128k tokens)
+    const int64_t resident = D == 128 ? 256 : 512;
+    p.target = (resident + groups - 1) / groups;
+    p.min_tiles = p.subs;
     const int64_t most = B * ((tiles + p.min_tiles - 1) / p.min_tiles);
     p.slots = most < p.target + B ? most : p.target + B;
     return p;
@@ -866,24 +1158,34 @@ static PagesPlan plan_pages(bool mfma, int64_t B, int64_t Hq, int64_t Hkv, int64
 
 // Partials (m, l, o) of every slot and query head, and the requests' slot ranges.
 static int64_t pages_workspace(const PagesPlan& p, int64_t B, int64_t Hq, int64_t D) {
+  if (p.mfma && p.brief) return (B * p.slots * Hq * (D + 2) + B * p.units) * 8;
   return p.slots * Hq * (D + 2) * 4 + B * static_cast<int64_t>(sizeof(SlotRange)) + 8;
 }
 
 template <int S, int QD>
 static void launch_mfma_pages(const PagesPlan& p, const PagesArgs& a, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(p.slots), static_cast<unsigned>(p.units / p.waves_units));
-  const dim3 block(static_cast<unsigned>(64 * p.waves_units * p.subs));
-  const int64_t heads = a.g < 16 ? a.g : 16;
-  const unsigned smem = p.subs == 1 ? 0u : static_cast<unsigned>(p.waves_units * p.subs * heads * a.D * 4);
-#define HS_PAGES_D(DIM)                                                                                       \
-  do {                                                                                                        \
-    if (a.P % 16 == 0) hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, true>), grid, block, smem, s, a);    \
-    else hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, false>), grid, block, smem, s, a);                 \
+  const int64_t waves = p.brief ? 8 : p.waves_units * p.subs, heads = a.g < 16 ? a.g : 16;
+  const dim3 grid = p.brief ? dim3(static_cast<unsigned>(p.slots), static_cast<unsigned>(p.units), static_cast<unsigned>(a.B))
+                            : dim3(static_cast<unsigned>(p.slots), static_cast<unsigned>(p.units / p.waves_units));
+  const dim3 block(static_cast<unsigned>(64 * waves));
+  // the waves' sums; a short request's joins need PM_PARTS x 16 floats of it
+  int64_t bytes = !p.brief && p.subs == 1 ? 0 : waves * heads * (a.D + 4) * 4;
+  if (p.brief && bytes < PM_PARTS * 16 * 4) bytes = PM_PARTS * 16 * 4;
+  const unsigned smem = static_cast<unsigned>(bytes);
+#define HS_PAGES_RUN(DIM, U, SHORT) \
+  hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT>), grid, block, smem, s, a)
+#define HS_PAGES_D(DIM)                                         \
+  do {                                                          \
+    if (a.P % 16 == 0 && p.brief) HS_PAGES_RUN(DIM, true, true); \
+    else if (a.P % 16 == 0) HS_PAGES_RUN(DIM, true, false);     \
+    else if (p.brief) HS_PAGES_RUN(DIM, false, true);           \
+    else HS_PAGES_RUN(DIM, false, false);                       \
   } while (0)
   if (a.D == 32) HS_PAGES_D(32);
   else if (a.D == 64) HS_PAGES_D(64);
   else HS_PAGES_D(128);
 #undef HS_PAGES_D
+#undef HS_PAGES_RUN
 }
 
 template <int S>
@@ -908,7 +1210,6 @@ static void launch_general(const PagesPlan& p, const PagesArgs& a, bool vec, hip
   }
 }
 
-static int64_t pool_elem_bytes(int code) { return code == HS_DTYPE_F32 ? 4 : (quantised(code) ? 1 : 2); }
 
 static int check_pages(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
                        int64_t pages) {
@@ -932,8 +1233,8 @@ extern "C" int64_t hs_attend_pages_workspace_bytes(int32_t query_dtype, int32_t 
   // either kernel may run on it (a pool that is not 16-byte aligned goes to the general one)
   int64_t need = 0;
   for (const bool mfma : {false, true}) {
-    if (mfma && !pages_mfma_shape(pool_code, head_dim)) continue;
-    const int64_t bytes = pages_workspace(plan_pages(mfma, batch, heads, kv_heads, head_dim, pages * page_size), batch,
+    if (mfma && !pages_mfma_shape(head_dim)) continue;
+    const int64_t bytes = pages_workspace(plan_pages(mfma, pool_elem_bytes(pool_code), batch, heads, kv_heads, head_dim, pages * page_size), batch,
                                           heads, head_dim);
     need = bytes > need ? bytes : need;
   }
@@ -954,10 +1255,11 @@ extern "C" int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_
   HS_CHECK_ARG(query && pool && tables && lengths && out, "null page attention pointer");
   HS_CHECK_ARG(valid_code(pool_code) == (scales != nullptr), "scales go with a quantised pool, and only with one");
   HS_CHECK_ARG(blocks >= 1 && blocks <= 0x7fffffff, "a pool has 1 to 2^31 - 1 blocks");
-  const bool mfma = pages_mfma_shape(pool_code, head_dim) && reinterpret_cast<uintptr_t>(pool) % 16 == 0;
-  const PagesPlan p = plan_pages(mfma, batch, heads, kv_heads, head_dim, pages * page_size);
+  const bool mfma = pages_mfma_shape(head_dim) && reinterpret_cast<uintptr_t>(pool) % 16 == 0 &&
+                    kv_heads * head_dim * pool_elem_bytes(pool_code) < (int64_t{1} << 27);  // 32-bit lane offsets
+  const PagesPlan p = plan_pages(mfma, pool_elem_bytes(pool_code), batch, heads, kv_heads, head_dim, pages * page_size);
   const int64_t need = pages_workspace(p, batch, heads, head_dim);
-  HS_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0,
+  HS_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                "page attention workspace too small or unaligned: need %lld bytes", static_cast<long long>(need));
   PagesArgs a{};
   a.q = query;
@@ -982,23 +1284,33 @@ extern "C" int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_
   a.splits = p.splits;
   a.chunk = p.chunk;
   a.scale = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(head_dim)));
-  a.part_m = static_cast<float*>(workspace);
+  a.part_o = static_cast<float*>(workspace);
+  a.part_m = a.part_o + p.slots * heads * head_dim;
   a.part_l = a.part_m + p.slots * heads;
-  a.part_o = a.part_l + p.slots * heads;
   a.ranges = nullptr;
   a.out = out;
   a.o_sb = o_stride_b;
   a.o_sh = o_stride_h;
   if (p.mfma) {
-    const uintptr_t end = reinterpret_cast<uintptr_t>(a.part_o + p.slots * heads * head_dim);
-    a.ranges = reinterpret_cast<SlotRange*>((end + 7) / 8 * 8);
     a.units = p.units;
-    a.waves_units = p.waves_units;
-    a.subs = p.subs;
-    a.target = p.target;
     a.min_tiles = p.min_tiles;
+    if (p.brief) {
+      a.max_parts = static_cast<int>(p.slots);
+      a.word_o = static_cast<unsigned long long*>(workspace);
+      a.word_m = a.word_o + batch * p.slots * heads * head_dim;
+      a.word_l = a.word_m + batch * p.slots * heads;
+      a.arrivals = a.word_l + batch * p.slots * heads;
+      a.epoch = next_epoch();
+    } else {
+      const uintptr_t end = reinterpret_cast<uintptr_t>(a.part_l + p.slots * heads);
+      a.ranges = reinterpret_cast<SlotRange*>((end + 7) / 8 * 8);
+      a.waves_units = p.waves_units;
+      a.subs = p.subs;
+      a.target = p.target;
+    }
     a.q_vec = reinterpret_cast<uintptr_t>(query) % 16 == 0 && q_stride_b % 8 == 0 && q_stride_h % 8 == 0;
     switch (pool_code) {
+      case HS_DTYPE_F32: launch_mfma_pages<HS_DTYPE_F32, HS_DTYPE_F32>(p, a, stream); break;
       case HS_DTYPE_F16: launch_mfma_pages<HS_DTYPE_F16, HS_DTYPE_F16>(p, a, stream); break;
       case HS_DTYPE_BF16: launch_mfma_pages<HS_DTYPE_BF16, HS_DTYPE_BF16>(p, a, stream); break;
       case HS_DTYPE_I8: launch_mfma_codes<HS_DTYPE_I8>(p, a, stream); break;
@@ -1015,9 +1327,12 @@ extern "C" int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_
     }
   }
   HS_CHECK_LAUNCH("page attention");
-  const unsigned threads = head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256);
-  hipLaunchKernelGGL(pages_merge_kernel, dim3(static_cast<unsigned>(heads), static_cast<unsigned>(batch)),
-                     dim3(threads), 0, stream, a);
+  if (p.mfma && p.brief) return HS_OK;
+  const int64_t columns = PJ_T * (head_dim % 4 == 0 ? 4 : 1);
+  const dim3 joins(static_cast<unsigned>(heads), static_cast<unsigned>(batch),
+                   static_cast<unsigned>((head_dim + columns - 1) / columns));
+  if (head_dim % 4 == 0) hipLaunchKernelGGL(pages_merge_kernel<4>, joins, dim3(PJ_T), 0, stream, a);
+  else hipLaunchKernelGGL(pages_merge_kernel<1>, joins, dim3(PJ_T), 0, stream, a);
   HS_CHECK_LAUNCH("page attention merge");
   return HS_OK;
 }

@@ -25,13 +25,13 @@ def rows_of(values, code):
 
 
 def case(batch, heads, kv, dim, page, lengths, code, dtype, device, seed=0, absent=0.0, per_head=False, spare=3,
-         amplitude=1.0):
+         amplitude=1.0, wide=2):
     """A batch whose tables are scattered over the pool.  Rows no request may use -- past a
     length, of blocks in no table -- are NaN (for int8 codes: NaN scales and any codes)."""
     gen = torch.Generator().manual_seed(seed + dim + page + sum(lengths))
     lists = kv if per_head else 1
     pages = [-(-n // page) for n in lengths]
-    width = max(1, max(pages)) + 2
+    width = max(1, max(pages)) + wide
     blocks = lists * sum(pages) + spare
     order = torch.randperm(blocks, generator=gen)
     tables = torch.randint(-3, blocks + 3, (batch, lists, width), generator=gen)  # past the pages: anything
@@ -132,26 +132,32 @@ def check(got, args, held=None):
 
 
 SHAPES = [(28, 4, 128), (14, 2, 64), (4, 2, 32), (8, 8, 128), (16, 1, 128), (20, 1, 64), (36, 1, 128), (12, 3, 96),
-          (5, 5, 80), (3, 1, 256), (2, 2, 512), (2, 1, 20), (3, 3, 7), (1, 1, 1), (22, 11, 64)]
+          (5, 5, 80), (3, 1, 256), (2, 2, 512), (2, 1, 20), (3, 3, 7), (1, 1, 1), (22, 11, 64), (2, 1, 511)]
 POOLS = [("int8", "bf16"), ("e4m3", "bf16"), ("int8", "f16"), ("e4m3", "f16"), ("int8", "f32"), ("e4m3", "f32"),
          ("bf16", "bf16"), ("f16", "f16"), ("f32", "f32")]
 
 
+# a table of this many columns more goes over the launch for long histories
+WIDE = 20_000
+
+
 @pytest.mark.gpu
+@pytest.mark.parametrize("wide", [2, WIDE])
 @pytest.mark.parametrize("code,dtype", POOLS)
 @pytest.mark.parametrize("heads,kv,dim", SHAPES)
-def test_matches_the_formula(gpu, heads, kv, dim, code, dtype):
-    args = case(3, heads, kv, dim, 16, [333, 1, 97], code, dtype, gpu)
+def test_matches_the_formula(gpu, heads, kv, dim, code, dtype, wide):
+    args = case(3, heads, kv, dim, 16, [333, 1, 97], code, dtype, gpu, wide=wide)
     check(attend_pages(*args), args)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("e4m3", "f32"), ("bf16", "bf16"), ("f32", "f32")])
 @pytest.mark.parametrize("page", [1, 3, 8, 12, 16, 32, 48, 64, 256])
-def test_page_sizes(gpu, page, code, dtype):
-    args = case(2, 14, 2, 64, page, [401, 256], code, dtype, gpu)
+@pytest.mark.parametrize("wide", [2, 300_000])
+def test_page_sizes(gpu, page, code, dtype, wide):
+    args = case(2, 14, 2, 64, page, [401, 256], code, dtype, gpu, wide=wide)
     check(attend_pages(*args), args)
-    args = case(1, 8, 4, 128, page, [63], code, dtype, gpu)
+    args = case(1, 8, 4, 128, page, [63], code, dtype, gpu, wide=wide)
     check(attend_pages(*args), args)
 
 
@@ -159,13 +165,14 @@ def test_page_sizes(gpu, page, code, dtype):
 @pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("e4m3", "f16"), ("f16", "f16"), ("f32", "f32")])
 def test_lengths_around_the_tiles(gpu, code, dtype):
     """Lengths on both sides of a page, a tile and a split, and none at all."""
-    for lengths in ([0], [1], [2], [15, 16, 17], [31, 32, 33], [63, 64, 65, 0, 127, 128, 129], [255, 0, 256, 257],
-                    [511, 512, 513], [2047, 2048, 2049], [4000, 3, 0]):
-        args = case(len(lengths), 8, 2, 128, 16, lengths, code, dtype, gpu)
-        got = attend_pages(*args)
-        check(got, args)
-        for b, n in enumerate(lengths):
-            assert n or (got[b] == 0).all()
+    for wide in (2, WIDE):
+        for lengths in ([0], [1], [2], [15, 16, 17], [31, 32, 33], [63, 64, 65, 0, 127, 128, 129],
+                        [255, 0, 256, 257], [511, 512, 513], [2047, 2048, 2049], [4000, 3, 0]):
+            args = case(len(lengths), 8, 2, 128, 16, lengths, code, dtype, gpu, wide=wide)
+            got = attend_pages(*args)
+            check(got, args)
+            for b, n in enumerate(lengths):
+                assert n or (got[b] == 0).all()
 
 
 @pytest.mark.gpu
@@ -174,10 +181,12 @@ def test_lengths_around_the_tiles(gpu, code, dtype):
 def test_absent_pages_and_tables_per_head(gpu, page, code, dtype):
     for per_head in (False, True):
         for absent in (0.0, 0.4, 1.0):
-            args = case(3, 14, 2, 64, page, [700, 33, 16], code, dtype, gpu, absent=absent, per_head=per_head)
-            got = attend_pages(*args)
-            check(got, args)
-            assert absent < 1.0 or (got == 0).all()
+            for wide in (2, WIDE):
+                args = case(3, 14, 2, 64, page, [700, 33, 16], code, dtype, gpu, absent=absent, per_head=per_head,
+                            wide=wide)
+                got = attend_pages(*args)
+                check(got, args)
+                assert absent < 1.0 or (got == 0).all()
 
 
 @pytest.mark.gpu
@@ -386,7 +395,7 @@ def test_entry_point_refusals_without_a_gpu():
                 dict(blocks=0), dict(blocks=2**31), dict(page=0), dict(kv=0), dict(kv=3), dict(dim=0), dict(dim=513),
                 dict(tables=None), dict(pages=0), dict(pages=2**31), dict(page=2**20, pages=2**12), dict(lengths=None),
                 dict(batch=0), dict(batch=70_000), dict(heads=0), dict(out=None), dict(ws=None), dict(nbytes=16),
-                dict(ws=at + 4)):
+                dict(ws=at + 8)):
         assert call(**bad) == -1, bad
         assert lib.hs_last_error()
     size = lib.hs_attend_pages_workspace_bytes
