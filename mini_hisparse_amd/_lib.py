@@ -233,23 +233,30 @@ def check(status: int, what: str):
         raise HipLibraryError(f"{what} failed ({status}): {message}")
 
 
-def dtype_code(dtype) -> int:
+_DTYPE_CODES = {}  # torch dtype -> element code, filled at the first use (torch is imported lazily)
+
+
+def _element_codes():
     import torch
 
-    codes = {torch.float32: HS_DTYPE_F32, torch.float16: HS_DTYPE_F16, torch.bfloat16: HS_DTYPE_BF16}
-    if dtype not in codes:
+    _DTYPE_CODES.update({torch.float32: HS_DTYPE_F32, torch.float16: HS_DTYPE_F16, torch.bfloat16: HS_DTYPE_BF16,
+                         torch.int8: HS_DTYPE_I8, torch.float8_e4m3fn: HS_DTYPE_E4M3})
+    return _DTYPE_CODES
+
+
+def dtype_code(dtype) -> int:
+    code = (_DTYPE_CODES or _element_codes()).get(dtype, HS_DTYPE_I8)
+    if code >= HS_DTYPE_I8:
         raise ValueError("KV dtype must be float32, float16 or bfloat16")
-    return codes[dtype]
+    return code
 
 
 def cache_code(dtype) -> int:
     """Element code of a quantised pool's codes."""
-    import torch
-
-    codes = {torch.int8: HS_DTYPE_I8, torch.float8_e4m3fn: HS_DTYPE_E4M3}
-    if dtype not in codes:
+    code = (_DTYPE_CODES or _element_codes()).get(dtype, 0)
+    if code < HS_DTYPE_I8:
         raise ValueError("cache codes must be int8 or float8_e4m3fn")
-    return codes[dtype]
+    return code
 
 
 def ptr(tensor) -> int:
@@ -274,11 +281,20 @@ def stream_handle(device=None) -> int:
 
 
 _SAME_DEVICE = contextlib.nullcontext()
+_DEVICE_NOW = None  # torch._C._cuda_getDevice
 
 
 def on_device(device):
     """Context in which ``device`` (a tensor's) is the current device: a kernel is launched
     on a stream of the current device only.  Free where it is current already."""
+    global _DEVICE_NOW
+    if _DEVICE_NOW is None:
+        import torch
+
+        torch.cuda.current_device()  # initialises the runtime
+        _DEVICE_NOW = torch._C._cuda_getDevice
+    if device.index == _DEVICE_NOW():
+        return _SAME_DEVICE
     import torch
 
-    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return torch.cuda.device(device)

@@ -12,7 +12,7 @@ inline bool valid_code(int code) { return code == HS_DTYPE_I8 || code == HS_DTYP
 
 // The largest code: a head vector's scale is its largest magnitude over this.
 template <int CODE>
-__device__ __forceinline__ constexpr float code_top() {
+constexpr __device__ __forceinline__ float code_top() {
   return CODE == HS_DTYPE_I8 ? 127.f : 448.f;
 }
 

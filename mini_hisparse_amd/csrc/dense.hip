@@ -181,11 +181,9 @@ __global__ __launch_bounds__(DN_T) void rotary_split_kernel(const void* qkv, int
 //
 // in fp32, rounded once.  The angle is reduced to a part of one turn in 64 bits: at
 // position 10^5 an fp32 angle is off by up to 4e-3, more than a bf16 step of the result.
-// A head vector is held by `lanes` lanes of NH_E pairs each (D = 128: 16 lanes of 4), so
-// both halves of a pair meet in one lane and the norm's sum is a butterfly within the
-// lanes.  A workgroup takes `brows` rows: its threads first fill the rows' cos/sin table in
+// A head vector is held by `lanes` lanes of NE pairs each, so both halves of a pair meet in
+// one lane and the norm's sum is a butterfly within the lanes.  A workgroup takes `brows` rows: its threads first fill the rows' cos/sin table in
 // LDS (one 64-bit reduction per row and pair, shared by all heads), then walk the rows' heads.
-constexpr int NH_E = 4;      // rotation pairs per lane
 constexpr int NH_TAB = 512;  // cos/sin pairs of a workgroup's table
 
 struct NormRotaryArgs {
@@ -198,69 +196,104 @@ struct NormRotaryArgs {
   int D, lanes_log2, brows;
 };
 
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_pairs(const void* base, int64_t at, int lane, int lanes, int half,
-                                           float (&x)[NH_E]) {
-  if constexpr (VEC) {
-    const bool in = lane * NH_E < half;
-    const int64_t i = at + (in ? lane * NH_E : 0);
-    if constexpr (DT == HS_DTYPE_F32) {
-      const f32x4 w = *reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + i);
+// Elements of half a head vector that a lane holds, as loaded: NE neighbours (VEC), or one of
+// every `lanes` (then as floats).
+template <int DT, int NE, bool VEC>
+struct HalfVector {
+  static constexpr int WORDS = VEC && DT != HS_DTYPE_F32 ? NE / 2 : NE;
+  uint32_t w[WORDS];
+
+  __device__ __forceinline__ void load(const void* base, int64_t at, int lane, int lanes, int half) {
+    if constexpr (VEC) {
+      const char* p = static_cast<const char*>(base) + (at + (lane * NE < half ? lane * NE : 0)) * (DT == HS_DTYPE_F32 ? 4 : 2);
+      if constexpr (WORDS == 4) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-      for (int e = 0; e < NH_E; ++e) x[e] = in ? w[e] : 0.f;
+        for (int i = 0; i < 4; ++i) w[i] = v[i];
+      } else {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+        w[0] = v[0];
+        w[1] = v[1];
+      }
     } else {
-      const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const unsigned short*>(base) + i);
 #pragma unroll
-      for (int e = 0; e < NH_E; ++e) {
-        const unsigned short b = static_cast<unsigned short>((in ? w[e >> 1] : 0u) >> (16 * (e & 1)));
-        x[e] = DT == HS_DTYPE_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+      for (int e = 0; e < NE; ++e) {
+        const int i = lane + lanes * e;
+        w[e] = __float_as_uint(i < half ? load_elem<DT>(base, at + i) : 0.f);
       }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < NH_E; ++e) {
-      const int i = lane + lanes * e;
-      x[e] = i < half ? load_elem<DT>(base, at + i) : 0.f;
-    }
   }
-}
-
-template <int DT, bool VEC>
-__device__ __forceinline__ void store_pairs(void* base, int64_t at, int lane, int lanes, int half,
-                                            const float (&x)[NH_E]) {
-  if constexpr (VEC) {
-    if (lane * NH_E >= half) return;
-    const int64_t i = at + lane * NH_E;
-    if constexpr (DT == HS_DTYPE_F32) {
-      *reinterpret_cast<f32x4*>(static_cast<float*>(base) + i) = f32x4{x[0], x[1], x[2], x[3]};
+  __device__ __forceinline__ void store(void* base, int64_t at, int lane, int lanes, int half) const {
+    if constexpr (VEC) {
+      if (lane * NE >= half) return;
+      char* p = static_cast<char*>(base) + (at + lane * NE) * (DT == HS_DTYPE_F32 ? 4 : 2);
+      if constexpr (WORDS == 4) *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+      else *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
     } else {
-      u32x2 w;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        w[e] = DT == HS_DTYPE_BF16
-                   ? f32_to_bf16_bits(x[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(x[2 * e + 1])) << 16
-                   : f32_to_f16_bits(x[2 * e]) | static_cast<uint32_t>(f32_to_f16_bits(x[2 * e + 1])) << 16;
-      *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(base) + i) = w;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < NH_E; ++e) {
-      const int i = lane + lanes * e;
-      if (i < half) store_elem<DT>(base, at + i, x[e]);
+      for (int e = 0; e < NE; ++e) {
+        const int i = lane + lanes * e;
+        if (i < half) store_elem<DT>(base, at + i, __uint_as_float(w[e]));
+      }
     }
   }
-}
+  __device__ __forceinline__ void floats(float (&x)[NE], bool in) const {  // zeros past the vector's end
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      if constexpr (WORDS == NE) {
+        x[e] = __uint_as_float(w[e]);
+      } else {
+        const unsigned short b = static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1)));
+        x[e] = DT == HS_DTYPE_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+      }
+      if constexpr (VEC) x[e] = in ? x[e] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void round_from(const float (&x)[NE]) {
+#pragma unroll
+    for (int e = 0; e < WORDS; ++e) {
+      if constexpr (WORDS == NE) w[e] = __float_as_uint(x[e]);
+      else w[e] = pack16<DT == HS_DTYPE_F16>(x[2 * e], x[2 * e + 1]);
+    }
+  }
+};
 
-template <int DT, bool VEC>
+template <int DT, int NE, bool VEC>
 __global__ __launch_bounds__(DN_T) void norm_rotary_split_kernel(NormRotaryArgs a) {
-  __shared__ float s_cos[NH_TAB], s_sin[NH_TAB];
+  using Half = HalfVector<DT, NE, VEC>;
+  __shared__ __attribute__((aligned(16))) float s_cos[NH_TAB], s_sin[NH_TAB];
   const int half = a.D / 2, lanes = 1 << a.lanes_log2;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.brows;
   const int nrows = static_cast<int>(a.rows - row0 < a.brows ? a.rows - row0 : a.brows);
+  const int H = static_cast<int>(a.heads), K = static_cast<int>(a.kv_heads), total = H + 2 * K;
+  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> a.lanes_log2, groups = DN_T >> a.lanes_log2;
+  const bool in = !VEC || lane * NE < half;
+  // this group's heads: h = first, first + step, ... of every row in turn; the next head's loads
+  // go out before the current one is worked on
+  const int step = static_cast<int>(gridDim.y) * groups;
+  int r = 0, h = static_cast<int>(blockIdx.y) * groups + group;
+  auto settle = [&]() {
+    while (h >= total && r < nrows) {
+      h -= total;
+      ++r;
+    }
+  };
+  Half lo, hi, wq[2], wk[2];
+  auto fetch = [&](Half& x, Half& y) {
+    const int64_t src = (row0 + r) * a.qkv_stride + static_cast<int64_t>(h) * a.D;
+    x.load(a.qkv, src, lane, lanes, half);
+    y.load(a.qkv, src + half, lane, lanes, half);
+  };
+  settle();
+  if (r < nrows) fetch(lo, hi);
+  for (int i = 0; i < 2; ++i) {
+    wq[i].load(a.wq, i * half, lane, lanes, half);
+    wk[i].load(a.wk, i * half, lane, lanes, half);
+  }
   for (int t = threadIdx.x; t < nrows * half; t += DN_T) {
-    const int r = t / half, i = t - r * half;
+    const int tr = t / half, i = t - tr * half;
     // turns = position * theta^(-2i/D) / 2 pi
-    const double turns = static_cast<double>(a.positions[row0 + r]) *
+    const double turns = static_cast<double>(a.positions[row0 + tr]) *
                          (exp2(-(2.0 * i / a.D) * a.log2_theta) * 0.15915494309189535);
     float s, c;
     sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
@@ -268,39 +301,38 @@ __global__ __launch_bounds__(DN_T) void norm_rotary_split_kernel(NormRotaryArgs 
     s_sin[t] = s;
   }
   __syncthreads();
-  const int64_t H = a.heads, K = a.kv_heads, total = H + 2 * K;
-  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> a.lanes_log2, groups = DN_T >> a.lanes_log2;
-  const int64_t tasks = nrows * total;
-  for (int64_t t = static_cast<int64_t>(blockIdx.y) * groups + group; t < tasks;
-       t += static_cast<int64_t>(gridDim.y) * groups) {
-    const int64_t r = t / total, h = t - r * total;
-    const int64_t row = row0 + r;
-    const int64_t src = row * a.qkv_stride + h * a.D;
-    float lo[NH_E], hi[NH_E];
-    load_pairs<DT, VEC>(a.qkv, src, lane, lanes, half, lo);
-    load_pairs<DT, VEC>(a.qkv, src + half, lane, lanes, half, hi);
-    void* dst = h < H ? a.q : (h < H + K ? a.k : a.v);
-    const int64_t to = (h < H ? row * H + h : (h < H + K ? row * K + h - H : row * K + h - H - K)) * a.D;
-    if (h < H + K) {  // one condition for all lanes of the head
-      float wl[NH_E], wh[NH_E], sq = 0.f;
-      const void* w = h < H ? a.wq : a.wk;
-      load_pairs<DT, VEC>(w, 0, lane, lanes, half, wl);
-      load_pairs<DT, VEC>(w, half, lane, lanes, half, wh);
+  while (r < nrows) {
+    const int cr = r, ch = h;
+    Half cur[2] = {lo, hi};
+    h += step;
+    settle();
+    if (r < nrows) fetch(lo, hi);
+    const int64_t row = row0 + cr;
+    void* dst = ch < H ? a.q : (ch < H + K ? a.k : a.v);
+    const int64_t to = (ch < H ? row * H + ch : (ch < H + K ? row * K + ch - H : row * K + ch - H - K)) * a.D;
+    if (ch < H + K) {  // one condition for all lanes of the head
+      float x[NE], y[NE], u[NE], v[NE], sq = 0.f;
+      cur[0].floats(x, in);
+      cur[1].floats(y, in);
 #pragma unroll
-      for (int e = 0; e < NH_E; ++e) sq += lo[e] * lo[e] + hi[e] * hi[e];
+      for (int e = 0; e < NE; ++e) sq += x[e] * x[e] + y[e] * y[e];
       for (int off = lanes >> 1; off > 0; off >>= 1) sq += __shfl_xor(sq, off, 64);
       const float norm = rsqrtf(sq / static_cast<float>(a.D) + a.eps);
+      (ch < H ? wq[0] : wk[0]).floats(u, in);
+      (ch < H ? wq[1] : wk[1]).floats(v, in);
 #pragma unroll
-      for (int e = 0; e < NH_E; ++e) {
-        const int i = VEC ? lane * NH_E + e : lane + lanes * e;
-        const int at = i < half ? static_cast<int>(r) * half + i : 0;
-        const float x = lo[e] * norm * wl[e], y = hi[e] * norm * wh[e], c = s_cos[at], s = s_sin[at];
-        lo[e] = x * c - y * s;
-        hi[e] = y * c + x * s;
+      for (int e = 0; e < NE; ++e) {
+        const int i = VEC ? lane * NE + e : lane + lanes * e;
+        const int at = i < half ? cr * half + i : 0;
+        const float p = x[e] * norm * u[e], q = y[e] * norm * v[e], c = s_cos[at], s = s_sin[at];
+        x[e] = p * c - q * s;
+        y[e] = q * c + p * s;
       }
+      cur[0].round_from(x);
+      cur[1].round_from(y);
     }
-    store_pairs<DT, VEC>(dst, to, lane, lanes, half, lo);
-    store_pairs<DT, VEC>(dst, to + half, lane, lanes, half, hi);
+    cur[0].store(dst, to, lane, lanes, half);
+    cur[1].store(dst, to + half, lane, lanes, half);
   }
 }
 
@@ -369,16 +401,19 @@ extern "C" int hs_norm_rotary_split(const void* qkv, int64_t qkv_stride, const v
   HS_CHECK_ARG(qkv && q_weight && k_weight && q && k && v && positions, "null normed rotary pointer");
   HS_CHECK_ARG(theta > 0.0 && isfinite(theta) && eps >= 0.f, "theta must be positive and eps not negative");
   const int half = static_cast<int>(head_dim / 2);
-  const uintptr_t bytes = NH_E * elem_bytes(dtype);  // a lane's vector
   const uintptr_t all = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_weight) |
                         reinterpret_cast<uintptr_t>(k_weight) | reinterpret_cast<uintptr_t>(q) |
                         reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
-  const bool vec = half % NH_E == 0 && qkv_stride % NH_E == 0 && all % bytes == 0;
+  // pairs of a lane: a load of 16 bytes where the head dim and the addresses allow it, else of 8
+  // (16-bit types), else element by element over a whole wave
+  int ne = 0;
+  for (const int n : {16 / elem_bytes(dtype), 4})
+    if (ne == 0 && half % n == 0 && qkv_stride % n == 0 && all % (n * elem_bytes(dtype)) == 0) ne = n;
   NormRotaryArgs a{qkv, q_weight, k_weight, q, k, v, positions, qkv_stride, rows, heads, kv_heads, log2(theta), eps,
                    static_cast<int>(head_dim), 6, 1};
-  if (vec) {
+  if (ne) {
     a.lanes_log2 = 0;
-    while ((NH_E << a.lanes_log2) < half) ++a.lanes_log2;
+    while ((ne << a.lanes_log2) < half) ++a.lanes_log2;
   }
   const int64_t groups = DN_T >> a.lanes_log2, total = heads + 2 * kv_heads;
   // Rows per workgroup: as many as give every thread one cos/sin pair, once that still
@@ -392,15 +427,21 @@ extern "C" int hs_norm_rotary_split(const void* qkv, int64_t qkv_stride, const v
     if (spread > most) spread = most;
   }
   const dim3 grid(static_cast<unsigned>((rows + a.brows - 1) / a.brows), static_cast<unsigned>(spread));
-  if (vec) {
-    if (dtype == HS_DTYPE_BF16) hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_BF16, true>), grid, dim3(DN_T), 0, stream, a);
-    else if (dtype == HS_DTYPE_F16) hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_F16, true>), grid, dim3(DN_T), 0, stream, a);
-    else hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_F32, true>), grid, dim3(DN_T), 0, stream, a);
+#define HS_NORM_ROTARY(DT, NE, VEC) \
+  hipLaunchKernelGGL((norm_rotary_split_kernel<DT, NE, VEC>), grid, dim3(DN_T), 0, stream, a)
+  if (dtype == HS_DTYPE_F32) {
+    if (ne) HS_NORM_ROTARY(HS_DTYPE_F32, 4, true);
+    else HS_NORM_ROTARY(HS_DTYPE_F32, 4, false);
+  } else if (dtype == HS_DTYPE_BF16) {
+    if (ne == 8) HS_NORM_ROTARY(HS_DTYPE_BF16, 8, true);
+    else if (ne) HS_NORM_ROTARY(HS_DTYPE_BF16, 4, true);
+    else HS_NORM_ROTARY(HS_DTYPE_BF16, 4, false);
   } else {
-    if (dtype == HS_DTYPE_BF16) hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_BF16, false>), grid, dim3(DN_T), 0, stream, a);
-    else if (dtype == HS_DTYPE_F16) hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_F16, false>), grid, dim3(DN_T), 0, stream, a);
-    else hipLaunchKernelGGL((norm_rotary_split_kernel<HS_DTYPE_F32, false>), grid, dim3(DN_T), 0, stream, a);
+    if (ne == 8) HS_NORM_ROTARY(HS_DTYPE_F16, 8, true);
+    else if (ne) HS_NORM_ROTARY(HS_DTYPE_F16, 4, true);
+    else HS_NORM_ROTARY(HS_DTYPE_F16, 4, false);
   }
+#undef HS_NORM_ROTARY
   HS_CHECK_LAUNCH("norm_rotary_split");
   return HS_OK;
 }

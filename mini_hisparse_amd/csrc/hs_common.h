@@ -58,6 +58,15 @@ __device__ __forceinline__ unsigned short f32_to_f16_bits(float f) {
   return b;
 }
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Two floats as a pair of 16-bit values, rounded to nearest.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (F16) return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
+  else return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(lo), static_cast<__bf16>(hi)});
+}
 // Storage element -> float for the three cache dtypes.
 template <int DT>
 __device__ __forceinline__ float load_elem(const void* base, int64_t i) {

@@ -312,15 +312,6 @@ constexpr int query_parts() { return !quantised(S) ? 1 : (QD == HS_DTYPE_BF16 ? 
 template <int S, int QD>
 constexpr int weight_parts() { return quantised(S) && QD == HS_DTYPE_F32 ? 3 : 2; }
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
-// Two floats as a pair of 16-bit values, rounded to nearest.
-template <bool F16>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-  if constexpr (F16) return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
-  else return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(lo), static_cast<__bf16>(hi)});
-}
 template <bool F16>
 __device__ __forceinline__ float low16(uint32_t w) {
   return F16 ? f16_bits_to_f32(static_cast<unsigned short>(w)) : __uint_as_float(w << 16);

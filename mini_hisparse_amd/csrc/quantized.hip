@@ -147,96 +147,131 @@ __device__ __forceinline__ u32x2 encode8(const float (&x)[QZ_E], float scale) {
   return w;
 }
 
-// One head vector per group of 1 << lanes_log2 lanes, in the order (token, plane, head).
-template <int DT, int CODE, bool VEC>
-__global__ __launch_bounds__(QZ_T) void append_quantized_kernel(QuantArgs a) {
-  const int lanes = 1 << a.lanes_log2;
-  const int64_t vec = (static_cast<int64_t>(blockIdx.x) * QZ_T + threadIdx.x) >> a.lanes_log2;
-  const int lane = threadIdx.x & (lanes - 1);
-  if (vec >= a.tokens * 2 * a.Hkv) return;  // whole groups leave: the butterfly stays within a group
-  const int64_t head = vec % a.Hkv, tp = vec / a.Hkv;
-  const int64_t token = tp >> 1;
-  const int plane = static_cast<int>(tp & 1);
-  const int64_t row = a.rows[token];
-  if (row < 0 || row >= a.pool_rows) return;
-  float x[QZ_E];
-  load_vector<DT, VEC>(plane ? a.v : a.k,
-                       plane ? token * a.v_st + head * a.v_sh : token * a.k_st + head * a.k_sh, lane, lanes, a.D, x);
-  // the largest magnitude as bits: NaN > infinity > every finite value
-  uint32_t top = 0;
-#pragma unroll
-  for (int e = 0; e < QZ_E; ++e) {
-    const uint32_t bits = __float_as_uint(x[e]) & 0x7fffffffu;
-    top = bits > top ? bits : top;
+// Where a head vector of K lies in the pool (vectors; V's is P * Hkv further): 32-bit division
+// unless the pool has more rows than that.
+__device__ __forceinline__ int64_t vector_at(int64_t row, int64_t head, int64_t pool_rows, int64_t P, int64_t Hkv) {
+  if (pool_rows <= 0xffffffffll) {
+    const uint32_t r = static_cast<uint32_t>(row), p = static_cast<uint32_t>(P), block = r / p;
+    return (static_cast<int64_t>(block) * 2 * P + (r - block * p)) * Hkv + head;
   }
-  for (int off = lanes >> 1; off > 0; off >>= 1) {
-    const uint32_t other = __shfl_xor(top, off, 64);
-    top = other > top ? other : top;
-  }
-  const bool finite = top < 0x7f800000u;
-  const float scale = finite ? __uint_as_float(top) / code_top<CODE>() : __uint_as_float(0x7fc00000u);
-  u32x2 w = {0u, 0u};
-  if (finite && scale > 0.f) w = encode8<CODE>(x, scale);
-  const int64_t block = row / a.P, within = row - block * a.P;
-  const int64_t at = ((block * 2 + plane) * a.P + within) * a.Hkv + head;
-  if (lane == 0) a.scales[at] = scale;
+  const int64_t block = row / P;
+  return (block * 2 * P + (row - block * P)) * Hkv + head;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_codes(unsigned char* codes, int64_t at, int lane, int lanes, int D, u32x2 w) {
   if constexpr (VEC) {
-    if (lane * QZ_E < a.D) *reinterpret_cast<u32x2*>(a.codes + at * a.D + lane * QZ_E) = w;
+    if (lane * QZ_E < D) *reinterpret_cast<u32x2*>(codes + at * D + lane * QZ_E) = w;
   } else {
 #pragma unroll
     for (int e = 0; e < QZ_E; ++e) {
       const int d = lane + lanes * e;
-      if (d < a.D) a.codes[at * a.D + d] = static_cast<unsigned char>(w[e >> 2] >> (8 * (e & 3)));
+      if (d < D) codes[at * D + d] = static_cast<unsigned char>(w[e >> 2] >> (8 * (e & 3)));
     }
+  }
+}
+
+// The K and the V vector of one (token, head) per group of 1 << lanes_log2 lanes: they share
+// the row and the index arithmetic, and their loads go out with the row's, together.
+template <int DT, int CODE, bool VEC>
+__global__ __launch_bounds__(QZ_T) void append_quantized_kernel(QuantArgs a) {
+  const int lanes = 1 << a.lanes_log2;
+  const uint32_t vec = (blockIdx.x * static_cast<uint32_t>(QZ_T) + threadIdx.x) >> a.lanes_log2;
+  const int lane = threadIdx.x & (lanes - 1);
+  const uint32_t Hkv = static_cast<uint32_t>(a.Hkv), token = vec / Hkv, head = vec - token * Hkv;
+  if (token >= a.tokens) return;  // whole groups leave: the butterfly stays within a group
+  const int64_t row = a.rows[token];
+  float x[2][QZ_E];
+  load_vector<DT, VEC>(a.k, token * a.k_st + head * a.k_sh, lane, lanes, a.D, x[0]);
+  load_vector<DT, VEC>(a.v, token * a.v_st + head * a.v_sh, lane, lanes, a.D, x[1]);
+  // the largest magnitude as bits: NaN > infinity > every finite value
+  uint32_t top[2] = {0u, 0u};
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+#pragma unroll
+    for (int e = 0; e < QZ_E; ++e) {
+      const uint32_t bits = __float_as_uint(x[p][e]) & 0x7fffffffu;
+      top[p] = bits > top[p] ? bits : top[p];
+    }
+  }
+  for (int off = lanes >> 1; off > 0; off >>= 1) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const uint32_t other = __shfl_xor(top[p], off, 64);
+      top[p] = other > top[p] ? other : top[p];
+    }
+  }
+  if (row < 0 || row >= a.pool_rows) return;
+  const int64_t at = vector_at(row, head, a.pool_rows, a.P, a.Hkv);
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const bool finite = top[p] < 0x7f800000u;
+    const float scale = finite ? __uint_as_float(top[p]) / code_top<CODE>() : __uint_as_float(0x7fc00000u);
+    u32x2 w = {0u, 0u};
+    if (finite && scale > 0.f) w = encode8<CODE>(x[p], scale);
+    const int64_t to = at + (p ? a.P * a.Hkv : 0);
+    if (lane == 0) a.scales[to] = scale;
+    store_codes<VEC>(a.codes, to, lane, lanes, a.D, w);
+  }
+}
+
+template <int DT, int CODE, bool VEC>
+__device__ __forceinline__ void widen_vector(void* dst, int64_t to, u32x2 w, float scale, int lane, int lanes, int D) {
+  float x[2][4];
+  decode4<CODE>(w[0], x[0]);
+  decode4<CODE>(w[1], x[1]);
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int e = 0; e < QZ_E; ++e) {
+      const int d = lane + lanes * e;
+      if (d < D) store_elem<DT>(dst, to + d, mul_rn(x[e >> 2][e & 3], scale));
+    }
+  } else if constexpr (DT == HS_DTYPE_F32) {
+    float* p = static_cast<float*>(dst) + to + lane * QZ_E;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      *reinterpret_cast<f32x4*>(p + 4 * h) = f32x4{x[h][0] * scale, x[h][1] * scale, x[h][2] * scale, x[h][3] * scale};
+  } else {
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = pack16<DT == HS_DTYPE_F16>(mul_rn(x[e >> 1][2 * (e & 1)], scale), mul_rn(x[e >> 1][2 * (e & 1) + 1], scale));
+    *reinterpret_cast<u32x4*>(static_cast<unsigned short*>(dst) + to + lane * QZ_E) = o;
   }
 }
 
 template <int DT, int CODE, bool VEC>
 __global__ __launch_bounds__(QZ_T) void read_quantized_kernel(ReadArgs a) {
   const int lanes = 1 << a.lanes_log2;
-  const int64_t vec = (static_cast<int64_t>(blockIdx.x) * QZ_T + threadIdx.x) >> a.lanes_log2;
+  const uint32_t vec = (blockIdx.x * static_cast<uint32_t>(QZ_T) + threadIdx.x) >> a.lanes_log2;
   const int lane = threadIdx.x & (lanes - 1);
-  if (vec >= a.n * 2 * a.Hkv) return;
-  const int64_t head = vec % a.Hkv, tp = vec / a.Hkv;
-  const int64_t i = tp >> 1;
-  const int plane = static_cast<int>(tp & 1);
+  const uint32_t Hkv = static_cast<uint32_t>(a.Hkv), i = vec / Hkv, head = vec - i * Hkv;
+  if (i >= a.n || (VEC && lane * QZ_E >= a.D)) return;
   const int64_t row = a.rows[i];
   const bool there = row >= 0 && row < a.pool_rows;  // else the row reads as zeros
-  const int64_t block = there ? row / a.P : 0, within = there ? row - block * a.P : 0;
-  const int64_t at = ((block * 2 + plane) * a.P + within) * a.Hkv + head;
-  const float scale = there ? a.scales[at] : 0.f;
-  void* dst = plane ? a.v : a.k;
-  const int64_t to = (i * a.Hkv + head) * a.D;
-  if constexpr (VEC) {
-    if (lane * QZ_E >= a.D) return;
-    u32x2 w = {0u, 0u};
-    if (there) w = *reinterpret_cast<const u32x2*>(a.codes + at * a.D + lane * QZ_E);
-    float x[2][4];
-    decode4<CODE>(w[0], x[0]);
-    decode4<CODE>(w[1], x[1]);
-    if constexpr (DT == HS_DTYPE_F32) {
-      float* p = static_cast<float*>(dst) + to + lane * QZ_E;
+  const int64_t at = there ? vector_at(row, head, a.pool_rows, a.P, a.Hkv) : 0;
+  const int64_t to = (static_cast<int64_t>(i) * a.Hkv + head) * a.D;
+  u32x2 w[2];
+  float scale[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<f32x4*>(p + 4 * h) =
-            f32x4{x[h][0] * scale, x[h][1] * scale, x[h][2] * scale, x[h][3] * scale};
+  for (int p = 0; p < 2; ++p) {
+    const int64_t from = at + (p ? a.P * a.Hkv : 0);
+    scale[p] = a.scales[from];
+    if constexpr (VEC) {
+      w[p] = *reinterpret_cast<const u32x2*>(a.codes + from * a.D + lane * QZ_E);
     } else {
-      u32x4 o;
+      w[p] = u32x2{0u, 0u};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float lo = mul_rn(x[e >> 1][2 * (e & 1)], scale), hi = mul_rn(x[e >> 1][2 * (e & 1) + 1], scale);
-        o[e] = DT == HS_DTYPE_BF16 ? f32_to_bf16_bits(lo) | static_cast<uint32_t>(f32_to_bf16_bits(hi)) << 16
-                                   : f32_to_f16_bits(lo) | static_cast<uint32_t>(f32_to_f16_bits(hi)) << 16;
+      for (int e = 0; e < QZ_E; ++e) {
+        const int d = lane + lanes * e;
+        if (d < a.D) w[p][e >> 2] |= static_cast<uint32_t>(a.codes[from * a.D + d]) << (8 * (e & 3));
       }
-      *reinterpret_cast<u32x4*>(static_cast<unsigned short*>(dst) + to + lane * QZ_E) = o;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < QZ_E; ++e) {
-      const int d = lane + lanes * e;
-      if (d < a.D) store_elem<DT>(dst, to + d, there ? mul_rn(decode1<CODE>(a.codes[at * a.D + d]), scale) : 0.f);
     }
   }
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+    widen_vector<DT, CODE, VEC>(p ? a.v : a.k, to, there ? w[p] : u32x2{0u, 0u}, there ? scale[p] : 0.f, lane, lanes,
+                                a.D);
 }
 
 // log2 of the lanes of a head vector: 8 elements a lane, or a whole wave when strided.
@@ -253,7 +288,8 @@ static int check_quantized(int64_t rows_n, int64_t kv_heads, int64_t head_dim, i
   HS_CHECK_ARG(valid_code(code), "invalid cache code %d", code);
   HS_CHECK_ARG(rows_n >= 0 && kv_heads >= 1 && head_dim >= 1 && head_dim <= 512 && page_size >= 1 && pool_rows >= 1,
                "quantised rows need positive sizes and a head_dim of at most 512");
-  HS_CHECK_ARG(kv_heads <= (int64_t{1} << 20) && rows_n <= (int64_t{1} << 31) / kv_heads,
+  // head vectors, at up to 64 lanes each, are counted in 32 bits
+  HS_CHECK_ARG(kv_heads <= (int64_t{1} << 20) && rows_n <= (int64_t{1} << 25) / kv_heads,
                "too many quantised head vectors in one call");
   HS_CHECK_ARG(codes && scales, "null quantised pool pointer");
   HS_CHECK_ARG((reinterpret_cast<uintptr_t>(scales) & 3) == 0, "scales must be 4-byte aligned");
@@ -299,8 +335,7 @@ extern "C" int hs_append_quantized(const void* k, int64_t k_stride_t, int64_t k_
   QuantArgs a{k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, rows, static_cast<unsigned char*>(codes), scales,
               tokens, pool_rows, page_size, kv_heads, static_cast<int>(head_dim), vector_lanes_log2(vec, head_dim)};
   const int64_t per = QZ_T >> a.lanes_log2;
-  const int64_t blocks = (tokens * 2 * kv_heads + per - 1) / per;
-  HS_CHECK_ARG(blocks <= 0x7fffffff, "too many quantised head vectors in one call");
+  const int64_t blocks = (tokens * kv_heads + per - 1) / per;
   const dim3 grid(static_cast<unsigned>(blocks));
   HS_QUANT_DISPATCH(append_quantized_kernel, dtype, code, vec, grid, stream, a);
   HS_CHECK_LAUNCH("append_quantized");
@@ -318,8 +353,7 @@ extern "C" int hs_read_quantized(const void* codes, const float* scales, int32_t
   ReadArgs a{static_cast<const unsigned char*>(codes), scales, rows, k, v, n, pool_rows, page_size, kv_heads,
              static_cast<int>(head_dim), vector_lanes_log2(vec, head_dim)};
   const int64_t per = QZ_T >> a.lanes_log2;
-  const int64_t blocks = (n * 2 * kv_heads + per - 1) / per;
-  HS_CHECK_ARG(blocks <= 0x7fffffff, "too many quantised head vectors in one call");
+  const int64_t blocks = (n * kv_heads + per - 1) / per;
   const dim3 grid(static_cast<unsigned>(blocks));
   HS_QUANT_DISPATCH(read_quantized_kernel, dtype, code, vec, grid, stream, a);
   HS_CHECK_LAUNCH("read_quantized");

@@ -328,27 +328,33 @@ def prepare_rotary_split(qkv, positions, heads, kv_heads, head_dim, theta, out):
 def _norm_rotary_check(qkv, q_weight, k_weight, positions, heads, kv_heads, head_dim, out):
     if heads < 1 or kv_heads < 1 or head_dim < 2 or head_dim % 2 or head_dim > 512:
         raise ValueError("norm_rotary_split takes positive head counts and an even head_dim of at most 512")
-    if qkv.dim() != 2 or qkv.shape[0] < 1:
-        raise ValueError("qkv must be [rows, (heads + 2 kv_heads) head_dim] with at least one row")
-    if qkv.stride(0) < qkv.shape[1] and qkv.shape[0] > 1:
+    shape, stride, dtype, device = qkv.shape, qkv.stride(), qkv.dtype, qkv.device
+    if len(shape) != 2 or shape[0] < 1 or shape[1] != (heads + 2 * kv_heads) * head_dim or stride[1] != 1:
+        raise ValueError("qkv must be [rows, (heads + 2 kv_heads) head_dim] with at least one row and unit inner "
+                         "stride")
+    if stride[0] < shape[1] and shape[0] > 1:
         raise ValueError("qkv rows must not overlap")
-    _rotary_check(qkv, positions, heads, kv_heads, head_dim, out)
-    if not positions.is_contiguous():
-        raise ValueError("positions must be contiguous")
-    for name, weight in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if (weight.shape != (head_dim,) or weight.dtype != qkv.dtype or weight.device != qkv.device
-                or not weight.is_contiguous()):
-            raise ValueError(f"{name} must be [head_dim] contiguous in the dtype and on the device of qkv")
-    if qkv.device.type != "cuda":
+    if positions.dtype != torch.int64 or positions.shape != shape[:1] or positions.device != device \
+            or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int64 [rows] on the device of qkv")
+    width = (head_dim,)
+    if q_weight.shape != width or q_weight.dtype != dtype or q_weight.device != device or not q_weight.is_contiguous():
+        raise ValueError("q_weight must be [head_dim] contiguous in the dtype and on the device of qkv")
+    if k_weight.shape != width or k_weight.dtype != dtype or k_weight.device != device or not k_weight.is_contiguous():
+        raise ValueError("k_weight must be [head_dim] contiguous in the dtype and on the device of qkv")
+    if out is not None:
+        for name, x, count in zip("qkv", out, (heads, kv_heads, kv_heads)):
+            _check_out(x, (shape[0], count, head_dim), qkv, f"norm_rotary_split {name}")
+    if device.type != "cuda":
         raise ValueError("norm_rotary_split needs ROCm device tensors (HIP kernels only)")
 
 
-def _norm_rotary_launch(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, q, k, v):
-    return Launch(_lib.load().hs_norm_rotary_split,
-                  (qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]), q_weight.data_ptr(), k_weight.data_ptr(),
-                   float(eps), q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), qkv.shape[0], heads,
-                   kv_heads, head_dim, float(theta), _lib.dtype_code(qkv.dtype)),
-                  "hs_norm_rotary_split")
+def _norm_rotary_args(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, q, k, v):
+    rows, width = qkv.shape
+    stride = qkv.stride(0)
+    return (qkv.data_ptr(), stride if stride > width else width, q_weight.data_ptr(), k_weight.data_ptr(), eps,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), rows, heads, kv_heads, head_dim, theta,
+            _lib.dtype_code(qkv.dtype))
 
 
 def norm_rotary_split(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, out=None):
@@ -358,16 +364,20 @@ def norm_rotary_split(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, 
     in float32, angles in 64 bits, and rounded once (``rotary_split`` rounds after every op
     of the model's chain, and its angles are float32)."""
     _norm_rotary_check(qkv, q_weight, k_weight, positions, heads, kv_heads, head_dim, out)
-    rows = qkv.shape[0]
     if out is None:
-        q = torch.empty((rows, heads, head_dim), dtype=qkv.dtype, device=qkv.device)
-        k = torch.empty((rows, kv_heads, head_dim), dtype=qkv.dtype, device=qkv.device)
+        rows = qkv.shape[0]
+        q = qkv.new_empty((rows, heads, head_dim))
+        k = qkv.new_empty((rows, kv_heads, head_dim))
         v = torch.empty_like(k)
     else:
         q, k, v = out
-    with _lib.on_device(qkv.device):
-        _norm_rotary_launch(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, q, k,
-                            v)(_stream(qkv))
+    device = qkv.device
+    with _lib.on_device(device):
+        status = _lib.load().hs_norm_rotary_split(
+            *_norm_rotary_args(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, q, k, v),
+            _lib.stream_handle(device))
+    if status:
+        _lib.check(status, "hs_norm_rotary_split")
     return q, k, v
 
 
@@ -377,7 +387,9 @@ def prepare_norm_rotary_split(qkv, q_weight, k_weight, eps, positions, heads, kv
     _norm_rotary_check(qkv, q_weight, k_weight, positions, heads, kv_heads, head_dim, out)
     if out is None:
         raise ValueError("prepare_norm_rotary_split writes into a given out")
-    return _norm_rotary_launch(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, *out)
+    return Launch(_lib.load().hs_norm_rotary_split,
+                  _norm_rotary_args(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, *out),
+                  "hs_norm_rotary_split")
 
 
 def _silu_check(gate_up, out):

@@ -9,10 +9,12 @@ driver calls.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
+from .quantized import QuantizedPool
 
 
 class MappedHost:
@@ -282,49 +284,60 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
     call replays with their contents of the moment.  Returns [B, Hq, D] in the query dtype
     (``out`` when given); zeros for a request without a token.
     """
-    from .quantized import QuantizedPool
-
     quantized = isinstance(pool, QuantizedPool)
     store = pool.codes if quantized else pool
-    if query.dim() != 3 or store.dim() != 5 or store.shape[1] != 2 or 0 in store.shape or 0 in query.shape:
+    if query.dim() != 3 or store.dim() != 5:
         raise ValueError("attend_pages takes query [B, Hq, D] and a pool [blocks, 2, page_size, kv_heads, head_dim]")
     batch, heads, dim = query.shape
-    blocks, _, page_size, kv_heads, head_dim = store.shape
+    blocks, planes, page_size, kv_heads, head_dim = store.shape
+    if planes != 2 or not (batch and heads and dim and blocks and page_size and kv_heads):
+        raise ValueError("attend_pages takes query [B, Hq, D] and a pool [blocks, 2, page_size, kv_heads, head_dim]")
     if dim != head_dim or heads % kv_heads or dim > 512:
         raise ValueError("query and pool differ in head_dim (at most 512), or query heads are no multiple of KV heads")
-    code = _lib.dtype_code(query.dtype)
-    if not quantized and store.dtype != query.dtype:
+    code, device = _lib.dtype_code(query.dtype), query.device
+    if quantized:
+        pool_code, scales = pool.code, pool.scales.data_ptr()
+    elif store.dtype != query.dtype:
         raise ValueError("attend_pages: a plain pool must hold the query dtype")
-    pool_code = _lib.cache_code(store.dtype) if quantized else code
-    if not store.is_contiguous():
+    elif not store.is_contiguous():
         raise ValueError("attend_pages needs a contiguous pool")
+    else:
+        pool_code, scales = code, None
     per_head = tables.dim() == 3
-    if tables.dtype != torch.int32 or tables.shape[:-1] != ((batch, kv_heads) if per_head else (batch,)) \
-            or tables.shape[-1] < 1 or tables.stride(-1) != 1 and tables.shape[-1] > 1:
+    t_shape, t_stride = tables.shape, tables.stride()
+    if tables.dtype != torch.int32 or t_shape[:-1] != ((batch, kv_heads) if per_head else (batch,)) \
+            or t_shape[-1] < 1 or t_stride[-1] != 1 and t_shape[-1] > 1:
         raise ValueError("page tables must be int32 [B, pages] or [B, kv_heads, pages] of unit inner stride")
     if lengths.dtype != torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous():
         raise ValueError("lengths must be contiguous int32 [B]")
-    if any(t.device != query.device for t in (store, tables, lengths)):
+    if store.device != device or tables.device != device or lengths.device != device:
         raise ValueError("query, pool, tables and lengths must be on one device")
-    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.device != device
                             or not out.is_contiguous()):
         raise ValueError("attend_pages: out must be contiguous, of the query's shape, dtype and device")
-    if query.device.type != "cuda":
+    if device.type != "cuda":
         raise ValueError("attend_pages needs ROCm device tensors (HIP kernels only)")
-    q = query if query.stride(2) == 1 or dim == 1 else query.contiguous()
-    result = torch.empty((batch, heads, dim), dtype=query.dtype, device=query.device) if out is None else out
-    pages = tables.shape[-1]
-    lib = _lib.load()
-    with _lib.on_device(query.device):
+    q_stride = query.stride()
+    if q_stride[2] != 1 and dim > 1:
+        query = query.contiguous()
+        q_stride = query.stride()
+    result = torch.empty_like(query, memory_format=torch.contiguous_format) if out is None else out
+    pages = t_shape[-1]
+    nbytes = _pages_workspace_bytes(code, pool_code, batch, heads, kv_heads, dim, page_size, pages)
+    with _lib.on_device(device):
         # a workspace of this call's own: calls on other streams and captured graphs share none
-        ws_bytes = lib.hs_attend_pages_workspace_bytes(code, pool_code, batch, heads, kv_heads, dim, page_size, pages)
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device)
-        status = lib.hs_attend_pages(
-            q.data_ptr(), q.stride(0), q.stride(1), code, store.data_ptr(),
-            pool.scales.data_ptr() if quantized else None, pool_code, blocks, page_size, kv_heads, dim,
-            tables.data_ptr(), tables.stride(0), tables.stride(1) if per_head else 0, pages, lengths.data_ptr(), batch,
-            heads, result.data_ptr(), result.stride(0), result.stride(1), workspace.data_ptr(), ws_bytes,
-            _lib.stream_handle(query.device),
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        status = _lib.load().hs_attend_pages(
+            query.data_ptr(), q_stride[0], q_stride[1], code, store.data_ptr(), scales, pool_code, blocks, page_size,
+            kv_heads, dim, tables.data_ptr(), t_stride[0], t_stride[1] if per_head else 0, pages, lengths.data_ptr(),
+            batch, heads, result.data_ptr(), heads * dim, dim, workspace.data_ptr(), nbytes,
+            _lib.stream_handle(device),
         )
-    _lib.check(status, "hs_attend_pages")
+    if status:
+        _lib.check(status, "hs_attend_pages")
     return result
+
+
+@functools.lru_cache(maxsize=1024)
+def _pages_workspace_bytes(*sizes):
+    return _lib.load().hs_attend_pages_workspace_bytes(*sizes)
