@@ -316,7 +316,7 @@ __global__ __launch_bounds__(DN_T) void norm_rotary_split_kernel(NormRotaryArgs 
       cur[1].floats(y, in);
 #pragma unroll
       for (int e = 0; e < NE; ++e) sq += x[e] * x[e] + y[e] * y[e];
-      for (int off = lanes >> 1; off > 0; off >>= 1) sq += __shfl_xor(sq, off, 64);
+      sq = group_reduce(sq, lanes, [](float p, float q) { return p + q; });
       const float norm = rsqrtf(sq / static_cast<float>(a.D) + a.eps);
       (ch < H ? wq[0] : wk[0]).floats(u, in);
       (ch < H ? wq[1] : wk[1]).floats(v, in);

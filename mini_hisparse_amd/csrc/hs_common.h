@@ -162,6 +162,24 @@ __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// Butterfly over groups of `lanes` lanes (a power of two, the same for the whole wave):
+// every lane receives op over its group, for a commutative op.  Up to 16 lanes it runs on
+// the vector unit: xor 1 and 2 within quads, then mirrors of 8 and 16 lanes (whose quads
+// hold equal values by then).
+template <typename T, typename Op>
+__device__ __forceinline__ T group_reduce(T v, int lanes, Op op) {
+  static_assert(sizeof(T) == 4, "one register");
+  auto other = [&](int bits) { return __builtin_bit_cast(T, bits); };
+  const auto raw = [&]() { return __builtin_bit_cast(int, v); };
+  if (lanes >= 2) v = op(v, other(__builtin_amdgcn_update_dpp(0, raw(), 0xb1, 0xf, 0xf, true)));
+  if (lanes >= 4) v = op(v, other(__builtin_amdgcn_update_dpp(0, raw(), 0x4e, 0xf, 0xf, true)));
+  if (lanes >= 8) v = op(v, other(__builtin_amdgcn_update_dpp(0, raw(), 0x141, 0xf, 0xf, true)));
+  if (lanes >= 16) v = op(v, other(__builtin_amdgcn_update_dpp(0, raw(), 0x140, 0xf, 0xf, true)));
+  if (lanes >= 32) v = op(v, other(__shfl_xor(raw(), 16, 64)));
+  if (lanes >= 64) v = op(v, other(__shfl_xor(raw(), 32, 64)));
+  return v;
+}
+
 template <typename T>
 __device__ __forceinline__ T wave_inclusive_sum(T v) {
   const int lane = threadIdx.x & 63;

@@ -50,101 +50,161 @@ __device__ __forceinline__ int elem_index(int lane, int lanes, int e) {
   return VEC ? lane * QZ_E + e : lane + lanes * e;
 }
 
+// A lane's elements of a head vector, and the largest magnitude of them as float bits (their
+// order is that of the magnitudes: NaN > infinity > every finite value).  16-bit elements are
+// compared as they are, two at a time.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+template <int DT>
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {  // of two pairs, or of two float32
+  if constexpr (DT == HS_DTYPE_F32) return a > b ? a : b;
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+
 template <int DT, bool VEC>
-__device__ __forceinline__ void load_vector(const void* base, int64_t at, int lane, int lanes, int D,
-                                            float (&x)[QZ_E]) {
-  if constexpr (VEC) {
-    const bool in = lane * QZ_E < D;
-    const int64_t i = at + (in ? lane * QZ_E : 0);
-    if constexpr (DT == HS_DTYPE_F32) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + i);
-      const f32x4 b = *reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + i + 4);
+struct Elements {
+  static constexpr int WORDS = VEC && DT != HS_DTYPE_F32 ? QZ_E / 2 : QZ_E;
+  uint32_t w[WORDS];  // as stored (VEC), else floats
+
+  __device__ __forceinline__ void load(const void* base, int64_t at, int lane, int lanes, int D) {
+    if constexpr (VEC) {
+      const bool in = lane * QZ_E < D;
+      const char* p = static_cast<const char*>(base) + (at + (in ? lane * QZ_E : 0)) * (DT == HS_DTYPE_F32 ? 4 : 2);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = in ? a[e] : 0.f;
-        x[4 + e] = in ? b[e] : 0.f;
+      for (int i = 0; i < WORDS; i += 4) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(p + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[i + e] = in ? v[e] : 0u;
       }
     } else {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const unsigned short*>(base) + i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t p = in ? w[e] : 0u;
-        const unsigned short lo = static_cast<unsigned short>(p), hi = static_cast<unsigned short>(p >> 16);
-        x[2 * e] = DT == HS_DTYPE_BF16 ? bf16_bits_to_f32(lo) : f16_bits_to_f32(lo);
-        x[2 * e + 1] = DT == HS_DTYPE_BF16 ? bf16_bits_to_f32(hi) : f16_bits_to_f32(hi);
+      for (int e = 0; e < QZ_E; ++e) {
+        const int d = lane + lanes * e;
+        w[e] = __float_as_uint(d < D ? load_elem<DT>(base, at + d) : 0.f);
       }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < QZ_E; ++e) {
-      const int d = lane + lanes * e;
-      x[e] = d < D ? load_elem<DT>(base, at + d) : 0.f;
-    }
   }
-}
+  __device__ __forceinline__ uint32_t largest(int lanes) const {  // over the head vector's lanes
+    constexpr int T = WORDS == QZ_E ? HS_DTYPE_F32 : DT;
+    constexpr uint32_t MAGNITUDE = T == HS_DTYPE_F32 ? 0x7fffffffu : 0x7fff7fffu;
+    uint32_t top = w[0] & MAGNITUDE;
+#pragma unroll
+    for (int i = 1; i < WORDS; ++i) top = larger<T>(top, w[i] & MAGNITUDE);
+    top = group_reduce(top, lanes, [](uint32_t a, uint32_t b) { return larger<T>(a, b); });
+    if constexpr (T == HS_DTYPE_F32) return top;
+    const uint32_t lo = top & 0xffffu, hi = top >> 16, one = lo > hi ? lo : hi;
+    return T == HS_DTYPE_BF16 ? one << 16 : __float_as_uint(f16_bits_to_f32(static_cast<unsigned short>(one)));
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (WORDS == QZ_E) return __uint_as_float(w[e]);
+    else if constexpr (DT == HS_DTYPE_BF16) return e & 1 ? __uint_as_float(w[e >> 1] & 0xffff0000u) : __uint_as_float(w[e >> 1] << 16);
+    else return f16_bits_to_f32(static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1))));
+  }
+};
 
-// Magnitude of the e4m3 code nearest to a (0 <= a <= 448), ties to even, as a float.
-__device__ __forceinline__ float e4m3_nearest(double a) {
-  const int ex = a > 0.0 ? __builtin_amdgcn_frexp_exp(a) : -99;  // a = m 2^ex, m in [0.5, 1)
-  const int step = (ex - 1 < -6 ? -6 : ex - 1) - 3;              // log2 of the grid's spacing at a
-  return static_cast<float>(ldexp(rint(ldexp(a, -step)), step));
-}
+// Adding it rounds a small float to a whole number (ties to even) and leaves that in the low bits.
+constexpr float WHOLE = 12582912.f;  // 1.5 * 2^23
 
-// Code of one element by the exact quotient (64 bits hold it well enough: a quotient of
-// two 24-bit values that is no border of the grid is at least 2^-34 of itself away from one).
+// Four floats of the code's range as codes, rounded to nearest; int8's come with WHOLE added.
 template <int CODE>
-__device__ __forceinline__ float code_exact(float x, float scale) {
-  double q = static_cast<double>(x) / static_cast<double>(scale);
-  q = fmin(fmax(q, -static_cast<double>(code_top<CODE>())), static_cast<double>(code_top<CODE>()));
-  if constexpr (CODE == HS_DTYPE_I8) return static_cast<float>(rint(q));
-  else return copysignf(e4m3_nearest(fabs(q)), x);
-}
-
-// The quotient x * (1 / scale) in 32 bits is within 2^-22 of itself; the code it rounds to
-// is the right one unless it lies that close to a border between two codes.
-template <int CODE>
-__device__ __forceinline__ bool near_border(float q) {
+__device__ __forceinline__ uint32_t codes4(const float (&q)[4]) {
   if constexpr (CODE == HS_DTYPE_I8) {
-    return fabsf(fabsf(q - rintf(q)) - 0.5f) < 0x1p-14f;  // |q| <= 127: off by at most 2^-15
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(q[1]), __float_as_uint(q[0]), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(q[3]), __float_as_uint(q[2]), 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
   } else {
-    const uint32_t below = __float_as_uint(q) & 0xfffffu;  // significand bits under e4m3's
-    const float t = fabsf(q) * 512.f;                      // multiples of 2^-9 below 2^-6
-    const bool normal = below - 0x7fff0u <= 0x20u;
-    return t >= 8.f ? normal : fabsf(t - floorf(t) - 0.5f) < 0x1p-16f;
+    const int p = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], p, true));
   }
 }
 
+// largest / top, correctly rounded: one Newton step on the product with the reciprocal (with the
+// remainder exact; checked for every significand), or the division where it would underflow.
 template <int CODE>
-__device__ __forceinline__ u32x2 encode8(const float (&x)[QZ_E], float scale) {
-  float c[QZ_E];
-  const float inverse = 1.f / scale;
-  // a scale so small that its inverse overflows takes the exact way throughout
-  bool exact = !(scale >= 0x1p-100f);
-#pragma unroll
-  for (int e = 0; e < QZ_E; ++e) {
-    const float q = x[e] * inverse;
-    exact = exact || near_border<CODE>(q);
-    c[e] = CODE == HS_DTYPE_I8 ? rintf(q) : q;
+__device__ __forceinline__ float scale_of(float largest) {
+  constexpr float TOP = code_top<CODE>(), RECIPROCAL = 1.f / TOP;
+  if (largest < 0x1p-90f) return largest / TOP;
+  const float q = largest * RECIPROCAL;
+  return fmaf(fmaf(-TOP, q, largest), RECIPROCAL, q);
+}
+
+// A quotient next to a border between two codes, settled: the border t is exact in fp32, the sign
+// of x - t * scale is that of one rounded multiply-add, and the result is t, or a value past
+// it on x's side, which rounds as the exact quotient does.  (64-bit divisions here, in the one
+// wave in 30 that comes by, took 8 of 19 us of a 16k-token prompt.)
+template <int CODE>
+__device__ __forceinline__ float settle(float q, float x, float scale) {
+  if constexpr (CODE == HS_DTYPE_I8) {
+    const float t = floorf(q) + 0.5f;
+    if (!(fabsf(q - t) < 0x1p-15f)) return q;
+    const float r = fmaf(-t, scale, x);
+    return r > 0.f ? t + 0.25f : (r < 0.f ? t - 0.25f : t);
+  } else {
+    // five significand bits hold codes and borders; below 2^-6 the grid keeps the spacing of
+    // [2^-6, 2^-5), to which the value is moved and moved back
+    const float a = fabsf(q), up = a < 0x1p-6f ? 0x1p-6f : 0.f;
+    const uint32_t b = __float_as_uint(a + up);
+    if (((b + 0x80004u) & 0xfffffu) > 8u) return q;
+    const float t = __uint_as_float((b + 0x40000u) & 0xfff80000u) - up;
+    const float r = fmaf(-t, scale, fabsf(x));
+    const float v = __uint_as_float(__float_as_uint(t) + (r > 0.f ? 1u : 0u) - (r < 0.f ? 1u : 0u));
+    return copysignf(v, x);
   }
-  if (exact) {
-#pragma unroll
-    for (int e = 0; e < QZ_E; ++e) c[e] = code_exact<CODE>(x[e], scale);
-  }
-  u32x2 w;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
+}
+
+// A quotient in 64 bits, for scales whose inverse overflows: two 24-bit values' quotient that
+// is no border of the grid is at least 2^-34 of itself away from one.  It is rounded on to
+// fp32 towards zero, with the last bit set where that lost something: no border has that bit.
+template <int CODE>
+__device__ __forceinline__ float quotient64(float x, float scale) {
+  constexpr double TOP = static_cast<double>(code_top<CODE>());
+  const double q = fmin(fmax(static_cast<double>(x) / static_cast<double>(scale), -TOP), TOP);
+  const float f = static_cast<float>(q);
+  const double f64 = static_cast<double>(f);
+  if (f64 == q) return f;
+  return __uint_as_float((__float_as_uint(f) - (fabs(f64) > fabs(q) ? 1u : 0u)) | 1u);
+}
+
+// The codes of a lane's elements.  x * (1 / scale) in 32 bits (the reciprocal to one step) is within
+// 1.5 * 2^-23 of the quotient, so the code it rounds to is the right one unless it lies that close
+// to a border between two codes (one wave in 30 of int8's, in 200 of e4m3's, for normal values).
+template <int CODE, typename X>
+__device__ __forceinline__ u32x2 encode8(const X& x, float scale) {
+  constexpr float ADD = CODE == HS_DTYPE_I8 ? WHOLE : 0.f;
+  float q[2][4];
+  if (scale >= 0x1p-100f) {
+    const float inverse = __builtin_amdgcn_rcpf(scale);
+    bool near;
     if constexpr (CODE == HS_DTYPE_I8) {
-      w[h] = 0;
+      float off = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[h] |= (static_cast<uint32_t>(static_cast<int32_t>(c[4 * h + e])) & 0xffu) << (8 * e);
+      for (int e = 0; e < QZ_E; ++e) {
+        const float v = x.get(e), t = fmaf(v, inverse, WHOLE);
+        q[e >> 2][e & 3] = t;
+        off = fmaxf(off, fabsf(fmaf(v, inverse, WHOLE - t)));  // |quotient - code|
+      }
+      near = off > 0.5f - 0x1p-15f;
     } else {
-      int p = __builtin_amdgcn_cvt_pk_fp8_f32(c[4 * h], c[4 * h + 1], 0, false);
-      p = __builtin_amdgcn_cvt_pk_fp8_f32(c[4 * h + 2], c[4 * h + 3], p, true);
-      w[h] = static_cast<uint32_t>(p);
+      uint32_t off = 0xffffffffu;
+#pragma unroll
+      for (int e = 0; e < QZ_E; ++e) {
+        const float v = x.get(e) * inverse, a = fabsf(v), b = a < 0x1p-6f ? a + 0x1p-6f : a;
+        q[e >> 2][e & 3] = v;
+        const uint32_t d = (__float_as_uint(b) + 0x80004u) & 0xfffffu;  // 4 at a border
+        off = d < off ? d : off;
+      }
+      near = off <= 8u;
     }
+    if (near) {
+#pragma unroll
+      for (int e = 0; e < QZ_E; ++e) q[e >> 2][e & 3] = settle<CODE>(x.get(e) * inverse, x.get(e), scale) + ADD;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < QZ_E; ++e) q[e >> 2][e & 3] = quotient64<CODE>(x.get(e), scale) + ADD;
   }
-  return w;
+  return u32x2{codes4<CODE>(q[0]), codes4<CODE>(q[1])};
 }
 
 // Where a head vector of K lies in the pool (vectors; V's is P * Hkv further): 32-bit division
@@ -172,7 +232,9 @@ __device__ __forceinline__ void store_codes(unsigned char* codes, int64_t at, in
 }
 
 // The K and the V vector of one (token, head) per group of 1 << lanes_log2 lanes: they share
-// the row and the index arithmetic, and their loads go out with the row's, together.
+// the row and the index arithmetic, and their loads go out with the row's, together.  (A grid
+// of the workgroups that run at once, striding with the next pair's loads in flight, took
+// 16.8 us for a 16k-token prompt at the 7B shape, this 14.0.)
 template <int DT, int CODE, bool VEC>
 __global__ __launch_bounds__(QZ_T) void append_quantized_kernel(QuantArgs a) {
   const int lanes = 1 << a.lanes_log2;
@@ -181,32 +243,16 @@ __global__ __launch_bounds__(QZ_T) void append_quantized_kernel(QuantArgs a) {
   const uint32_t Hkv = static_cast<uint32_t>(a.Hkv), token = vec / Hkv, head = vec - token * Hkv;
   if (token >= a.tokens) return;  // whole groups leave: the butterfly stays within a group
   const int64_t row = a.rows[token];
-  float x[2][QZ_E];
-  load_vector<DT, VEC>(a.k, token * a.k_st + head * a.k_sh, lane, lanes, a.D, x[0]);
-  load_vector<DT, VEC>(a.v, token * a.v_st + head * a.v_sh, lane, lanes, a.D, x[1]);
-  // the largest magnitude as bits: NaN > infinity > every finite value
-  uint32_t top[2] = {0u, 0u};
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-#pragma unroll
-    for (int e = 0; e < QZ_E; ++e) {
-      const uint32_t bits = __float_as_uint(x[p][e]) & 0x7fffffffu;
-      top[p] = bits > top[p] ? bits : top[p];
-    }
-  }
-  for (int off = lanes >> 1; off > 0; off >>= 1) {
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const uint32_t other = __shfl_xor(top[p], off, 64);
-      top[p] = other > top[p] ? other : top[p];
-    }
-  }
+  Elements<DT, VEC> x[2];
+  x[0].load(a.k, token * a.k_st + head * a.k_sh, lane, lanes, a.D);
+  x[1].load(a.v, token * a.v_st + head * a.v_sh, lane, lanes, a.D);
+  const uint32_t top[2] = {x[0].largest(lanes), x[1].largest(lanes)};
   if (row < 0 || row >= a.pool_rows) return;
   const int64_t at = vector_at(row, head, a.pool_rows, a.P, a.Hkv);
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     const bool finite = top[p] < 0x7f800000u;
-    const float scale = finite ? __uint_as_float(top[p]) / code_top<CODE>() : __uint_as_float(0x7fc00000u);
+    const float scale = finite ? scale_of<CODE>(__uint_as_float(top[p])) : __uint_as_float(0x7fc00000u);
     u32x2 w = {0u, 0u};
     if (finite && scale > 0.f) w = encode8<CODE>(x[p], scale);
     const int64_t to = at + (p ? a.P * a.Hkv : 0);
