@@ -47,7 +47,7 @@ struct PagesArgs {
   SlotRange* ranges;                // [B] written by the MFMA kernel; null: `splits` slots a request
   int units, waves_units, subs;     // MFMA kernel: (KV head, 16 heads) units, of a workgroup, waves of one
   int64_t target, min_tiles;        // long: workgroups aimed at; both: the fewest tiles of a part
-  int q_vec;
+  int q_vec, o_vec;  // query and output rows aligned for vector loads and stores
   // short: tagged partial words [B, max_parts, Hq] m and l, [B, max_parts, Hq, D] o, and the
   // arrival counters [B, units] (arrive.h)
   unsigned long long *word_m, *word_l, *word_o, *arrivals;
@@ -76,6 +76,26 @@ __device__ __forceinline__ void store_any(void* base, int64_t i, float v, int dt
 
 // 2^x on the transcendental unit; scores and maxima are held in powers of two.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Four neighbouring elements, rounded; `vec` when the address allows one store.
+template <int DT>
+__device__ __forceinline__ void store_quad(void* base, int64_t i, f32x4 v, bool vec) {
+  if constexpr (DT == HS_DTYPE_F32) {
+    float* p = static_cast<float*>(base) + i;
+    if (vec) *reinterpret_cast<f32x4*>(p) = v;
+    else
+      for (int e = 0; e < 4; ++e) p[e] = v[e];
+  } else {
+    unsigned short* p = static_cast<unsigned short*>(base) + i;
+    const u32x2 w = {pack16<DT == HS_DTYPE_F16>(v[0], v[1]), pack16<DT == HS_DTYPE_F16>(v[2], v[3])};
+    if (vec) {
+      *reinterpret_cast<u32x2*>(p) = w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+}
 
 constexpr bool quantised(int S) { return S == HS_DTYPE_I8 || S == HS_DTYPE_E4M3; }
 
@@ -499,13 +519,17 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
   // reads the table for 32 of its tiles at once (lane l: half l), keeps the halves' byte offsets
   // in a register and takes each tile's from there; tiles without a page are passed over.
   // Else lanes 0-31 find their token's row, one tile ahead, and the others take it from them.
-  int32_t entry = 0;  // table entry of this lane's half (UNIFORM: in the next batch) or token (in the next tile)
+  // Table entry, and row within its page, of this lane's half (UNIFORM: in the next batch) or
+  // token (in the next tile).
+  int32_t entry = 0;
+  uint32_t within = 0;
   auto half_token = [&](int32_t batch) {  // first token of this lane's half in the batch
     return static_cast<uint32_t>(tile0 + sub + (batch + (lane >> 1)) * subs) * 32u + 16u * (lane & 1);
   };
   auto token_of = [&](int32_t tile) { return static_cast<uint32_t>(tile) * 32u + (lane & 31); };
   auto fetch = [&](uint32_t token) {
     const uint32_t page = token / P;
+    within = token - page * P;
     entry = table[page < pages ? page : 0u];
   };
   int32_t at_tile = tile0 + sub;  // !UNIFORM: the tile `entry` belongs to
@@ -725,13 +749,13 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
 
   if constexpr (UNIFORM) {
     const int32_t mine = tile1 - tile0 > sub ? (tile1 - tile0 - sub + subs - 1) / subs : 0;  // tiles of this wave
-    int32_t batch = 0;
+    int32_t batch = -32;  // none yet
     uint64_t present = 0;
     int64_t offset = 0;  // byte offset of the half's first K row of this KV head
     auto open = [&]() {  // the batch of `entry` becomes current, and the next one's table loads start
       const uint32_t t = half_token(batch);
       const bool ok = batch + (lane >> 1) < mine && t < static_cast<uint32_t>(n) && entry >= 0 && entry < a.blocks;
-      offset = ok ? ((static_cast<int64_t>(entry) * 2 * P + t % P) * a.Hkv + kv) * (D * ES) : 0;
+      offset = ok ? ((static_cast<int64_t>(entry) * 2 * P + within) * a.Hkv + kv) * (D * ES) : 0;
       present = __ballot(ok);
       if (batch + 32 < mine) fetch(half_token(batch + 32));
     };
@@ -787,18 +811,15 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
         for (int i = 0; i < VB / VL; ++i) load_words<VL>(p + v_lane[e & 3] + VL * i, &vw[e][i * 4]);
       }
     };
-    if (mine > 0) {
-      open();
-      if (advance()) {
-        load_k();
-        load_v();
-        split_query();
-        while (true) {
-          const uint32_t now = valid;
-          const bool more = advance();  // past the end the offsets stay: the last tile is read again, unused
-          use_tile(now, load_k, load_v);
-          if (!more) break;
-        }
+    if (advance()) {
+      load_k();
+      load_v();
+      split_query();
+      bool more = true;
+      while (more) {
+        const uint32_t now = valid;
+        more = advance();  // past the end the offsets stay: the last tile is read again, unused
+        use_tile(now, load_k, load_v);
       }
     }
   } else {
@@ -807,7 +828,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     auto advance = [&]() {
       const uint32_t t = token_of(at_tile);
       const bool ok = at_tile < tile1 && t < static_cast<uint32_t>(n) && entry >= 0 && entry < a.blocks;
-      row = ok ? (static_cast<int64_t>(entry) * 2 * P + t % P) * a.Hkv + kv : 0;
+      row = ok ? (static_cast<int64_t>(entry) * 2 * P + within) * a.Hkv + kv : 0;
       valid = static_cast<uint32_t>(__ballot(ok));
       at_tile += subs;
       fetch(token_of(at_tile));
@@ -904,9 +925,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     const int64_t head = static_cast<int64_t>(un / a.head_chunks) * a.g + first + h;
     if constexpr (SHORT) {
       if (sh.parts == 1) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          store_any(a.out, b * a.o_sb + head * a.o_sh + d + e, L != 0.f ? O[e] / L : 0.f, a.q_dtype);
+        store_quad<QD>(a.out, b * a.o_sb + head * a.o_sh + d, L != 0.f ? O * (1.f / L) : f32x4{0.f, 0.f, 0.f, 0.f}, a.o_vec);
       } else {
         const int64_t at = (b * a.max_parts + sh.part) * a.Hq + head;
         if (d == 0) {
@@ -963,26 +982,22 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     __syncthreads();
     for (int i = threadIdx.x; i < heads * D; i += 512) {
       const int h = i / D, d = i % D;
+      unsigned long long w[PM_PARTS];
+      unsigned long long* const at = a.word_o + (base + h) * D + d;
+      const int64_t next = a.Hq * D;
+#pragma unroll
+      for (int u = 0; u < PM_PARTS; ++u)  // all in flight, with no branch between them
+        w[u] = __hip_atomic_load(at + (u < sh.parts ? u : 0) * next, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       float O = 0.f;
-      for (int p0 = 0; p0 < sh.parts; p0 += 8) {
-        unsigned long long w[8];
-        unsigned long long* at[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int p = p0 + u < sh.parts ? p0 + u : p0;
-          at[u] = a.word_o + (base + p * a.Hq + h) * D + d;
-          w[u] = __hip_atomic_load(at[u], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (p0 + u >= sh.parts) continue;
-          if (static_cast<uint32_t>(w[u] >> 32) != tag) w[u] = partial_reread(at[u], tag);
-          __hip_atomic_store(at[u], 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          O += s_w[p0 + u][h] * partial_value(w[u]);
-        }
+      for (int u = 0; u < PM_PARTS; ++u) {
+        if (u >= sh.parts) continue;
+        if (static_cast<uint32_t>(w[u] >> 32) != tag) w[u] = partial_reread(at + u * next, tag);
+        __hip_atomic_store(at + u * next, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        O += s_w[u][h] * partial_value(w[u]);
       }
       const float L = s_sum[h];
-      store_any(a.out, b * a.o_sb + (kv * a.g + h0 + h) * a.o_sh + d, L != 0.f ? O / L : 0.f, a.q_dtype);
+      store_elem<QD>(a.out, b * a.o_sb + (kv * a.g + h0 + h) * a.o_sh + d, L != 0.f ? O / L : 0.f);
     }
     if (threadIdx.x == 0)  // a replay of this launch counts from zero in the next round
       __hip_atomic_store(counter,
@@ -1299,6 +1314,7 @@ extern "C" int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_
       a.subs = p.subs;
       a.target = p.target;
     }
+    a.o_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && o_stride_b % 4 == 0 && o_stride_h % 4 == 0;
     a.q_vec = reinterpret_cast<uintptr_t>(query) % 16 == 0 && q_stride_b % 8 == 0 && q_stride_h % 8 == 0;
     switch (pool_code) {
       case HS_DTYPE_F32: launch_mfma_pages<HS_DTYPE_F32, HS_DTYPE_F32>(p, a, stream); break;
