@@ -45,7 +45,7 @@ struct PagesArgs {
   float scale;
   float *part_m, *part_l, *part_o;  // [slots, Hq], [slots, Hq], [slots, Hq, D]
   SlotRange* ranges;                // [B] written by the MFMA kernel; null: `splits` slots a request
-  int units, waves_units, subs;     // MFMA kernel: (KV head, 16 heads) units, of a workgroup, waves of one
+  int units, waves_units, subs;     // MFMA kernel: (KV head, 16 heads) units; a workgroup's; waves of one
   int64_t target, min_tiles;        // long: workgroups aimed at; both: the fewest tiles of a part
   int q_vec, o_vec;  // query and output rows aligned for vector loads and stores
   // short: tagged partial words [B, max_parts, Hq] m and l, [B, max_parts, Hq, D] o, and the
@@ -450,7 +450,7 @@ __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& o
 // SHORT: few tokens in all.  Every unit has workgroups of its own (eight waves on its tiles), a
 // request `max_parts` at most, in a fixed grid, so that the table, the length and the query
 // load together; a part alone writes the output, several are joined by the last to arrive.
-// Else the schedule of share_of over workgroups of up to eight units (a page's rows are
+// Else the schedule of share_of over workgroups of up to four units (a page's rows are
 // contiguous over the KV heads), joined by pages_merge_kernel.
 template <int S, int QD, int D, bool UNIFORM, bool SHORT>
 __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
@@ -1134,14 +1134,15 @@ static PagesPlan plan_pages(bool mfma, int64_t elem, int64_t B, int64_t Hq, int6
       p.slots = (tiles + p.min_tiles - 1) / p.min_tiles;
       return p;
     }
-    p.waves_units = 8;
+    // Long: one workgroup a CU, of eight waves over up to four units.  us at 4 histories of 32768
+    // tokens, 14 query and 2 KV heads of 64 in bf16, for 256, 512 and 768 workgroups 20.4 21.4
+    // 24.2; 28 and 4 heads of 128 in int8 32.5 38.9 45.4; 16 of 16384, 40 and 8 heads of 128 in
+    // e4m3, with four units a workgroup 109, with eight 110, with one 192.
+    p.waves_units = 4;
     while (p.units % p.waves_units) --p.waves_units;
     p.subs = 8 / p.waves_units;
     const int64_t groups = p.units / p.waves_units;
-    // workgroups that run at once: one of eight waves on a CU at D = 128 (registers), else two
-    // (a second round half filled cost 202 us against 191 at 8 histories of 128k tokens)
-    const int64_t resident = D == 128 ? 256 : 512;
-    p.target = (resident + groups - 1) / groups;
+    p.target = (256 + groups - 1) / groups;
     p.min_tiles = p.subs;
     const int64_t most = B * ((tiles + p.min_tiles - 1) / p.min_tiles);
     p.slots = most < p.target + B ? most : p.target + B;
