@@ -199,12 +199,15 @@ def test_uneven_batches(gpu, code):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("int8", "f16"), ("e4m3", "f32")])
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("int8", "f16"), ("e4m3", "f32"), ("f16", "f16"),
+                                        ("bf16", "bf16")])
 def test_small_and_large_values(gpu, code, dtype):
-    """V rows of any size: the weights times a scale keep their precision (float16 queries too)."""
+    """V rows of any size: the weights times a scale keep their precision (float16 queries too),
+    and float16's subnormal values count (1e-6 is 17 of their steps)."""
     for amplitude in (1e-6, 1e-3, 2000.0):
-        args = case(2, 8, 2, 128, 16, [300, 1], code, dtype, gpu, amplitude=amplitude)
-        check(attend_pages(*args), args)
+        for wide in (2, WIDE):
+            args = case(2, 8, 2, 128, 16, [300, 1], code, dtype, gpu, amplitude=amplitude, wide=wide)
+            check(attend_pages(*args), args)
 
 
 @pytest.mark.gpu
