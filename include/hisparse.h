@@ -424,8 +424,8 @@ int hs_attend_window(const void* query, int64_t q_stride_h, const void* pool, in
  *            pages * P); rows past them are never used
  *   out      [batch, heads, head_dim] in query_dtype; 0 for a request without a token
  * Scores, softmax statistics and sums are fp32.  The workspace
- * (hs_attend_pages_workspace_bytes of the same sizes, 16-byte aligned) may hold anything
- * before a call; calls that share one must run in order.  Nothing is read on the host, so
+ * (hs_attend_pages_workspace_bytes of the same sizes; 0: none, null then; 16-byte aligned)
+ * may hold anything before a call; calls that share one must run in order.  Nothing is read on the host, so
  * a captured call replays with the tables and lengths of the moment.
  */
 int64_t hs_attend_pages_workspace_bytes(int32_t query_dtype, int32_t pool_code, int64_t batch, int64_t heads,

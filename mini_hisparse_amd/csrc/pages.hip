@@ -290,7 +290,12 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
         O += f * smem[(w * G + h) * D + d];
       }
     }
-    const int64_t at = (b * a.splits + split) * a.Hq + kv * a.g + h0 + h;
+    const int64_t head = kv * a.g + h0 + h;
+    if (a.splits == 1) {
+      store_any(a.out, b * a.o_sb + head * a.o_sh + d, L != 0.f ? O / L : 0.f, a.q_dtype);
+      continue;
+    }
+    const int64_t at = (b * a.splits + split) * a.Hq + head;
     if (d == 0) {
       a.part_m[at] = M;
       a.part_l[at] = L;
@@ -498,8 +503,10 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
   unsigned long long seen = 0;
   int32_t share, tile0;
   if constexpr (SHORT) {
-    counter = a.arrivals + b * a.units + unit;
-    seen = __hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (a.max_parts > 1) {  // else there is no workspace
+      counter = a.arrivals + b * a.units + unit;
+      seen = __hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     share = static_cast<int32_t>(a.min_tiles);
     tile0 = sh.part * share;
   }
@@ -1107,10 +1114,15 @@ struct PagesPlan {
   int64_t target, min_tiles, slots;
 };
 
-static bool pages_mfma_shape(int64_t D) { return D == 32 || D == 64 || D == 128; }
+// The MFMA kernel's shapes: its lane offsets within 16 rows are 32-bit.
+static bool pages_mfma_shape(int64_t elem, int64_t Hkv, int64_t D) {
+  return (D == 32 || D == 64 || D == 128) && Hkv * D * elem < (int64_t{1} << 27);
+}
 
 // Splits of the token axis: about 2048 workgroups, each with at least one tile per wave.
-static PagesPlan plan_pages(bool mfma, int64_t elem, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t tokens) {
+// `whole`: the general kernel takes a request in one split (the workspace was sized for a kernel
+// that needs none).
+static PagesPlan plan_pages(bool mfma, bool whole, int64_t elem, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t tokens) {
   PagesPlan p{};
   const int64_t g = Hq / Hkv;
   p.mfma = mfma;
@@ -1154,6 +1166,7 @@ static PagesPlan plan_pages(bool mfma, int64_t elem, int64_t B, int64_t Hq, int6
   int64_t splits = (2048 + groups - 1) / groups;
   const int64_t cap = (tokens + PG_T - 1) / PG_T;
   if (splits > cap) splits = cap;
+  if (whole || tokens <= 2 * PG_T) splits = 1;  // written without a join: one launch
   if (splits < 1) splits = 1;
   p.chunk = ((tokens + splits - 1) / splits + PG_T - 1) / PG_T * PG_T;
   if (p.chunk < PG_T) p.chunk = PG_T;
@@ -1165,7 +1178,8 @@ static PagesPlan plan_pages(bool mfma, int64_t elem, int64_t B, int64_t Hq, int6
 
 // Partials (m, l, o) of every slot and query head, and the requests' slot ranges.
 static int64_t pages_workspace(const PagesPlan& p, int64_t B, int64_t Hq, int64_t D) {
-  if (p.mfma && p.brief) return (B * p.slots * Hq * (D + 2) + B * p.units) * 8;
+  if (!p.mfma && p.splits == 1) return 0;
+  if (p.mfma && p.brief) return p.slots == 1 ? 0 : (B * p.slots * Hq * (D + 2) + B * p.units) * 8;
   return p.slots * Hq * (D + 2) * 4 + B * static_cast<int64_t>(sizeof(SlotRange)) + 8;
 }
 
@@ -1237,15 +1251,15 @@ extern "C" int64_t hs_attend_pages_workspace_bytes(int32_t query_dtype, int32_t 
                                                    int64_t heads, int64_t kv_heads, int64_t head_dim,
                                                    int64_t page_size, int64_t pages) {
   if (check_pages(batch, heads, kv_heads, head_dim, page_size, pages)) return 256;
-  // either kernel may run on it (a pool that is not 16-byte aligned goes to the general one)
-  int64_t need = 0;
-  for (const bool mfma : {false, true}) {
-    if (mfma && !pages_mfma_shape(head_dim)) continue;
-    const int64_t bytes = pages_workspace(plan_pages(mfma, pool_elem_bytes(pool_code), batch, heads, kv_heads, head_dim, pages * page_size), batch,
-                                          heads, head_dim);
-    need = bytes > need ? bytes : need;
-  }
-  return need;
+  const int64_t elem = pool_elem_bytes(pool_code), tokens = pages * page_size;
+  const bool shape = pages_mfma_shape(elem, kv_heads, head_dim);
+  const int64_t need = pages_workspace(plan_pages(shape, false, elem, batch, heads, kv_heads, head_dim, tokens), batch,
+                                       heads, head_dim);
+  if (!shape) return need;
+  // a pool that is not 16-byte aligned goes to the general kernel
+  const int64_t other = pages_workspace(plan_pages(false, need == 0, elem, batch, heads, kv_heads, head_dim, tokens),
+                                        batch, heads, head_dim);
+  return need > other ? need : other;
 }
 
 extern "C" int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_stride_h, int32_t query_dtype,
@@ -1262,11 +1276,15 @@ extern "C" int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_
   HS_CHECK_ARG(query && pool && tables && lengths && out, "null page attention pointer");
   HS_CHECK_ARG(valid_code(pool_code) == (scales != nullptr), "scales go with a quantised pool, and only with one");
   HS_CHECK_ARG(blocks >= 1 && blocks <= 0x7fffffff, "a pool has 1 to 2^31 - 1 blocks");
-  const bool mfma = pages_mfma_shape(head_dim) && reinterpret_cast<uintptr_t>(pool) % 16 == 0 &&
-                    kv_heads * head_dim * pool_elem_bytes(pool_code) < (int64_t{1} << 27);  // 32-bit lane offsets
-  const PagesPlan p = plan_pages(mfma, pool_elem_bytes(pool_code), batch, heads, kv_heads, head_dim, pages * page_size);
+  const int64_t elem = pool_elem_bytes(pool_code), tokens = pages * page_size;
+  const bool shape = pages_mfma_shape(elem, kv_heads, head_dim);
+  const bool mfma = shape && reinterpret_cast<uintptr_t>(pool) % 16 == 0;
+  PagesPlan p = plan_pages(shape, false, elem, batch, heads, kv_heads, head_dim, tokens);
+  if (shape && !mfma)
+    p = plan_pages(false, pages_workspace(p, batch, heads, head_dim) == 0, elem, batch, heads, kv_heads, head_dim, tokens);
   const int64_t need = pages_workspace(p, batch, heads, head_dim);
-  HS_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+  HS_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need &&
+                             (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                "page attention workspace too small or unaligned: need %lld bytes", static_cast<long long>(need));
   PagesArgs a{};
   a.q = query;
@@ -1335,7 +1353,7 @@ extern "C" int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_
     }
   }
   HS_CHECK_LAUNCH("page attention");
-  if (p.mfma && p.brief) return HS_OK;
+  if (p.mfma ? p.brief : p.splits == 1) return HS_OK;
   const int64_t columns = PJ_T * (head_dim % 4 == 0 ? 4 : 1);
   const dim3 joins(static_cast<unsigned>(heads), static_cast<unsigned>(batch),
                    static_cast<unsigned>((head_dim + columns - 1) / columns));

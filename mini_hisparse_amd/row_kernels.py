@@ -286,15 +286,14 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
     """
     quantized = isinstance(pool, QuantizedPool)
     store = pool.codes if quantized else pool
-    if query.dim() != 3 or store.dim() != 5:
+    shape, s_shape, device = query.shape, store.shape, query.device
+    if len(shape) != 3 or len(s_shape) != 5 or s_shape[1] != 2 or 0 in shape or 0 in s_shape:
         raise ValueError("attend_pages takes query [B, Hq, D] and a pool [blocks, 2, page_size, kv_heads, head_dim]")
-    batch, heads, dim = query.shape
-    blocks, planes, page_size, kv_heads, head_dim = store.shape
-    if planes != 2 or not (batch and heads and dim and blocks and page_size and kv_heads):
-        raise ValueError("attend_pages takes query [B, Hq, D] and a pool [blocks, 2, page_size, kv_heads, head_dim]")
+    batch, heads, dim = shape
+    blocks, _, page_size, kv_heads, head_dim = s_shape
     if dim != head_dim or heads % kv_heads or dim > 512:
         raise ValueError("query and pool differ in head_dim (at most 512), or query heads are no multiple of KV heads")
-    code, device = _lib.dtype_code(query.dtype), query.device
+    code = _lib.dtype_code(query.dtype)
     if quantized:
         pool_code, scales = pool.code, pool.scales.data_ptr()
     elif store.dtype != query.dtype:
@@ -303,16 +302,16 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
         raise ValueError("attend_pages needs a contiguous pool")
     else:
         pool_code, scales = code, None
-    per_head = tables.dim() == 3
     t_shape, t_stride = tables.shape, tables.stride()
-    if tables.dtype != torch.int32 or t_shape[:-1] != ((batch, kv_heads) if per_head else (batch,)) \
-            or t_shape[-1] < 1 or t_stride[-1] != 1 and t_shape[-1] > 1:
+    pages, per_head = t_shape[-1] if t_shape else 0, len(t_shape) == 3
+    if tables.dtype != torch.int32 or t_shape != ((batch, kv_heads, pages) if per_head else (batch, pages)) \
+            or pages < 1 or t_stride[-1] != 1 and pages > 1:
         raise ValueError("page tables must be int32 [B, pages] or [B, kv_heads, pages] of unit inner stride")
     if lengths.dtype != torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous():
         raise ValueError("lengths must be contiguous int32 [B]")
     if store.device != device or tables.device != device or lengths.device != device:
         raise ValueError("query, pool, tables and lengths must be on one device")
-    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.device != device
+    if out is not None and (out.shape != shape or out.dtype != query.dtype or out.device != device
                             or not out.is_contiguous()):
         raise ValueError("attend_pages: out must be contiguous, of the query's shape, dtype and device")
     if device.type != "cuda":
@@ -321,16 +320,15 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
     if q_stride[2] != 1 and dim > 1:
         query = query.contiguous()
         q_stride = query.stride()
-    result = torch.empty_like(query, memory_format=torch.contiguous_format) if out is None else out
-    pages = t_shape[-1]
+    result = query.new_empty(shape) if out is None else out
     nbytes = _pages_workspace_bytes(code, pool_code, batch, heads, kv_heads, dim, page_size, pages)
     with _lib.on_device(device):
         # a workspace of this call's own: calls on other streams and captured graphs share none
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         status = _lib.load().hs_attend_pages(
             query.data_ptr(), q_stride[0], q_stride[1], code, store.data_ptr(), scales, pool_code, blocks, page_size,
             kv_heads, dim, tables.data_ptr(), t_stride[0], t_stride[1] if per_head else 0, pages, lengths.data_ptr(),
-            batch, heads, result.data_ptr(), heads * dim, dim, workspace.data_ptr(), nbytes,
+            batch, heads, result.data_ptr(), heads * dim, dim, workspace.data_ptr() if nbytes else None, nbytes,
             _lib.stream_handle(device),
         )
     if status:

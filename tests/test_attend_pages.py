@@ -260,14 +260,17 @@ def test_strides_outputs_and_misaligned_buffers(gpu, code, dtype):
     got = attend_pages(query, pool, tables, lengths, out=guarded[1:4])
     assert got.data_ptr() == guarded[1].data_ptr() and torch.equal(got, want)
     assert (guarded[0] == 9).all() and (guarded[4] == 9).all()
-    # a pool that starts at an odd element: same result from the element-wise kernel
+    # a pool that starts at an odd element: the element-wise kernel, on a workspace of any size
     store = pool.codes if code in CODES else pool
     room = torch.empty(store.numel() + 1, dtype=torch.int8 if code in CODES else store.dtype, device=gpu)
     moved = room[1:].view(store.shape)
     moved.copy_(store.view(room.dtype))
     moved = QuantizedPool(moved.view(store.dtype), pool.scales) if code in CODES else moved
-    args = (query, moved, tables, lengths)
-    check(attend_pages(*args), args)
+    for columns in (tables.shape[1], 400, 30_000):  # one part, a few, the long launch
+        padded = torch.full((3, columns), -1, dtype=torch.int32, device=gpu)
+        padded[:, : tables.shape[1]] = tables
+        args = (query, moved, padded, lengths)
+        check(attend_pages(*args), args)
 
 
 @pytest.mark.gpu
@@ -389,8 +392,8 @@ def test_entry_point_refusals_without_a_gpu():
     at = ctypes.addressof(buffer)
     at += -at % 16
 
-    def call(q=at, qd=2, pool=at, scales=at, code=3, blocks=4, page=16, kv=1, dim=64, tables=at, pages=1, lengths=at,
-             batch=1, heads=2, out=at, ws=at, nbytes=1 << 40):
+    def call(q=at, qd=2, pool=at, scales=at, code=3, blocks=4, page=16, kv=1, dim=64, tables=at, pages=1000,
+             lengths=at, batch=1, heads=2, out=at, ws=at, nbytes=1 << 40):
         return lib.hs_attend_pages(q, heads * dim, dim, qd, pool, scales, code, blocks, page, kv, dim, tables, pages,
                                    0, pages, lengths, batch, heads, out, heads * dim, dim, ws, nbytes, None)
 
@@ -402,4 +405,5 @@ def test_entry_point_refusals_without_a_gpu():
         assert call(**bad) == -1, bad
         assert lib.hs_last_error()
     size = lib.hs_attend_pages_workspace_bytes
-    assert size(2, 3, 0, 1, 1, 64, 16, 1) == 256 and size(2, 3, 4, 14, 2, 64, 16, 100) > 0
+    assert size(2, 3, 0, 1, 1, 64, 16, 1) == 256
+    assert size(2, 3, 4, 14, 2, 64, 16, 10) == 0 and size(2, 3, 4, 14, 2, 64, 16, 1000) > 0  # one part, several
