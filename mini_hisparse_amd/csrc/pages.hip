@@ -963,16 +963,34 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     __syncthreads();
     if (!s_last) return;
     const int64_t base = b * a.max_parts * a.Hq + kv * a.g + h0;  // word of head h, part p: base + p * Hq + h
-    auto word = [&](unsigned long long* p) {
-      unsigned long long w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (static_cast<uint32_t>(w >> 32) != tag) w = partial_reread(p, tag);
+    const int64_t next = a.Hq * D;                                // from a part's o word to the next part's
+    // Every word goes out before any is used, with no branch between them (a part past the last
+    // reads part 0's again): o words of the thread's (head, dim) pairs, then its m and its l.
+    constexpr int PAIRS = (16 * D + 511) / 512;
+    unsigned long long w[PAIRS][PM_PARTS];
+    auto pair_word = [&](int r) {
+      const int i = threadIdx.x + 512 * r < heads * D ? threadIdx.x + 512 * r : 0;
+      return a.word_o + (base + i / D) * D + i % D;
+    };
+#pragma unroll
+    for (int r = 0; r < PAIRS; ++r) {
+      if (512 * r >= heads * D) continue;
+#pragma unroll
+      for (int u = 0; u < PM_PARTS; ++u)
+        w[r][u] = __hip_atomic_load(pair_word(r) + (u < sh.parts ? u : 0) * next, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    auto taken = [&](unsigned long long* p, unsigned long long v) {  // a word's value, the word cleared
+      if (static_cast<uint32_t>(v >> 32) != tag) v = partial_reread(p, tag);
       __hip_atomic_store(p, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      return partial_value(w);
+      return partial_value(v);
     };
     if (threadIdx.x < sh.parts * 16 && (threadIdx.x & 15) < heads) {
       const int i = threadIdx.x, p = i >> 4, h = i & 15;
-      s_w[p][h] = word(a.word_m + base + p * a.Hq + h);
-      smem[i] = word(a.word_l + base + p * a.Hq + h);
+      unsigned long long *pm = a.word_m + base + p * a.Hq + h, *pl = a.word_l + base + p * a.Hq + h;
+      const unsigned long long vm = __hip_atomic_load(pm, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const unsigned long long vl = __hip_atomic_load(pl, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_w[p][h] = taken(pm, vm);
+      smem[i] = taken(pl, vl);
     }
     __syncthreads();
     if (threadIdx.x < heads) {
@@ -987,22 +1005,16 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
       s_sum[h] = L;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * D; i += 512) {
-      const int h = i / D, d = i % D;
-      unsigned long long w[PM_PARTS];
-      unsigned long long* const at = a.word_o + (base + h) * D + d;
-      const int64_t next = a.Hq * D;
 #pragma unroll
-      for (int u = 0; u < PM_PARTS; ++u)  // all in flight, with no branch between them
-        w[u] = __hip_atomic_load(at + (u < sh.parts ? u : 0) * next, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int r = 0; r < PAIRS; ++r) {
+      const int i = threadIdx.x + 512 * r;
+      if (i >= heads * D) continue;
+      const int h = i / D, d = i % D;
+      unsigned long long* const at = pair_word(r);
       float O = 0.f;
 #pragma unroll
-      for (int u = 0; u < PM_PARTS; ++u) {
-        if (u >= sh.parts) continue;
-        if (static_cast<uint32_t>(w[u] >> 32) != tag) w[u] = partial_reread(at + u * next, tag);
-        __hip_atomic_store(at + u * next, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        O += s_w[u][h] * partial_value(w[u]);
-      }
+      for (int u = 0; u < PM_PARTS; ++u)
+        if (u < sh.parts) O += s_w[u][h] * taken(at + u * next, w[r][u]);
       const float L = s_sum[h];
       store_elem<QD>(a.out, b * a.o_sb + (kv * a.g + h0 + h) * a.o_sh + d, L != 0.f ? O / L : 0.f);
     }
