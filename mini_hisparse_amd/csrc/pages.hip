@@ -305,22 +305,22 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
 }
 
 // ---- the matrix-core kernel ---------------------------------------------------------------
-// Head dims of 32, 64 and 128.  A wave owns one unit (a KV head and
-// up to 16 of its query heads) and walks tiles of 32 tokens, with no shared memory:
+// Head dims of 32, 64, 96 and 128.  A wave owns one unit (a KV head and up to 16 of its query
+// heads) and walks tiles of 32 tokens, with no shared memory:
 //
 //   S^T = K Q^T   A: K rows (lane (j, c): row c, 8 of the head dim), B: the heads' queries;
 //                 lane (j, c) receives head c's scores of tokens 4j .. 4j+3 and 16 + those
 //   O^T += V^T P  B: those eight scores' weights, held already where the product wants them;
 //                 A: lane (j, c) the same eight tokens' V at dims (D/16) c .., so that a V row
-//                 is one contiguous load of the 16 lanes of a group and the transpose is the
-//                 pairing of two tokens in a register
+//                 is one contiguous load of the 16 lanes of a group (of 96 dims two: 4c .. and
+//                 64 + 2c ..) and the transpose is the pairing of two tokens in a register
 //
 // with (j, c) = (lane / 16, lane % 16).  Codes widen to bf16 in registers (exact); queries and
 // weights go in as sums of bf16 parts: as many of the query as its type has significand (1
 // for bf16, 2 for float16, 3 for float32) and of the weights two (2^-16 of a weight; three
 // for float32 queries).  float16 pools use float16 products, float32 pools float32 ones (four
-// of the head dim, or four tokens, at a time; the same lanes hold the same values).  A tile's scales are one dword a
-// lane, spread over the group by the broadcast of the multiply itself.
+// of the head dim, or four tokens, at a time; the same lanes hold the same values).  A tile's
+// scales are one dword a lane, spread over the group by the broadcast of the multiply itself.
 // The running maximum moves only when a score passes it by more than SLACK (the sums then
 // hold weights up to 2^SLACK, no less precise): no cross-lane step in most tiles.
 
@@ -465,11 +465,13 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
   constexpr int E = D / 16;                  // V elements of a lane and token
   constexpr int NQ = query_parts<S, QD>(), NP = weight_parts<S, QD>();
   constexpr int KROW = D / 4 * ES;           // K bytes of a lane and row
-  constexpr int KL = KROW < 16 ? KROW : 16;  // a K load
+  constexpr int KL = KROW < 16 ? KROW : (KROW % 16 ? 8 : 16);  // a K load
   constexpr int KN = KROW / KL;
-  constexpr int VB = E * ES;                 // V bytes of a lane and token
+  constexpr int E0 = D == 96 ? 4 : E;        // V elements of a lane and token in its first load(s)
+  constexpr int VB = E0 * ES;                // their bytes
   constexpr int VL = VB < 16 ? VB : 16;      // a V load
-  constexpr int VW = VB < 4 ? 1 : VB / 4;
+  constexpr int VB1 = (E - E0) * ES;         // bytes of the second part, from dim 16 E0
+  constexpr int VW0 = VB < 4 ? 1 : VB / 4, VW = VW0 + (VB1 + 3) / 4;
   constexpr int SD = D + 4;                  // row stride of the waves' sums in LDS: no bank conflicts
   extern __shared__ __attribute__((aligned(16))) float smem[];
   __shared__ float s_m[8][16], s_l[8][16];
@@ -523,7 +525,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
   }
 
   // UNIFORM: pages of a multiple of 16 rows, so a tile's two halves lie in one page each.  A wave
-  // reads the table for 32 of its tiles at once (lane l: half l), keeps the halves' byte offsets
+  // reads the table for 32 of its tiles at once (lane l: half l), keeps the halves' first rows
   // in a register and takes each tile's from there; tiles without a page are passed over.
   // Else lanes 0-31 find their token's row, one tile ahead, and the others take it from them.
   // Table entry, and row within its page, of this lane's half (UNIFORM: in the next batch) or
@@ -547,7 +549,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
   // of the lane's kk-th K word
   auto d0_of = [&](int kk) {
     return F32 ? 16 * (kk >> 2) + 4 * j + (kk & 3)
-               : (ES == 1 && D >= 64 ? 64 * (kk >> 1) + 16 * j + 8 * (kk & 1) : 32 * kk + 8 * j);
+               : (ES == 1 && KL == 16 ? 64 * (kk >> 1) + 16 * j + 8 * (kk & 1) : 32 * kk + 8 * j);
   };
   const bool live = c < heads;
   const int64_t q_at = b * a.q_sb + (kv * a.g + h0 + (live ? c : 0)) * a.q_sh;
@@ -758,11 +760,11 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     const int32_t mine = tile1 - tile0 > sub ? (tile1 - tile0 - sub + subs - 1) / subs : 0;  // tiles of this wave
     int32_t batch = -32;  // none yet
     uint64_t present = 0;
-    int64_t offset = 0;  // byte offset of the half's first K row of this KV head
+    int64_t offset = 0;  // the half's first K row of this KV head, in head vectors
     auto open = [&]() {  // the batch of `entry` becomes current, and the next one's table loads start
       const uint32_t t = half_token(batch);
       const bool ok = batch + (lane >> 1) < mine && t < static_cast<uint32_t>(n) && entry >= 0 && entry < a.blocks;
-      offset = ok ? ((static_cast<int64_t>(entry) * 2 * P + within) * a.Hkv + kv) * (D * ES) : 0;
+      offset = ok ? (static_cast<int64_t>(entry) * 2 * P + within) * a.Hkv + kv : 0;
       present = __ballot(ok);
       if (batch + 32 < mine) fetch(half_token(batch + 32));
     };
@@ -797,25 +799,27 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     const uint32_t s_lane = static_cast<uint32_t>(s_token) * static_cast<uint32_t>(a.Hkv);
     uint32_t v_lane[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v_lane[e] = (4 * j + e) * row_bytes + c * VB;
+    for (int e = 0; e < 4; ++e) v_lane[e] = (4 * j + e) * row_bytes;
+    const uint32_t v_col = c * VB, v_col1 = 16 * VB + c * VB1;
     auto load_k = [&]() {
       if constexpr (quantised(S)) {
-        const uint64_t row = (s_half ? off1 : off0) / (D * ES) + (c >= 8 ? a.P * a.Hkv : 0);
+        const uint64_t row = (s_half ? off1 : off0) + (c >= 8 ? a.P * a.Hkv : 0);
         sc = a.scales[row + s_lane];
       }
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt) {
-        const char* p = pool + (rt ? off1 : off0);
+        const char* p = pool + (rt ? off1 : off0) * (D * ES);
 #pragma unroll
-        for (int i = 0; i < KN; ++i) load_words<KL>(p + k_lane + 64 * i, &kw[rt][i * (KL / 4)]);
+        for (int i = 0; i < KN; ++i) load_words<KL>(p + k_lane + 4 * KL * i, &kw[rt][i * (KL / 4)]);
       }
     };
     auto load_v = [&]() {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const char* p = pool + v_plane + (e < 4 ? off0 : off1);
+        const char* p = pool + v_plane + (e < 4 ? off0 : off1) * (D * ES);
 #pragma unroll
-        for (int i = 0; i < VB / VL; ++i) load_words<VL>(p + v_lane[e & 3] + VL * i, &vw[e][i * 4]);
+        for (int i = 0; i < VB / VL; ++i) load_words<VL>(p + (v_lane[e & 3] + v_col) + VL * i, &vw[e][i * 4]);
+        if constexpr (VB1 > 0) load_words<VB1>(p + (v_lane[e & 3] + v_col1), &vw[e][VW0]);
       }
     };
     if (advance()) {
@@ -847,15 +851,16 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
       for (int rt = 0; rt < 2; ++rt) {
         const char* p = pool + row_of(16 * rt + c) * (D * ES) + j * KL;
 #pragma unroll
-        for (int i = 0; i < KN; ++i) load_words<KL>(p + 64 * i, &kw[rt][i * (KL / 4)]);
+        for (int i = 0; i < KN; ++i) load_words<KL>(p + 4 * KL * i, &kw[rt][i * (KL / 4)]);
       }
     };
     auto load_v = [&]() {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const char* p = pool + row_of(16 * (e >> 2) + 4 * j + (e & 3)) * (D * ES) + v_plane + c * VB;
+        const char* p = pool + row_of(16 * (e >> 2) + 4 * j + (e & 3)) * (D * ES) + v_plane;
 #pragma unroll
-        for (int i = 0; i < VB / VL; ++i) load_words<VL>(p + VL * i, &vw[e][i * 4]);
+        for (int i = 0; i < VB / VL; ++i) load_words<VL>(p + c * VB + VL * i, &vw[e][i * 4]);
+        if constexpr (VB1 > 0) load_words<VB1>(p + 16 * VB + c * VB1, &vw[e][VW0]);
       }
     };
     if (at_tile < tile1) {
@@ -873,6 +878,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     }
   }
 
+  auto dim_of = [](int v_lane, int e) { return e < E0 ? E0 * v_lane + e : 16 * E0 + (E - E0) * v_lane + e - E0; };
   // the totals of a head over the four groups, then the waves of a unit, then the partial
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
@@ -887,7 +893,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) a.part_o[at * D + E * (4 * j + i) + e] = acc[e][i];
+        for (int e = 0; e < E; ++e) a.part_o[at * D + dim_of(4 * j + i, e)] = acc[e][i];
       }
     }
     return;
@@ -901,7 +907,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) smem[(wave * rows + c) * SD + E * (4 * j + i) + e] = acc[e][i];
+      for (int e = 0; e < E; ++e) smem[(wave * rows + c) * SD + dim_of(4 * j + i, e)] = acc[e][i];
     }
   }
   __syncthreads();
@@ -1027,8 +1033,8 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
 }
 
 // out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a head's slots; 0 if all are empty.
-// One workgroup per (query head, request; and 256 C of the head dim).  The slots' weights go to LDS, one slot a thread;
-// then the sums: C elements a lane, 256 / (D / C) slots abreast and PJ_U of each in flight, so
+// One workgroup per (query head, request; and 256 C of the head dim).  The slots' weights go to
+// LDS, one slot a thread; then the sums: C elements a lane, 256 / (D / C) slots abreast and PJ_U of each in flight, so
 // that a long history's slots are a few rounds of loads (one slot after another took 66 of
 // 87 us at 128 slots of D = 64), joined over LDS in a fixed order.
 constexpr int PJ_T = 256;
@@ -1126,9 +1132,11 @@ struct PagesPlan {
   int64_t target, min_tiles, slots;
 };
 
-// The MFMA kernel's shapes: its lane offsets within 16 rows are 32-bit.
+// The MFMA kernel's shapes: its lane offsets within 16 rows are 32-bit.  (16 requests of 4096
+// tokens, 32 query and 8 KV heads: of 96 on the vector unit 64.8 us in int8 and 78.5 in bf16, here
+// 30.6 and 38.7; of 80, which the vector unit keeps, 55.8 and 65.2.)
 static bool pages_mfma_shape(int64_t elem, int64_t Hkv, int64_t D) {
-  return (D == 32 || D == 64 || D == 128) && Hkv * D * elem < (int64_t{1} << 27);
+  return (D == 32 || D == 64 || D == 96 || D == 128) && Hkv * D * elem < (int64_t{1} << 27);
 }
 
 // Splits of the token axis: about 2048 workgroups, each with at least one tile per wave.
@@ -1216,6 +1224,7 @@ static void launch_mfma_pages(const PagesPlan& p, const PagesArgs& a, hipStream_
   } while (0)
   if (a.D == 32) HS_PAGES_D(32);
   else if (a.D == 64) HS_PAGES_D(64);
+  else if (a.D == 96) HS_PAGES_D(96);
   else HS_PAGES_D(128);
 #undef HS_PAGES_D
 #undef HS_PAGES_RUN
@@ -1242,7 +1251,6 @@ static void launch_general(const PagesPlan& p, const PagesArgs& a, bool vec, hip
     else hipLaunchKernelGGL((pages_general_kernel<S, 1, 4, 8>), grid, dim3(PG_T), smem, s, a);
   }
 }
-
 
 static int check_pages(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
                        int64_t pages) {
