@@ -28,6 +28,10 @@ namespace hs {
 struct SlotRange {
   int32_t first, count;
 };
+// A workgroup's share: part `part` of the `parts` of request b, which has n tokens.
+struct alignas(16) Slot {
+  int32_t b, part, parts, n;
+};
 
 struct PagesArgs {
   const void* q;
@@ -45,6 +49,7 @@ struct PagesArgs {
   float scale;
   float *part_m, *part_l, *part_o;  // [slots, Hq], [slots, Hq], [slots, Hq, D]
   SlotRange* ranges;                // [B] written by the MFMA kernel; null: `splits` slots a request
+  Slot* shares;                     // long, above PM_LANES requests: the schedule written out
   int units, waves_units, subs;     // MFMA kernel: (KV head, 16 heads) units; a workgroup's; waves of one
   int64_t target, min_tiles;        // long: workgroups aimed at; both: the fewest tiles of a part
   int q_vec, o_vec;  // query and output rows aligned for vector loads and stores
@@ -326,6 +331,7 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
 
 constexpr int PM_TILE = 32;
 constexpr int PM_PARTS = 8;  // parts of a short request
+constexpr int PM_LANES = 64;  // requests whose schedule a wave derives by itself
 constexpr float PM_SLACK = 6.f;
 
 template <int S>
@@ -411,45 +417,87 @@ __device__ __forceinline__ T scan_lanes(T v) {
   return v;
 }
 
-// The request and part of workgroup w: every wave derives the same schedule from the lengths.
+// A request's tokens, at most `limit`, and their tiles.
+__device__ __forceinline__ int32_t clamp_length(int64_t n, int64_t limit) {
+  return static_cast<int32_t>(n < 0 ? 0 : (n < limit ? n : limit));
+}
+__device__ __forceinline__ int32_t tiles_of(int32_t n) {
+  return static_cast<int32_t>((static_cast<uint32_t>(n) + PM_TILE - 1) / PM_TILE);
+}
+
 // Parts are of `per` tiles, the fewest for which all requests together need at most `target`
 // workgroups (sum ceil(n_b / per) <= sum n_b / per + B); an empty request has one part.
+__device__ __forceinline__ uint32_t part_room(const PagesArgs& a) {
+  return static_cast<uint32_t>(a.target - (a.B < a.target / 2 ? a.B : a.target / 2));
+}
+__device__ __forceinline__ int32_t parts_of(int32_t tiles, uint32_t per) {
+  return tiles > static_cast<int64_t>(per) ? static_cast<int32_t>((static_cast<uint32_t>(tiles) + per - 1) / per) : 1;
+}
+
+// The request and part of workgroup w, of up to PM_LANES requests: every wave derives the same
+// schedule from the lengths, one request a lane.
 __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& out) {
   const int lane = threadIdx.x & 63;
-  const int64_t limit = a.pages * a.P;
-  auto length_at = [&](int64_t b) {
-    const int64_t n = a.lengths[b < a.B ? b : 0];
-    return b < a.B && n > 0 ? static_cast<int32_t>(n < limit ? n : limit) : 0;
-  };
-  auto tiles_of = [](int32_t n) { return static_cast<int32_t>((static_cast<uint32_t>(n) + PM_TILE - 1) / PM_TILE); };
-  const int32_t first = length_at(lane);
-  float total = static_cast<float>(tiles_of(first));
-  for (int64_t b0 = 64; b0 < a.B; b0 += 64) total += static_cast<float>(tiles_of(length_at(b0 + lane)));
-  total = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scan_lanes(total)), 63));
-  const uint32_t room = static_cast<uint32_t>(a.target - (a.B < a.target / 2 ? a.B : a.target / 2));
+  const int32_t n = lane < a.B ? clamp_length(a.lengths[lane], a.pages * a.P) : 0, tiles = tiles_of(n);
+  const float total =
+      __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scan_lanes(static_cast<float>(tiles))), 63));
+  const uint32_t room = part_room(a);
   // exact below 2^24 tiles; above, more than the sum's roundings can have lost
   uint32_t per = total < 0x1p24f ? (static_cast<uint32_t>(total) + room - 1) / room
                                  : static_cast<uint32_t>(total / static_cast<float>(room) * 1.0001f) + 1u;
   if (per < static_cast<uint32_t>(a.min_tiles)) per = static_cast<uint32_t>(a.min_tiles);
+  const int32_t parts = lane < a.B ? parts_of(tiles, per) : 0, through = scan_lanes(parts);
+  const uint64_t owners = __ballot(through > w);
+  if (!owners) return false;
+  const int src = __ffsll(static_cast<unsigned long long>(owners)) - 1;
+  out.b = src;
+  out.n = __builtin_amdgcn_readlane(n, src);
+  out.parts = __builtin_amdgcn_readlane(parts, src);
+  out.part = w - (__builtin_amdgcn_readlane(through, src) - out.parts);
+  out.slot = w;
+  return true;
+}
+
+// The same schedule for more requests, written out once: a workgroup's share (request -1: none)
+// and the requests' slots.  One workgroup; 1024 requests at a time.
+constexpr int PS_T = 1024;
+
+__global__ __launch_bounds__(PS_T) void pages_schedule_kernel(PagesArgs a, int64_t slots) {
+  __shared__ int64_t s_tiles[PS_T / 64];
+  __shared__ int32_t s_parts[2][PS_T / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t limit = a.pages * a.P;
+  int64_t total = 0;
+  for (int64_t b = threadIdx.x; b < a.B; b += PS_T) total += tiles_of(clamp_length(a.lengths[b], limit));
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(static_cast<long long>(total), off, 64);
+  if (lane == 0) s_tiles[wave] = total;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < PS_T / 64; ++w) total += s_tiles[w];
+  const int64_t room = part_room(a), fewest = (total + room - 1) / room;
+  const uint32_t per = static_cast<uint32_t>(fewest < a.min_tiles ? a.min_tiles : fewest);
   int32_t before = 0;
-  for (int64_t b0 = 0; b0 < a.B; b0 += 64) {
-    const int32_t n = b0 ? length_at(b0 + lane) : first;
-    const uint32_t tiles = static_cast<uint32_t>(tiles_of(n));
-    const int32_t parts = b0 + lane >= a.B ? 0 : (tiles > per ? static_cast<int32_t>((tiles + per - 1) / per) : 1);
-    const int32_t through = before + scan_lanes(parts);
-    const uint64_t owners = __ballot(through > w);
-    if (owners) {
-      const int src = __ffsll(static_cast<unsigned long long>(owners)) - 1;
-      out.b = b0 + src;
-      out.n = __builtin_amdgcn_readlane(n, src);
-      out.parts = __builtin_amdgcn_readlane(parts, src);
-      out.part = w - (__builtin_amdgcn_readlane(through, src) - out.parts);
-      out.slot = w;
-      return true;
+  for (int64_t b0 = 0, turn = 0; b0 < a.B; b0 += PS_T, turn ^= 1) {
+    const int64_t b = b0 + threadIdx.x;
+    const int32_t n = b < a.B ? clamp_length(a.lengths[b], limit) : 0;
+    const int32_t parts = b < a.B ? parts_of(tiles_of(n), per) : 0;
+    int32_t through = scan_lanes(parts);
+    if (lane == 63) s_parts[turn][wave] = through;
+    __syncthreads();  // the next turn writes the other half
+    int32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < PS_T / 64; ++w) {
+      if (w == wave) through += before + all;
+      all += s_parts[turn][w];
     }
-    before = __builtin_amdgcn_readlane(through, 63);
+    before += all;
+    const int32_t first = through - parts;
+    if (b < a.B) a.ranges[b] = SlotRange{first, parts};
+    for (int32_t p = 0; p < parts; ++p) a.shares[first + p] = Slot{static_cast<int32_t>(b), p, parts, n};
   }
-  return false;
+  for (int64_t w = before + threadIdx.x; w < slots; w += PS_T) a.shares[w] = Slot{-1, 0, 0, 0};
 }
 
 // SHORT: few tokens in all.  Every unit has workgroups of its own (eight waves on its tiles), a
@@ -482,8 +530,14 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     sh.b = blockIdx.z;
     sh.part = static_cast<int32_t>(blockIdx.x);
   } else {
-    if (!share_of(a, static_cast<int32_t>(blockIdx.x), sh)) return;  // the same for every wave
-    if (sh.part == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.ranges[sh.b] = SlotRange{sh.slot, sh.parts};
+    if (a.shares) {
+      const Slot t = a.shares[blockIdx.x];
+      if (t.b < 0) return;
+      sh = Share{t.b, static_cast<int32_t>(blockIdx.x), t.part, t.parts, t.n};
+    } else {
+      if (!share_of(a, static_cast<int32_t>(blockIdx.x), sh)) return;  // the same for every wave
+      if (sh.part == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.ranges[sh.b] = SlotRange{sh.slot, sh.parts};
+    }
   }
   const int64_t b = sh.b;
   const int unit = SHORT ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * a.waves_units + wave % a.waves_units;
@@ -1196,11 +1250,12 @@ static PagesPlan plan_pages(bool mfma, bool whole, int64_t elem, int64_t B, int6
   return p;
 }
 
-// Partials (m, l, o) of every slot and query head, and the requests' slot ranges.
+// Partials (m, l, o) of every slot and query head, the requests' slot ranges and the schedule.
 static int64_t pages_workspace(const PagesPlan& p, int64_t B, int64_t Hq, int64_t D) {
   if (!p.mfma && p.splits == 1) return 0;
   if (p.mfma && p.brief) return p.slots == 1 ? 0 : (B * p.slots * Hq * (D + 2) + B * p.units) * 8;
-  return p.slots * Hq * (D + 2) * 4 + B * static_cast<int64_t>(sizeof(SlotRange)) + 8;
+  return p.slots * Hq * (D + 2) * 4 + B * static_cast<int64_t>(sizeof(SlotRange)) + 8 +
+         (p.mfma && B > PM_LANES ? p.slots * static_cast<int64_t>(sizeof(Slot)) + 16 : 0);
 }
 
 template <int S, int QD>
@@ -1349,12 +1404,17 @@ extern "C" int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_
     } else {
       const uintptr_t end = reinterpret_cast<uintptr_t>(a.part_l + p.slots * heads);
       a.ranges = reinterpret_cast<SlotRange*>((end + 7) / 8 * 8);
+      if (batch > PM_LANES) a.shares = reinterpret_cast<Slot*>((reinterpret_cast<uintptr_t>(a.ranges + batch) + 15) / 16 * 16);
       a.waves_units = p.waves_units;
       a.subs = p.subs;
       a.target = p.target;
     }
     a.o_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && o_stride_b % 4 == 0 && o_stride_h % 4 == 0;
     a.q_vec = reinterpret_cast<uintptr_t>(query) % 16 == 0 && q_stride_b % 8 == 0 && q_stride_h % 8 == 0;
+    if (a.shares) {
+      hipLaunchKernelGGL(pages_schedule_kernel, dim3(1), dim3(PS_T), 0, stream, a, p.slots);
+      HS_CHECK_LAUNCH("page attention schedule");
+    }
     switch (pool_code) {
       case HS_DTYPE_F32: launch_mfma_pages<HS_DTYPE_F32, HS_DTYPE_F32>(p, a, stream); break;
       case HS_DTYPE_F16: launch_mfma_pages<HS_DTYPE_F16, HS_DTYPE_F16>(p, a, stream); break;

@@ -199,6 +199,34 @@ def test_uneven_batches(gpu, code):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 2, 32, 16), (5, 1, 64, 5)])
+@pytest.mark.parametrize("batch", [64, 65, 128, 1024, 1100, 2049])
+def test_many_requests(gpu, batch, heads, kv, dim, page):
+    """Batches on both sides of a wave's lanes and of the schedule's workgroup, with empty
+    requests, long ones first, last and alone; captured, with other lengths per replay."""
+    gen = torch.Generator().manual_seed(batch)
+    short = torch.randint(0, 60, (batch,), generator=gen)
+    short[::7] = 0
+    longest = 4000
+    first, last, none = short.clone(), short.clone(), torch.zeros_like(short)
+    first[0], first[1] = longest, 1
+    last[-1], last[batch // 2] = longest, 2500
+    most = torch.stack([first, last, short]).amax(0)
+    query, pool, tables, lengths = args = case(batch, heads, kv, dim, page, most.tolist(), "int8", "bf16", gpu, wide=200)
+    assert tables.shape[-1] * page > 32 * 32
+    check(attend_pages(*args), args)
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(query)
+    with torch.cuda.graph(graph):
+        attend_pages(*args, out=out)
+    for now in (first, none, last, short):
+        lengths.copy_(now)
+        out.fill_(7.0)
+        graph.replay()
+        assert out.isfinite().all() and torch.equal(out, attend_pages(*args))
+        check(out, args)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("int8", "f16"), ("e4m3", "f32"), ("f16", "f16"),
                                         ("bf16", "bf16")])
 def test_small_and_large_values(gpu, code, dtype):
