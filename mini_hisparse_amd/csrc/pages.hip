@@ -425,10 +425,21 @@ __device__ __forceinline__ int32_t tiles_of(int32_t n) {
   return static_cast<int32_t>((static_cast<uint32_t>(n) + PM_TILE - 1) / PM_TILE);
 }
 
-// Parts are of `per` tiles, the fewest for which all requests together need at most `target`
-// workgroups (sum ceil(n_b / per) <= sum n_b / per + B); an empty request has one part.
-__device__ __forceinline__ uint32_t part_room(const PagesArgs& a) {
+// Parts are of `per` tiles, and an empty request has one.  All requests together are to need at
+// most `target` workgroups: with per = sum n_b / (target - B) they surely do (sum ceil(n_b / per)
+// <= sum n_b / per + B), but with sum n_b / target they may, as equal lengths often do.  The first
+// of PM_TRIES sizes from this one up to the sure one that does is taken, where B is above a quarter
+// of the target (fewer leave three quarters of the CUs busy in any case, and the search costs 1 us).
+// In us without and with the smaller sizes: 64 requests of 16384, 40 query and 8 KV heads of 128
+// in e4m3, 531 and 403; 128 of 4096, 28 and 4 heads in int8, 154 and 115.
+constexpr int PM_TRIES = 4;
+
+__device__ __forceinline__ uint32_t sure_room(const PagesArgs& a) {
   return static_cast<uint32_t>(a.target - (a.B < a.target / 2 ? a.B : a.target / 2));
+}
+__device__ __forceinline__ uint32_t tried_size(uint32_t least, uint32_t sure, int k, uint32_t min_tiles) {
+  const uint32_t per = least + static_cast<uint32_t>(static_cast<uint64_t>(sure - least) * k / PM_TRIES);
+  return per < min_tiles ? min_tiles : per;
 }
 __device__ __forceinline__ int32_t parts_of(int32_t tiles, uint32_t per) {
   return tiles > static_cast<int64_t>(per) ? static_cast<int32_t>((static_cast<uint32_t>(tiles) + per - 1) / per) : 1;
@@ -441,11 +452,25 @@ __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& o
   const int32_t n = lane < a.B ? clamp_length(a.lengths[lane], a.pages * a.P) : 0, tiles = tiles_of(n);
   const float total =
       __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scan_lanes(static_cast<float>(tiles))), 63));
-  const uint32_t room = part_room(a);
+  const uint32_t room = sure_room(a), target = static_cast<uint32_t>(a.target), min_tiles = static_cast<uint32_t>(a.min_tiles);
   // exact below 2^24 tiles; above, more than the sum's roundings can have lost
-  uint32_t per = total < 0x1p24f ? (static_cast<uint32_t>(total) + room - 1) / room
-                                 : static_cast<uint32_t>(total / static_cast<float>(room) * 1.0001f) + 1u;
-  if (per < static_cast<uint32_t>(a.min_tiles)) per = static_cast<uint32_t>(a.min_tiles);
+  const uint32_t sum = static_cast<uint32_t>(total);
+  const uint32_t sure = total < 0x1p24f ? (sum + room - 1) / room
+                                        : static_cast<uint32_t>(total / static_cast<float>(room) * 1.0001f) + 1u;
+  uint32_t per = tried_size(sure, sure, 0, min_tiles);
+  if (total < 0x1p24f && a.B * 4 > a.target) {
+    const uint32_t least = (sum + target - 1) / target;
+    uint32_t count[PM_TRIES / 2];  // two sizes' parts in 16 bits each: at most target + B
+#pragma unroll
+    for (int k = 0; k < PM_TRIES; k += 2) {
+      const int32_t lo = parts_of(tiles, tried_size(least, sure, k, min_tiles));
+      const int32_t hi = parts_of(tiles, tried_size(least, sure, k + 1, min_tiles));
+      count[k / 2] = __builtin_amdgcn_readlane(scan_lanes(lane < a.B ? lo | hi << 16 : 0), 63);
+    }
+#pragma unroll
+    for (int k = PM_TRIES - 1; k >= 0; --k)
+      if ((count[k / 2] >> (16 * (k & 1)) & 0xffffu) <= target) per = tried_size(least, sure, k, min_tiles);
+  }
   const int32_t parts = lane < a.B ? parts_of(tiles, per) : 0, through = scan_lanes(parts);
   const uint64_t owners = __ballot(through > w);
   if (!owners) return false;
@@ -459,12 +484,13 @@ __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& o
 }
 
 // The same schedule for more requests, written out once: a workgroup's share (request -1: none)
-// and the requests' slots.  One workgroup; 1024 requests at a time.
+// and the requests' slots.  One workgroup; 1024 requests at a time.  (Walked by every wave, 64
+// lengths a step, it cost 16384 requests of 1 .. 1280 tokens 3033 us; they take 460 with this.)
 constexpr int PS_T = 1024;
 
 __global__ __launch_bounds__(PS_T) void pages_schedule_kernel(PagesArgs a, int64_t slots) {
   __shared__ int64_t s_tiles[PS_T / 64];
-  __shared__ int32_t s_parts[2][PS_T / 64];
+  __shared__ int32_t s_parts[2][PS_T / 64], s_count[PM_TRIES][PS_T / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t limit = a.pages * a.P;
   int64_t total = 0;
@@ -476,8 +502,31 @@ __global__ __launch_bounds__(PS_T) void pages_schedule_kernel(PagesArgs a, int64
   total = 0;
 #pragma unroll
   for (int w = 0; w < PS_T / 64; ++w) total += s_tiles[w];
-  const int64_t room = part_room(a), fewest = (total + room - 1) / room;
-  const uint32_t per = static_cast<uint32_t>(fewest < a.min_tiles ? a.min_tiles : fewest);
+  const int64_t room = sure_room(a);
+  const uint32_t least = static_cast<uint32_t>((total + a.target - 1) / a.target);
+  const uint32_t sure = static_cast<uint32_t>((total + room - 1) / room), min_tiles = static_cast<uint32_t>(a.min_tiles);
+  uint32_t per = tried_size(sure, sure, 0, min_tiles);
+  if (a.B <= a.target) {  // else every size gives more parts
+    int32_t count[PM_TRIES] = {};
+    for (int64_t b = threadIdx.x; b < a.B; b += PS_T) {
+      const int32_t tiles = tiles_of(clamp_length(a.lengths[b], limit));
+#pragma unroll
+      for (int k = 0; k < PM_TRIES; ++k) count[k] += parts_of(tiles, tried_size(least, sure, k, min_tiles));
+    }
+#pragma unroll
+    for (int k = 0; k < PM_TRIES; ++k) {
+      const int32_t all = scan_lanes(count[k]);
+      if (lane == 63) s_count[k][wave] = all;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = PM_TRIES - 1; k >= 0; --k) {
+      int32_t all = 0;
+#pragma unroll
+      for (int w = 0; w < PS_T / 64; ++w) all += s_count[k][w];
+      if (all <= a.target) per = tried_size(least, sure, k, min_tiles);
+    }
+  }
   int32_t before = 0;
   for (int64_t b0 = 0, turn = 0; b0 < a.B; b0 += PS_T, turn ^= 1) {
     const int64_t b = b0 + threadIdx.x;
@@ -1228,7 +1277,10 @@ static PagesPlan plan_pages(bool mfma, bool whole, int64_t elem, int64_t B, int6
     while (p.units % p.waves_units) --p.waves_units;
     p.subs = 8 / p.waves_units;
     const int64_t groups = p.units / p.waves_units;
-    p.target = (256 + groups - 1) / groups;
+    // Two of them for batches above a wave's lanes, whose ragged lengths then balance (28 and 4 heads
+    // of 128 in int8, 256 requests of 1 .. 4096 tokens 162 us with one a CU, 137 with two, 136 with
+    // three; 96 with 40 and 8 heads 120, 98, 98; 96 full ones of 4096 with 28 and 4 heads 90, 95, 101).
+    p.target = ((B > PM_LANES ? 512 : 256) + groups - 1) / groups;
     p.min_tiles = p.subs;
     const int64_t most = B * ((tiles + p.min_tiles - 1) / p.min_tiles);
     p.slots = most < p.target + B ? most : p.target + B;
