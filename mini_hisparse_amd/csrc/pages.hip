@@ -310,7 +310,7 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
 }
 
 // ---- the matrix-core kernel ---------------------------------------------------------------
-// Head dims of 32, 64, 96 and 128.  A wave owns one unit (a KV head and up to 16 of its query
+// Head dims of 32, 64, 96, 128 and 256.  A wave owns one unit (a KV head and up to 16 of its query
 // heads) and walks tiles of 32 tokens, with no shared memory:
 //
 //   S^T = K Q^T   A: K rows (lane (j, c): row c, 8 of the head dim), B: the heads' queries;
@@ -330,6 +330,8 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
 // hold weights up to 2^SLACK, no less precise): no cross-lane step in most tiles.
 
 constexpr int PM_TILE = 32;
+// Waves of a workgroup: half as many for 256 of the head dim, with twice the registers each.
+constexpr int mfma_waves(int64_t D) { return D > 128 ? 4 : 8; }
 constexpr int PM_PARTS = 8;  // parts of a short request
 constexpr int PM_LANES = 64;  // requests whose schedule a wave derives by itself
 constexpr float PM_SLACK = 6.f;
@@ -549,13 +551,14 @@ __global__ __launch_bounds__(PS_T) void pages_schedule_kernel(PagesArgs a, int64
   for (int64_t w = before + threadIdx.x; w < slots; w += PS_T) a.shares[w] = Slot{-1, 0, 0, 0};
 }
 
-// SHORT: few tokens in all.  Every unit has workgroups of its own (eight waves on its tiles), a
+// SHORT: few tokens in all.  Every unit has workgroups of its own (all waves on its tiles), a
 // request `max_parts` at most, in a fixed grid, so that the table, the length and the query
 // load together; a part alone writes the output, several are joined by the last to arrive.
 // Else the schedule of share_of over workgroups of up to four units (a page's rows are
 // contiguous over the KV heads), joined by pages_merge_kernel.
 template <int S, int QD, int D, bool UNIFORM, bool SHORT>
-__global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
+__global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArgs a) {
+  constexpr int W = mfma_waves(D), T = 64 * W;
   constexpr bool F16 = S == HS_DTYPE_F16, F32 = S == HS_DTYPE_F32;
   constexpr int ES = elem_size<S>();
   constexpr int KK = F32 ? D / 4 : D / 32;   // products over the head dim
@@ -571,7 +574,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
   constexpr int VW0 = VB < 4 ? 1 : VB / 4, VW = VW0 + (VB1 + 3) / 4;
   constexpr int SD = D + 4;                  // row stride of the waves' sums in LDS: no bank conflicts
   extern __shared__ __attribute__((aligned(16))) float smem[];
-  __shared__ float s_m[8][16], s_l[8][16];
+  __shared__ float s_m[W][16], s_l[W][16];
   const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   Share sh;
@@ -591,7 +594,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
   const int64_t b = sh.b;
   const int unit = SHORT ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * a.waves_units + wave % a.waves_units;
   const int sub = SHORT ? wave : wave / a.waves_units;
-  const int subs = SHORT ? 8 : a.subs;
+  const int subs = SHORT ? W : a.subs;
   const int kv = unit / a.head_chunks, h0 = unit % a.head_chunks * 16;
   const int heads = static_cast<int>(a.g - h0 < 16 ? a.g - h0 : 16);
   const int32_t* table = a.tables + b * a.t_sb + kv * a.t_sk;
@@ -1014,7 +1017,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     }
   }
   __syncthreads();
-  const int stride = SHORT ? 1 : a.waves_units, waves = SHORT ? 8 : a.waves_units * a.subs;
+  const int stride = SHORT ? 1 : a.waves_units, waves = SHORT ? W : a.waves_units * a.subs;
   const uint32_t tag = SHORT ? group_tag(a.epoch, counter_round(seen, a.epoch)) : 0u;
   constexpr int QUADS = D / 4;
   for (int i = threadIdx.x; i < stride * rows * QUADS; i += blockDim.x) {
@@ -1026,11 +1029,11 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     float M = -INFINITY, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 8; ++w)
+    for (int w = 0; w < W; ++w)
       if (u + w * stride < waves) M = fmaxf(M, s_m[u + w * stride][h]);
     if (M != -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
+      for (int w = 0; w < W; ++w) {
         const int at = u + w * stride;
         if (at >= waves) continue;
         const float f = exp2_(s_m[at][h] - M);  // 0 where a wave had no token
@@ -1075,15 +1078,15 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     const int64_t next = a.Hq * D;                                // from a part's o word to the next part's
     // Every word goes out before any is used, with no branch between them (a part past the last
     // reads part 0's again): o words of the thread's (head, dim) pairs, then its m and its l.
-    constexpr int PAIRS = (16 * D + 511) / 512;
+    constexpr int PAIRS = (16 * D + T - 1) / T;
     unsigned long long w[PAIRS][PM_PARTS];
     auto pair_word = [&](int r) {
-      const int i = threadIdx.x + 512 * r < heads * D ? threadIdx.x + 512 * r : 0;
+      const int i = threadIdx.x + T * r < heads * D ? threadIdx.x + T * r : 0;
       return a.word_o + (base + i / D) * D + i % D;
     };
 #pragma unroll
     for (int r = 0; r < PAIRS; ++r) {
-      if (512 * r >= heads * D) continue;
+      if (T * r >= heads * D) continue;
 #pragma unroll
       for (int u = 0; u < PM_PARTS; ++u)
         w[r][u] = __hip_atomic_load(pair_word(r) + (u < sh.parts ? u : 0) * next, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1116,7 +1119,7 @@ __global__ __launch_bounds__(512) void pages_mfma_kernel(PagesArgs a) {
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < PAIRS; ++r) {
-      const int i = threadIdx.x + 512 * r;
+      const int i = threadIdx.x + T * r;
       if (i >= heads * D) continue;
       const int h = i / D, d = i % D;
       unsigned long long* const at = pair_word(r);
@@ -1239,7 +1242,7 @@ struct PagesPlan {
 // tokens, 32 query and 8 KV heads: of 96 on the vector unit 64.8 us in int8 and 78.5 in bf16, here
 // 30.6 and 38.7; of 80, which the vector unit keeps, 55.8 and 65.2.)
 static bool pages_mfma_shape(int64_t elem, int64_t Hkv, int64_t D) {
-  return (D == 32 || D == 64 || D == 96 || D == 128) && Hkv * D * elem < (int64_t{1} << 27);
+  return (D == 32 || D == 64 || D == 96 || D == 128 || (D == 256 && elem < 4)) && Hkv * D * elem < (int64_t{1} << 27);
 }
 
 // Splits of the token axis: about 2048 workgroups, each with at least one tile per wave.
@@ -1254,7 +1257,7 @@ static PagesPlan plan_pages(bool mfma, bool whole, int64_t elem, int64_t B, int6
     p.units = static_cast<int>(Hkv * p.head_chunks);
     const int64_t tiles = (tokens + PM_TILE - 1) / PM_TILE;
     // Short: as many parts of a request as give every CU a workgroup, 8 at most (their join is one
-    // workgroup's work), of a tile for each of the eight waves at least.  Taken while a part is at
+    // workgroup's work), of a tile for each of the workgroup's waves at least.  Taken while a part is at
     // most 32 tiles: us by this launch and by the long one, 28 query and 4 KV heads of 128 in
     // int8, for 1 request of 256, 1024, 4096 and 16384 tokens 7.2 11.2 14.0 23.7 and 13.5 13.9
     // 14.6 18.8, for 16 requests of 1024, 4096 and 16384 13.3 21.0 62.7 and 16.7 23.5 61.3.
@@ -1263,19 +1266,19 @@ static PagesPlan plan_pages(bool mfma, bool whole, int64_t elem, int64_t B, int6
     int64_t parts = 256 / (B * p.units);
     parts = parts < 1 || tiles * 2 * PM_TILE * D * elem <= 128 * 1024 ? 1 : (parts > PM_PARTS ? PM_PARTS : parts);
     p.min_tiles = (tiles + parts - 1) / parts;
-    if (p.min_tiles < 8) p.min_tiles = 8;
+    if (p.min_tiles < mfma_waves(D)) p.min_tiles = mfma_waves(D);
     p.brief = p.min_tiles <= 32 && p.units <= 65535;
     if (p.brief) {
       p.slots = (tiles + p.min_tiles - 1) / p.min_tiles;
       return p;
     }
-    // Long: one workgroup a CU, of eight waves over up to four units.  us at 4 histories of 32768
+    // Long: one workgroup a CU, over up to four units.  us at 4 histories of 32768
     // tokens, 14 query and 2 KV heads of 64 in bf16, for 256, 512 and 768 workgroups 20.4 21.4
     // 24.2; 28 and 4 heads of 128 in int8 32.5 38.9 45.4; 16 of 16384, 40 and 8 heads of 128 in
     // e4m3, with four units a workgroup 109, with eight 110, with one 192.
     p.waves_units = 4;
     while (p.units % p.waves_units) --p.waves_units;
-    p.subs = 8 / p.waves_units;
+    p.subs = mfma_waves(D) / p.waves_units;
     const int64_t groups = p.units / p.waves_units;
     // Two of them for batches above a wave's lanes, whose ragged lengths then balance (28 and 4 heads
     // of 128 in int8, 256 requests of 1 .. 4096 tokens 162 us with one a CU, 137 with two, 136 with
@@ -1312,7 +1315,7 @@ static int64_t pages_workspace(const PagesPlan& p, int64_t B, int64_t Hq, int64_
 
 template <int S, int QD>
 static void launch_mfma_pages(const PagesPlan& p, const PagesArgs& a, hipStream_t s) {
-  const int64_t waves = p.brief ? 8 : p.waves_units * p.subs, heads = a.g < 16 ? a.g : 16;
+  const int64_t waves = p.brief ? mfma_waves(a.D) : p.waves_units * p.subs, heads = a.g < 16 ? a.g : 16;
   const dim3 grid = p.brief ? dim3(static_cast<unsigned>(p.slots), static_cast<unsigned>(p.units), static_cast<unsigned>(a.B))
                             : dim3(static_cast<unsigned>(p.slots), static_cast<unsigned>(p.units / p.waves_units));
   const dim3 block(static_cast<unsigned>(64 * waves));
@@ -1332,7 +1335,8 @@ static void launch_mfma_pages(const PagesPlan& p, const PagesArgs& a, hipStream_
   if (a.D == 32) HS_PAGES_D(32);
   else if (a.D == 64) HS_PAGES_D(64);
   else if (a.D == 96) HS_PAGES_D(96);
-  else HS_PAGES_D(128);
+  else if (S == HS_DTYPE_F32 || a.D == 128) HS_PAGES_D(128);
+  else if constexpr (S != HS_DTYPE_F32) HS_PAGES_D(256);
 #undef HS_PAGES_D
 #undef HS_PAGES_RUN
 }

@@ -259,13 +259,16 @@ def test_nan_in_a_used_row_reaches_its_heads_alone(gpu, code, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("code,dtype", POOLS)
-@pytest.mark.parametrize("dim", [80, 96])
+@pytest.mark.parametrize("dim", [80, 96, 256])
 def test_pages_masks_and_nan_at_other_head_dims(gpu, dim, code, dtype):
-    """80 of the head dim run on the vector unit, 96 in two column parts of a V row."""
+    """80 of the head dim run on the vector unit, 96 in two column parts of a V row, 256 in
+    workgroups of half the waves (float32 on the vector unit)."""
     for page in (1, 12, 16, 48):
         for wide in (2, WIDE):
             args = case(3, 6, 3, dim, page, [401, 0, 63], code, dtype, gpu, absent=0.3, per_head=page > 1, wide=wide)
             check(attend_pages(*args), args)
+    args = case(2, 40, 2, dim, 16, [2100, 700], code, dtype, gpu)  # several parts of a request, 16 heads and 4 of a unit
+    check(attend_pages(*args), args)
     query, pool, tables, lengths = case(2, 4, 2, dim, 16, [40, 40], code, dtype, gpu)
     block = tables[0, 1].item()
     (pool.scales if code in CODES else pool)[block, 1, 3, 1] = float("nan")  # a value of request 0, KV head 1
