@@ -425,8 +425,10 @@ int hs_attend_window(const void* query, int64_t q_stride_h, const void* pool, in
  *   out      [batch, heads, head_dim] in query_dtype; 0 for a request without a token
  * Scores, softmax statistics and sums are fp32.  The workspace
  * (hs_attend_pages_workspace_bytes of the same sizes; 0: none, null then; 16-byte aligned)
- * may hold anything before a call; calls that share one must run in order.  Nothing is read on the host, so
- * a captured call replays with the tables and lengths of the moment.
+ * may hold anything before a call; calls that share one must run in order.  Nothing is read on
+ * the host, so a captured call replays with the tables and lengths of the moment.  head_dim at
+ * most 512 (32, 64, 96, 128 and, but for float32 pools, 256 run on the matrix cores), batch and
+ * heads at most 65535, pages * page_size below 2^31.
  */
 int64_t hs_attend_pages_workspace_bytes(int32_t query_dtype, int32_t pool_code, int64_t batch, int64_t heads,
                                         int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t pages);
@@ -453,7 +455,8 @@ int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_stride_h, i
  *   k, v   hs_append_quantized: [tokens, Hkv, D] in `dtype`, element strides per token and
  *          head; hs_read_quantized: [n, Hkv, D] contiguous out, code * scale rounded to
  *          `dtype`
- * pool_rows = blocks * P; head_dim at most 512; tokens or n may be 0.
+ * pool_rows = blocks * P; head_dim at most 512; tokens or n may be 0, and times kv_heads at
+ * most 2^25.
  */
 int hs_append_quantized(const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, int32_t dtype, const int64_t* rows, int64_t tokens, void* codes,

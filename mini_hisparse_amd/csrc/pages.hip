@@ -12,7 +12,10 @@
 // multiplies its score, a V row's its weight, so codes are never widened in memory.
 //
 // The cache is read once and everything else is small, so the kernels are bound by its
-// bytes.  The token axis is split over workgroups; every split leaves its running
+// bytes: 8 requests of 131072 tokens, 28 query and 4 KV heads of 128 in int8, 1.08 GB, take
+// 183 .. 193 us and the join 5, 5.6 .. 5.9 TB/s where a plain read of 1 GiB runs at 6.07.  Small
+// calls are bound by a chain of loads (length and table, page, K, V) and joins: 8.6 us for one
+// request of 2000 tokens with 14 and 2 heads of 64, 0.5 MB.  The token axis is split over workgroups; every split leaves its running
 // (m, l, sum e^(s - m) V) in fp32 and `pages_merge_kernel` joins them.  Scores carry the
 // factor log2(e), so every exponential is a power of two.
 #include <math.h>
@@ -1240,7 +1243,8 @@ struct PagesPlan {
 
 // The MFMA kernel's shapes: its lane offsets within 16 rows are 32-bit.  (16 requests of 4096
 // tokens, 32 query and 8 KV heads: of 96 on the vector unit 64.8 us in int8 and 78.5 in bf16, here
-// 30.6 and 38.7; of 80, which the vector unit keeps, 55.8 and 65.2.)
+// 30.6 and 38.7; of 256 162 and 197, here 49 and 99; of 80, which the vector unit keeps, 55.8 and
+// 65.2.  float32 rows of 256 would spill registers.)
 static bool pages_mfma_shape(int64_t elem, int64_t Hkv, int64_t D) {
   return (D == 32 || D == 64 || D == 96 || D == 128 || (D == 256 && elem < 4)) && Hkv * D * elem < (int64_t{1} << 27);
 }
@@ -1256,29 +1260,31 @@ static PagesPlan plan_pages(bool mfma, bool whole, int64_t elem, int64_t B, int6
     p.head_chunks = static_cast<int>((g + 15) / 16);
     p.units = static_cast<int>(Hkv * p.head_chunks);
     const int64_t tiles = (tokens + PM_TILE - 1) / PM_TILE;
-    // Short: as many parts of a request as give every CU a workgroup, 8 at most (their join is one
-    // workgroup's work), of a tile for each of the workgroup's waves at least.  Taken while a part is at
-    // most 32 tiles: us by this launch and by the long one, 28 query and 4 KV heads of 128 in
-    // int8, for 1 request of 256, 1024, 4096 and 16384 tokens 7.2 11.2 14.0 23.7 and 13.5 13.9
-    // 14.6 18.8, for 16 requests of 1024, 4096 and 16384 13.3 21.0 62.7 and 16.7 23.5 61.3.
+    // Short: as many parts of a request as give every CU a workgroup, 8 at most, of a tile for each
+    // of its waves at least.  Taken while a wave has four tiles at most: us by this launch and by
+    // the long one, 28 query and 4 KV heads of 128 in int8, for 1 request of 256, 1024 and 4096
+    // tokens 7.2 11.2 14.0 and 13.5 13.9 14.6, for 16 of 1024, 4096 and 16384 13.3 21.0 62.7 and
+    // 16.7 23.5 61.3.  The parts' join is one workgroup's work and loses above 16 of their words a
+    // thread (16 heads of 128, 1 request of 512, 1024 and 2048 tokens, 8, 16 and 32 words: 8.7 13.3
+    // 14.7 here, 12.8 12.9 13.0 in the long one; 4 heads of 256, 4 requests of 512 and 1024 tokens,
+    // 16 and 32 words: 12.9 16.2 and 12.6 12.6).
     // A unit of at most 128 KiB stays one part (14 query and 2 KV heads of 64 in int8, 64 requests
     // of 1024 tokens: 10.4 in one part, 12.7 in two).
+    const int64_t W = mfma_waves(D), rows = g < 16 ? g : 16;
     int64_t parts = 256 / (B * p.units);
     parts = parts < 1 || tiles * 2 * PM_TILE * D * elem <= 128 * 1024 ? 1 : (parts > PM_PARTS ? PM_PARTS : parts);
     p.min_tiles = (tiles + parts - 1) / parts;
-    if (p.min_tiles < mfma_waves(D)) p.min_tiles = mfma_waves(D);
-    p.brief = p.min_tiles <= 32 && p.units <= 65535;
-    if (p.brief) {
-      p.slots = (tiles + p.min_tiles - 1) / p.min_tiles;
-      return p;
-    }
+    if (p.min_tiles < W) p.min_tiles = W;
+    p.slots = (tiles + p.min_tiles - 1) / p.min_tiles;
+    p.brief = p.min_tiles <= 4 * W && p.units <= 65535 && (p.slots == 1 || p.slots * rows * D < 16 * 64 * W);
+    if (p.brief) return p;
     // Long: one workgroup a CU, over up to four units.  us at 4 histories of 32768
     // tokens, 14 query and 2 KV heads of 64 in bf16, for 256, 512 and 768 workgroups 20.4 21.4
     // 24.2; 28 and 4 heads of 128 in int8 32.5 38.9 45.4; 16 of 16384, 40 and 8 heads of 128 in
     // e4m3, with four units a workgroup 109, with eight 110, with one 192.
     p.waves_units = 4;
     while (p.units % p.waves_units) --p.waves_units;
-    p.subs = mfma_waves(D) / p.waves_units;
+    p.subs = static_cast<int>(W) / p.waves_units;
     const int64_t groups = p.units / p.waves_units;
     // Two of them for batches above a wave's lanes, whose ragged lengths then balance (28 and 4 heads
     // of 128 in int8, 256 requests of 1 .. 4096 tokens 162 us with one a CU, 137 with two, 136 with
