@@ -1147,7 +1147,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
 // LDS, one slot a thread; then the sums: C elements a lane, 256 / (D / C) slots abreast and PJ_U of each in flight, so
 // that a long history's slots are a few rounds of loads (one slot after another took 66 of
 // 87 us at 128 slots of D = 64), joined over LDS in a fixed order.  Bound by its launch and two
-// rounds of loads: 3.9 us for 4 requests of 14 heads of 64 in 64 slots each, 5.6 for 8 of 28 heads
+// rounds of loads: 3.9 us for 4 requests of 14 heads of 64 in 61 slots each, 5.6 for 8 of 28 heads
 // of 128 in 31.
 constexpr int PJ_T = 256;
 constexpr int PJ_U = 4;

@@ -5,8 +5,9 @@ A :class:`QuantizedPool` has the layout of a plain pool, ``codes`` [blocks, 2, P
 vector; a row takes ``2 Hkv (D + 4)`` bytes.  :func:`append_quantized` quantises rows as
 they are written (a prompt's or one token of each request), :func:`read_quantized` widens
 rows again, and ``row_kernels.attend_pages`` attends over the codes themselves.  Rows are
-named by physical row (block * P + offset), as everywhere in this package.  No counterpart
-in the reference, whose cache holds the model dtype.
+named by physical row (block * P + offset), as everywhere in this package; a call takes up
+to 2^25 head vectors of K (rows times KV heads).  No counterpart in the reference, whose
+cache holds the model dtype.
 """
 
 from __future__ import annotations

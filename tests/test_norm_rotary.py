@@ -189,3 +189,12 @@ def test_entry_point_refusals_without_a_gpu():
                 dict(dtype=3), dict(qkv=None)):
         assert call(**bad) == -1, bad
         assert lib.hs_last_error()
+
+
+def test_more_rows_than_a_grid_holds_are_refused_without_a_gpu():
+    lib = _lib.load()
+    buffer = ctypes.create_string_buffer(256)
+    at = ctypes.addressof(buffer)
+    for rows in (2**24, 2**31 - 1, 2**31):
+        assert lib.hs_norm_rotary_split(at, 1536, at, at, 1e-6, at, at, at, at, rows, 1, 1, 512, 1e4, 2, None) == -1
+        assert b"too many rows" in lib.hs_last_error()
