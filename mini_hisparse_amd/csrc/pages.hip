@@ -138,7 +138,10 @@ __device__ __forceinline__ void load_pool(const void* pool, int64_t i, float (&x
 // takes tiles of 64 tokens: a lane scores one token for the G heads (its K row against the
 // queries in LDS, read as broadcasts), then the lanes turn to the head dim and add the
 // tile's V rows, C elements a lane and 64 / (D / C) rows at once, weighted by the heads'
-// probabilities from LDS.  Both products run on the vector unit in fp32 throughout.
+// probabilities from LDS.  Both products run on the vector unit in fp32 throughout,
+// and bound the kernel: 16 requests of 4096 tokens, 32 query and 8 KV heads of 80 in int8, 88 MB,
+// take 51.5 us, 1.7 TB/s; of 512 in bf16, 1.07 GB, 354, 3.0.  Odd head dims load single elements
+// (81: 141 us).
 constexpr int PG_W = 4;
 constexpr int PG_T = 64 * PG_W;
 
@@ -1246,13 +1249,12 @@ struct PagesPlan {
 
 // The MFMA kernel's shapes: its lane offsets within 16 rows are 32-bit.  (16 requests of 4096
 // tokens, 32 query and 8 KV heads: of 96 on the vector unit 64.8 us in int8 and 78.5 in bf16, here
-// 30.6 and 38.7; of 256 162 and 197, here 49 and 99; of 80, which the vector unit keeps, 55.8 and
-// 65.2.  float32 rows of 256 would spill registers.)
+// 30.6 and 38.7; of 256 162 and 197, here 49 and 99; of 80, which the vector unit keeps, 51.5 in
+// int8.  float32 rows of 256 would spill registers.)
 static bool pages_mfma_shape(int64_t elem, int64_t Hkv, int64_t D) {
   return (D == 32 || D == 64 || D == 96 || D == 128 || (D == 256 && elem < 4)) && Hkv * D * elem < (int64_t{1} << 27);
 }
 
-// Splits of the token axis: about 2048 workgroups, each with at least one tile per wave.
 // `whole`: the general kernel takes a request in one split (the workspace was sized for a kernel
 // that needs none).
 static PagesPlan plan_pages(bool mfma, bool whole, int64_t elem, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t tokens) {
@@ -1298,14 +1300,19 @@ static PagesPlan plan_pages(bool mfma, bool whole, int64_t elem, int64_t B, int6
     p.slots = most < p.target + B ? most : p.target + B;
     return p;
   }
-  p.G = g <= 4 || D > 256 ? 4 : 8;
-  p.head_chunks = static_cast<int>((g + p.G - 1) / p.G);
-  const int64_t groups = B * Hkv * p.head_chunks;
-  int64_t splits = (2048 + groups - 1) / groups;
+  // Query heads of a workgroup: two where there are no more, or where four would leave CUs idle.
+  // us with four and two, head dim 80 in int8: 16 requests of 4096 tokens, 8 KV heads of one, two
+  // and four query heads each 54 54 57 and 47 47 75; 1 of 1024, four each, 22 and 17; 4 of 4096, 16
+  // and 2 heads of 112, 26 and 22.  (Eight took 64 for 16 of 4096, 32 and 4 heads, four 56.)
   const int64_t cap = (tokens + PG_T - 1) / PG_T;
+  p.G = g <= 2 || B * Hkv * ((g + 3) / 4) * cap <= 256 ? 2 : 4;
+  p.head_chunks = static_cast<int>((g + p.G - 1) / p.G);
+  // Splits: about 1024 workgroups (16 requests of 16384 tokens, 32 and 8 heads of 80: 246 us with 768,
+  // 194 with 1024, 272 with 1536, 197 with 2048), a split no shorter than a tile a wave.
+  const int64_t groups = B * Hkv * p.head_chunks;
+  int64_t splits = (1024 + groups - 1) / groups;
   if (splits > cap) splits = cap;
-  if (whole || tokens <= 2 * PG_T) splits = 1;  // written without a join: one launch
-  if (splits < 1) splits = 1;
+  if (whole || splits < 1) splits = 1;
   p.chunk = ((tokens + splits - 1) / splits + PG_T - 1) / PG_T * PG_T;
   if (p.chunk < PG_T) p.chunk = PG_T;
   p.splits = (tokens + p.chunk - 1) / p.chunk;
@@ -1362,14 +1369,18 @@ static void launch_general(const PagesPlan& p, const PagesArgs& a, bool vec, hip
   const dim3 grid(static_cast<unsigned>(a.splits), static_cast<unsigned>(a.Hkv * p.head_chunks),
                   static_cast<unsigned>(a.B));
   const unsigned smem = static_cast<unsigned>(general_smem(p.G, a.D));
+#define HS_PAGES_RUN(C, NC, G) \
+  hipLaunchKernelGGL((pages_general_kernel<S, C, NC, G>), grid, dim3(PG_T), smem, s, a)
   if (p.G == 4) {
-    if (vec && a.D <= 256) hipLaunchKernelGGL((pages_general_kernel<S, 4, 1, 4>), grid, dim3(PG_T), smem, s, a);
-    else if (vec) hipLaunchKernelGGL((pages_general_kernel<S, 4, 2, 4>), grid, dim3(PG_T), smem, s, a);
-    else hipLaunchKernelGGL((pages_general_kernel<S, 1, 8, 4>), grid, dim3(PG_T), smem, s, a);
+    if (vec && a.D <= 256) HS_PAGES_RUN(4, 1, 4);
+    else if (vec) HS_PAGES_RUN(4, 2, 4);
+    else HS_PAGES_RUN(1, 8, 4);
   } else {
-    if (vec) hipLaunchKernelGGL((pages_general_kernel<S, 4, 1, 8>), grid, dim3(PG_T), smem, s, a);
-    else hipLaunchKernelGGL((pages_general_kernel<S, 1, 4, 8>), grid, dim3(PG_T), smem, s, a);
+    if (vec && a.D <= 256) HS_PAGES_RUN(4, 1, 2);
+    else if (vec) HS_PAGES_RUN(4, 2, 2);
+    else HS_PAGES_RUN(1, 8, 2);
   }
+#undef HS_PAGES_RUN
 }
 
 static int check_pages(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
