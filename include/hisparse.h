@@ -423,7 +423,10 @@ int hs_attend_window(const void* query, int64_t q_stride_h, const void* pool, in
  *   lengths  int32 [batch] on the device: tokens of each request (clamped to 0 ..
  *            pages * P); rows past them are never used
  *   out      [batch, heads, head_dim] in query_dtype; 0 for a request without a token
- * Scores, softmax statistics and sums are fp32.  The workspace
+ * Scores, softmax statistics and sums are fp32.  On the matrix cores a weight enters the
+ * second product as a sum of 16-bit parts, to 2^-16 of itself (8-bit pools with a float32
+ * query 2^-24; float16 pools 2^-22, and 2^-45 of the largest weight; float32 pools and other
+ * head dims fp32).  The workspace
  * (hs_attend_pages_workspace_bytes of the same sizes; 0: none, null then; 16-byte aligned)
  * may hold anything before a call; calls that share one must run in order.  Nothing is read on
  * the host, so a captured call replays with the tables and lengths of the moment.  head_dim at

@@ -329,9 +329,16 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
 //
 // with (j, c) = (lane / 16, lane % 16).  Codes widen to bf16 in registers (exact); queries and
 // weights go in as sums of bf16 parts: as many of the query as its type has significand (1
-// for bf16, 2 for float16, 3 for float32) and of the weights two (2^-16 of a weight; three
-// for float32 queries).  float16 pools use float16 products, float32 pools float32 ones (four
-// of the head dim, or four tokens, at a time; the same lanes hold the same values).  A tile's
+// for bf16, 2 for float16, 3 for float32) and of the weights two (which hold a weight to 2^-16 of
+// itself, a 256th of a bf16 output's half step and a 32nd of a float16's; three for float32
+// queries).  float16 pools use float16 products, float32 pools float32 ones (four
+// of the head dim, or four tokens, at a time; the same lanes hold the same values).  float16's
+// range is short for weights, so they are held at 2^LIFT times their size, what the first part
+// leaves at 2^LOW times that, and the products of the two are added in fp32: at most 2^-22 of a
+// weight and 2^-(25 + LIFT + LOW) = 2^-45 of the largest one are lost.  (Two parts at one scale
+// lose any weight below 2^-25 of the largest, which a long history behind one leading key adds
+// up.  16 requests of 4096 tokens, 32 query and 8 KV heads, us at head dim 64, 128 and 256: 31.5
+// 48.1 98 with these scales, as without.)  A tile's
 // scales are one dword a lane, spread over the group by the broadcast of the multiply itself.
 // The running maximum moves only when a score passes it by more than SLACK (the sums then
 // hold weights up to 2^SLACK, no less precise): no cross-lane step in most tiles.
@@ -342,6 +349,13 @@ constexpr int mfma_waves(int64_t D) { return D > 128 ? 4 : 8; }
 constexpr int PM_PARTS = 8;  // parts of a short request
 constexpr int PM_LANES = 64;  // requests whose schedule a wave derives by itself
 constexpr float PM_SLACK = 6.f;
+constexpr float PM_LIFT = 9.f;  // weights reach 2^(SLACK + LIFT) = 2^15, float16 65504
+constexpr int PM_LOW = 11;      // what a float16 leaves of 2^15 is at most 2^4
+
+// The power of two by which weights are held above the running maximum m's scale.  From 2^20 on
+// float32 holds scores to 2^-3 at best and their distance to m - LIFT no longer exactly: none then.
+template <bool F16>
+__device__ __forceinline__ float lift_at(float m) { return F16 && fabsf(m) < 0x1p20f ? PM_LIFT : 0.f; }
 
 template <int S>
 constexpr int elem_size() { return S == HS_DTYPE_F32 ? 4 : (quantised(S) ? 1 : 2); }
@@ -802,13 +816,14 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float m_new = fmaxf(m_run, top);
-      const float alpha = m_new == -INFINITY ? 1.f : exp2_(m_run - m_new);
+      const float alpha =
+          m_new == -INFINITY ? 1.f : exp2_((m_run - lift_at<F16>(m_run)) - (m_new - lift_at<F16>(m_new)));
       m_run = m_new;
       l_run *= alpha;
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] *= alpha;
     }
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    const float m_use = m_run == -INFINITY ? 0.f : m_run - lift_at<F16>(m_run);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] = exp2_(s[e] - m_use);
     l_run += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
@@ -837,8 +852,9 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
         for (int i = 0; i < 4; ++i) {
           pf[q][i] = pack16<F16>(s[2 * i], s[2 * i + 1]);
           if (q + 1 < NP) {
-            s[2 * i] -= low16<F16>(pf[q][i]);
-            s[2 * i + 1] -= high16<F16>(pf[q][i]);
+            constexpr float UP = F16 ? 1 << PM_LOW : 1;
+            s[2 * i] = (s[2 * i] - low16<F16>(pf[q][i])) * UP;
+            s[2 * i + 1] = (s[2 * i + 1] - high16<F16>(pf[q][i])) * UP;
           }
         }
       }
@@ -861,8 +877,15 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
         }
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
-          acc[e] = mfma_16x16x32<F16>(even, pf[q], acc[e]);
-          acc[e + 1] = mfma_16x16x32<F16>(odd, pf[q], acc[e + 1]);
+          if (F16 && q) {
+            constexpr float DOWN = 1.f / (1 << PM_LOW);
+            const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+            acc[e] += mfma_16x16x32<F16>(even, pf[q], none) * DOWN;
+            acc[e + 1] += mfma_16x16x32<F16>(odd, pf[q], none) * DOWN;
+          } else {
+            acc[e] = mfma_16x16x32<F16>(even, pf[q], acc[e]);
+            acc[e + 1] = mfma_16x16x32<F16>(odd, pf[q], acc[e + 1]);
+          }
         }
       }
     }
@@ -992,6 +1015,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
   }
 
   auto dim_of = [](int v_lane, int e) { return e < E0 ? E0 * v_lane + e : 16 * E0 + (E - E0) * v_lane + e - E0; };
+  m_run -= lift_at<F16>(m_run);  // the scale that the sums are at
   // the totals of a head over the four groups, then the waves of a unit, then the partial
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);

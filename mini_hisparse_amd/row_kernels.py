@@ -283,6 +283,11 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
     tables past them is not read).  Tables and lengths are read on the device, so a captured
     call replays with their contents of the moment.  Returns [B, Hq, D] in the query dtype
     (``out`` when given); zeros for a request without a token.
+
+    Scores, softmax statistics and sums are float32.  Where the matrix cores run (head dims
+    32, 64, 96, 128 and, but for float32 pools, 256) a weight enters the product with V to
+    2^-16 of itself (float16 pools 2^-22 and 2^-45 of the largest weight, 8-bit pools with a
+    float32 query 2^-24, float32 pools in full).
     """
     quantized = isinstance(pool, QuantizedPool)
     store = pool.codes if quantized else pool

@@ -402,6 +402,74 @@ def test_streams_and_captured_replays(gpu, code, dtype):
         assert torch.equal(outs[0], want_a) and torch.equal(outs[1], want_b)
 
 
+def behind_one_key(heads, kv, dim, page, lengths, nats, amplitude, device, wide):
+    """float16 requests whose first key stands ``nats`` above every other and has the value 0; the
+    others, with keys near 0, have values of one sign, so that nothing but their small weights is left."""
+    query, pool, tables, lengths = case(len(lengths), heads, kv, dim, page, lengths, "f16", "f16", device, wide=wide)
+    group = heads // kv
+    query = query[:, ::group].repeat_interleave(group, 1).contiguous()  # one direction for the heads of a group
+    pool[:, 0] *= 0.01
+    pool[:, 1] = pool[:, 1].abs().clamp(max=1.0) * amplitude
+    for b in range(len(query)):
+        block = tables[b, 0].item()
+        q = query[b, ::group].double()
+        pool[block, 0, 0] = (q * (nats * dim**0.5 / q.square().sum(-1, keepdim=True))).half()
+        pool[block, 1, 0] = 0
+    return query, pool, tables, lengths
+
+
+def check_float16(got, args):
+    """As ``check``, but for what float16's range may cost a weight: its two parts hold it to 2^-22 of
+    itself, and to 2^-45 of the largest (half a subnormal step, 2^-25, of weights held at 2^9, whose
+    remainders are held at 2^11)."""
+    query, pool = args[0], args[1]
+    want, weight, size, top, count = formula(*args)
+    u, dim = 2.0**-24, query.shape[-1]
+    weights = (dim + 4) * u * size + 8 * u * top + 4 * u + (count + 16) * u + 2.0**-22
+    largest = store_of(pool).nan_to_num(0.0).abs().amax().item()
+    tol = 2.0**-11 * want.abs() + 2.0**-25 + 2 * weights * weight + count * 2.0**-45 * largest
+    error = (got.double().cpu() - want).abs()
+    over = error > tol
+    assert not over.any(), (error[over].max().item(), tol[over].max().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 32), (6, 2, 64), (3, 3, 96), (14, 2, 128), (2, 2, 256), (2, 1, 80)])
+@pytest.mark.parametrize("nats", [10.0, 15.0, 16.0, 17.5, 20.0, 24.0])
+def test_small_weights_of_float16_pools_count(gpu, heads, kv, dim, nats):
+    """A first key that leads a history by far and has no value: the output is what the small weights
+    of all other tokens leave, in a tile, in a wave's tiles and in the long launch's."""
+    for page, lengths, wide in ((16, [32, 2], 2), (16, [700, 97], 2), (5, [300], 2), (16, [20_000, 33], WIDE)):
+        for amplitude in (1.0, 60_000.0):
+            args = behind_one_key(heads, kv, dim, page, lengths, nats, amplitude, gpu, wide)
+            check_float16(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+def test_float16_scores_of_any_size(gpu):
+    """Scores that float32 holds only to 2^-3 .. 2^8: the weights stay finite, the largest one wins."""
+    for size in (1e3, 1e5, 6e6, 6e7):
+        query, pool, tables, lengths = case(2, 8, 2, 128, 16, [300, 40], "f16", "f16", gpu)
+        used = torch.where(pool.isnan(), pool, pool.sign() * pool.abs().clamp(0.25, 2.0))
+        pool[:, 0] = used[:, 0] * size**0.5
+        query = query.sign() * query.abs().clamp(0.25, 2.0) * size**0.5
+        got = attend_pages(query, pool, tables, lengths)
+        want, _, magnitude, _, _ = formula(query, pool, tables, lengths)
+        assert got.isfinite().all()
+        # a head whose best key leads by more than the scores' rounding has that key's value
+        store, group = store_of(pool), 4
+        for b, n in enumerate(lengths.tolist()):
+            token = torch.arange(n)
+            block = tables[b].cpu().long()[token // 16]
+            for h in range(8):
+                k, v = (store[block, plane, token % 16, h // group] for plane in (0, 1))
+                scores = (k @ query[b, h].cpu().double()) * 128**-0.5
+                first, second = scores.topk(2).values
+                if first - second > 20 + 2 * 140 * 2.0**-24 * magnitude[b, h].item():
+                    best = v[scores.argmax()]
+                    assert ((got[b, h].cpu().double() - best).abs() <= 2.0**-11 * best.abs() + 1e-5).all()
+
+
 def test_refusals_without_a_gpu():
     pool = QuantizedPool.empty(4, 16, 2, 8, torch.int8, "cpu")
     plain = torch.zeros(4, 2, 16, 2, 8)
