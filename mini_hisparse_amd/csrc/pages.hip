@@ -25,6 +25,7 @@
 
 #include "arrive.h"
 #include "codes.h"
+#include "page_parts.h"
 
 namespace hs {
 
@@ -343,7 +344,6 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
 // The running maximum moves only when a score passes it by more than SLACK (the sums then
 // hold weights up to 2^SLACK, no less precise): no cross-lane step in most tiles.
 
-constexpr int PM_TILE = 32;
 // Waves of a workgroup: half as many for 256 of the head dim, with twice the registers each.
 constexpr int mfma_waves(int64_t D) { return D > 128 ? 4 : 8; }
 constexpr int PM_PARTS = 8;  // parts of a short request
@@ -440,34 +440,6 @@ __device__ __forceinline__ T scan_lanes(T v) {
   return v;
 }
 
-// A request's tokens, at most `limit`, and their tiles.
-__device__ __forceinline__ int32_t clamp_length(int64_t n, int64_t limit) {
-  return static_cast<int32_t>(n < 0 ? 0 : (n < limit ? n : limit));
-}
-__device__ __forceinline__ int32_t tiles_of(int32_t n) {
-  return static_cast<int32_t>((static_cast<uint32_t>(n) + PM_TILE - 1) / PM_TILE);
-}
-
-// Parts are of `per` tiles, and an empty request has one.  All requests together are to need at
-// most `target` workgroups: with per = sum n_b / (target - B) they surely do (sum ceil(n_b / per)
-// <= sum n_b / per + B), but with sum n_b / target they may, as equal lengths often do.  The first
-// of PM_TRIES sizes from this one up to the sure one that does is taken, where B is above a quarter
-// of the target (fewer leave three quarters of the CUs busy in any case, and the search costs 1 us).
-// In us without and with the smaller sizes: 64 requests of 16384, 40 query and 8 KV heads of 128
-// in e4m3, 531 and 403; 128 of 4096, 28 and 4 heads in int8, 154 and 115.
-constexpr int PM_TRIES = 4;
-
-__device__ __forceinline__ uint32_t sure_room(const PagesArgs& a) {
-  return static_cast<uint32_t>(a.target - (a.B < a.target / 2 ? a.B : a.target / 2));
-}
-__device__ __forceinline__ uint32_t tried_size(uint32_t least, uint32_t sure, int k, uint32_t min_tiles) {
-  const uint32_t per = least + static_cast<uint32_t>(static_cast<uint64_t>(sure - least) * k / PM_TRIES);
-  return per < min_tiles ? min_tiles : per;
-}
-__device__ __forceinline__ int32_t parts_of(int32_t tiles, uint32_t per) {
-  return tiles > static_cast<int64_t>(per) ? static_cast<int32_t>((static_cast<uint32_t>(tiles) + per - 1) / per) : 1;
-}
-
 // The request and part of workgroup w, of up to PM_LANES requests: every wave derives the same
 // schedule from the lengths, one request a lane.
 __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& out) {
@@ -475,14 +447,11 @@ __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& o
   const int32_t n = lane < a.B ? clamp_length(a.lengths[lane], a.pages * a.P) : 0, tiles = tiles_of(n);
   const float total =
       __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scan_lanes(static_cast<float>(tiles))), 63));
-  const uint32_t room = sure_room(a), target = static_cast<uint32_t>(a.target), min_tiles = static_cast<uint32_t>(a.min_tiles);
-  // exact below 2^24 tiles; above, more than the sum's roundings can have lost
-  const uint32_t sum = static_cast<uint32_t>(total);
-  const uint32_t sure = total < 0x1p24f ? (sum + room - 1) / room
-                                        : static_cast<uint32_t>(total / static_cast<float>(room) * 1.0001f) + 1u;
+  const uint32_t target = static_cast<uint32_t>(a.target), min_tiles = static_cast<uint32_t>(a.min_tiles);
+  const uint32_t sure = sure_size(total, sure_room(a.target, a.B));
   uint32_t per = tried_size(sure, sure, 0, min_tiles);
   if (total < 0x1p24f && a.B * 4 > a.target) {
-    const uint32_t least = (sum + target - 1) / target;
+    const uint32_t least = (static_cast<uint32_t>(total) + target - 1) / target;
     uint32_t count[PM_TRIES / 2];  // two sizes' parts in 16 bits each: at most target + B
 #pragma unroll
     for (int k = 0; k < PM_TRIES; k += 2) {
@@ -525,9 +494,8 @@ __global__ __launch_bounds__(PS_T) void pages_schedule_kernel(PagesArgs a, int64
   total = 0;
 #pragma unroll
   for (int w = 0; w < PS_T / 64; ++w) total += s_tiles[w];
-  const int64_t room = sure_room(a);
   const uint32_t least = static_cast<uint32_t>((total + a.target - 1) / a.target);
-  const uint32_t sure = static_cast<uint32_t>((total + room - 1) / room), min_tiles = static_cast<uint32_t>(a.min_tiles);
+  const uint32_t sure = sure_size(total, sure_room(a.target, a.B)), min_tiles = static_cast<uint32_t>(a.min_tiles);
   uint32_t per = tried_size(sure, sure, 0, min_tiles);
   if (a.B <= a.target) {  // else every size gives more parts
     int32_t count[PM_TRIES] = {};

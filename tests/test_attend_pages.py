@@ -2,11 +2,13 @@
 row it may not use filled with NaN, and the calls it refuses."""
 
 import ctypes
+import shutil
+import subprocess
 
 import pytest
 import torch
 
-from mini_hisparse_amd import _lib
+from mini_hisparse_amd import _lib, build
 from mini_hisparse_amd.quantized import QuantizedPool, append_quantized
 from mini_hisparse_amd.row_kernels import attend_pages, attend_rows
 
@@ -522,3 +524,50 @@ def test_entry_point_refusals_without_a_gpu():
     size = lib.hs_attend_pages_workspace_bytes
     assert size(2, 3, 0, 1, 1, 64, 16, 1) == 256
     assert size(2, 3, 4, 14, 2, 64, 16, 10) == 0 and size(2, 3, 4, 14, 2, 64, 16, 1000) > 0  # one part, several
+
+
+PARTS = r"""
+#include "page_parts.h"
+#include <vector>
+using namespace hs;
+
+// Parts of B requests of n tokens and, of the first, `first`, at the sure size: by the schedule
+// written out (lanes = 0) and by that of a wave's lanes (whose sum is held in fp32).
+extern "C" int64_t parts_at_the_sure_size(int64_t B, int64_t n, int64_t first, int64_t target, int64_t min_tiles,
+                                          int lanes) {
+  const int64_t limit = 0x7fffffff;
+  const int32_t rest = tiles_of(clamp_length(n, limit)), one = tiles_of(clamp_length(first, limit));
+  const int64_t total = one + (B - 1) * static_cast<int64_t>(rest);
+  const uint32_t room = sure_room(target, B);
+  const uint32_t sure = lanes ? sure_size(static_cast<float>(total), room) : sure_size(total, room);
+  const uint32_t per = tried_size(sure, sure, 0, static_cast<uint32_t>(min_tiles));
+  return parts_of(one, per) + (B - 1) * static_cast<int64_t>(parts_of(rest, per));
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def part_arithmetic(tmp_path_factory):
+    if shutil.which(build.HIPCC) is None:
+        pytest.skip("hipcc is not installed")
+    folder = tmp_path_factory.mktemp("parts")
+    (folder / "parts.hip").write_text(PARTS)
+    command = [build.HIPCC, "--offload-host-only", "-shared", "-fPIC", "-O1", f"-I{build.CSRC}",
+               str(folder / "parts.hip"), "-o", str(folder / "parts.so")]
+    subprocess.run(command, check=True, capture_output=True)
+    count = ctypes.CDLL(str(folder / "parts.so")).parts_at_the_sure_size
+    count.restype, count.argtypes = ctypes.c_int64, [ctypes.c_int64] * 5 + [ctypes.c_int]
+    return count
+
+
+def test_parts_stay_within_their_slots_at_any_length(part_arithmetic):
+    """The sure size gives at most target + B parts, for which the workspace has slots, also where
+    the tiles of all requests are more than 32 bits hold."""
+    longest = 2**31 - 1
+    for batch in (1, 2, 63, 64, 65, 66, 128, 512, 16_384, 16_385, 32_769, 65_535):
+        for target in (1, 2, 3, 7, 64, 128, 256, 512):
+            for n in (0, 1, 33, 4096, 10**6, 2**30, 2**30 + 2**25, longest):
+                for first in (0, n, 2 * n // 3, longest):
+                    for lanes in (0, 1) if batch <= 64 else (0,):
+                        parts = part_arithmetic(batch, n, first, target, 1, lanes)
+                        assert batch <= parts <= target + batch, (batch, target, n, first, lanes, parts)
