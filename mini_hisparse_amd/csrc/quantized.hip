@@ -337,6 +337,8 @@ static int check_quantized(int64_t rows_n, int64_t kv_heads, int64_t head_dim, i
   HS_CHECK_ARG(valid_code(code), "invalid cache code %d", code);
   HS_CHECK_ARG(rows_n >= 0 && kv_heads >= 1 && head_dim >= 1 && head_dim <= 512 && page_size >= 1 && pool_rows >= 1,
                "quantised rows need positive sizes and a head_dim of at most 512");
+  // a page's V rows lie past its K rows, and the kernels divide rows by a page size of at most the rows
+  HS_CHECK_ARG(pool_rows % page_size == 0, "pool_rows must be those of whole pages");
   // head vectors, at up to 64 lanes each, are counted in 32 bits
   HS_CHECK_ARG(kv_heads <= (int64_t{1} << 20) && rows_n <= (int64_t{1} << 25) / kv_heads,
                "too many quantised head vectors in one call");

@@ -327,3 +327,16 @@ def test_entry_point_refusals_without_a_gpu():
     for bad in (*shared, dict(n=-1), dict(n=2**40)):
         assert read(**bad) == -1, bad
     assert append(tokens=0, k=None, rows=None) == 0 and read(n=0, k=None, rows=None) == 0  # nothing to do
+
+
+def test_pools_that_are_no_whole_pages_are_refused_without_a_gpu():
+    """A page longer than the pool (2^32 rows would be 0 in 32 bits) and a last page that the pool ends in."""
+    lib = _lib.load()
+    buffer = ctypes.create_string_buffer(256)
+    at = ctypes.addressof(buffer)
+    at += -at % 16
+    for pool_rows, page in ((4, 8), (4, 2**32), (2**31, 2**32), (4, 2**62), (7, 4), (2**33 + 1, 2**32)):
+        assert lib.hs_append_quantized(at, 8, 8, at, 8, 8, 0, at, 1, at, at, 3, pool_rows, page, 1, 8, None) == -1
+        assert b"whole pages" in lib.hs_last_error()
+        assert lib.hs_read_quantized(at, at, 3, pool_rows, page, 1, 8, at, 1, at, at, 0, None) == -1
+        assert b"whole pages" in lib.hs_last_error()
