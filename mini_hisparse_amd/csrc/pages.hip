@@ -1146,7 +1146,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
 // of 128 in 31.
 constexpr int PJ_T = 256;
 constexpr int PJ_U = 4;
-constexpr int PJ_SLOTS = 2048;  // weights held at once
+constexpr int PJ_SLOTS = 1024;  // of a request, at most (plan_pages: as many splits, or `target` parts)
 
 template <int C>
 __global__ __launch_bounds__(PJ_T) void pages_merge_kernel(PagesArgs a) {
@@ -1180,38 +1180,34 @@ __global__ __launch_bounds__(PJ_T) void pages_merge_kernel(PagesArgs a) {
   const int abreast = PJ_T / columns;
   const int g = threadIdx.x / columns, d = blockIdx.z * PJ_T * C + (threadIdx.x - g * columns) * C;
   float L = 0.f, O[C] = {};
-  for (int s0 = 0; s0 < r.count; s0 += PJ_SLOTS) {
-    const int n = r.count - s0 < PJ_SLOTS ? r.count - s0 : PJ_SLOTS;
-    if (s0) __syncthreads();
-    for (int s = threadIdx.x; s < n; s += PJ_T) {
-      const int64_t at = base + (s0 + s) * a.Hq;
-      const float m = a.part_m[at], l = a.part_l[at];
-      const float w = m == -INFINITY ? 0.f : exp2_(m - M);
-      s_w[s] = w;
-      L += w * l;
-    }
-    __syncthreads();
-    if (g < abreast && d < D) {
-      for (int s = g; s < n; s += abreast * PJ_U) {
-        float x[PJ_U][C];
+  for (int s = threadIdx.x; s < r.count; s += PJ_T) {
+    const int64_t at = base + s * a.Hq;
+    const float m = a.part_m[at], l = a.part_l[at];
+    const float w = m == -INFINITY ? 0.f : exp2_(m - M);
+    s_w[s] = w;
+    L += w * l;
+  }
+  __syncthreads();
+  if (g < abreast && d < D) {
+    for (int s = g; s < r.count; s += abreast * PJ_U) {
+      float x[PJ_U][C];
 #pragma unroll
-        for (int u = 0; u < PJ_U; ++u) {
-          const int at = s + u * abreast < n ? s + u * abreast : s;
-          const float* p = a.part_o + (base + (s0 + at) * a.Hq) * D + d;
-          if constexpr (C == 4) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(p);
+      for (int u = 0; u < PJ_U; ++u) {
+        const int at = s + u * abreast < r.count ? s + u * abreast : s;
+        const float* p = a.part_o + (base + at * a.Hq) * D + d;
+        if constexpr (C == 4) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(p);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[u][e] = v[e];
-          } else {
-            x[u][0] = *p;
-          }
+          for (int e = 0; e < 4; ++e) x[u][e] = v[e];
+        } else {
+          x[u][0] = *p;
         }
+      }
 #pragma unroll
-        for (int u = 0; u < PJ_U; ++u) {
-          const float w = s + u * abreast < n ? s_w[s + u * abreast] : 0.f;
+      for (int u = 0; u < PJ_U; ++u) {
+        const float w = s + u * abreast < r.count ? s_w[s + u * abreast] : 0.f;
 #pragma unroll
-          for (int e = 0; e < C; ++e) O[e] += w * x[u][e];
-        }
+        for (int e = 0; e < C; ++e) O[e] += w * x[u][e];
       }
     }
   }
@@ -1425,6 +1421,7 @@ extern "C" int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_
   PagesPlan p = plan_pages(shape, false, elem, batch, heads, kv_heads, head_dim, tokens);
   if (shape && !mfma)
     p = plan_pages(false, pages_workspace(p, batch, heads, head_dim) == 0, elem, batch, heads, kv_heads, head_dim, tokens);
+  HS_CHECK_ARG((p.mfma ? p.target : p.splits) <= PJ_SLOTS, "page attention plan with too many parts of a request");
   const int64_t need = pages_workspace(p, batch, heads, head_dim);
   HS_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need &&
                              (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),

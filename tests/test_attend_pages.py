@@ -532,15 +532,16 @@ PARTS = r"""
 using namespace hs;
 
 // Parts of B requests of n tokens and, of the first, `first`, at the sure size: by the schedule
-// written out (lanes = 0) and by that of a wave's lanes (whose sum is held in fp32).
+// written out (lanes <= 0) and by that of a wave's lanes (whose sum is held in fp32).
 extern "C" int64_t parts_at_the_sure_size(int64_t B, int64_t n, int64_t first, int64_t target, int64_t min_tiles,
                                           int lanes) {
   const int64_t limit = 0x7fffffff;
   const int32_t rest = tiles_of(clamp_length(n, limit)), one = tiles_of(clamp_length(first, limit));
   const int64_t total = one + (B - 1) * static_cast<int64_t>(rest);
   const uint32_t room = sure_room(target, B);
-  const uint32_t sure = lanes ? sure_size(static_cast<float>(total), room) : sure_size(total, room);
+  const uint32_t sure = lanes > 0 ? sure_size(static_cast<float>(total), room) : sure_size(total, room);
   const uint32_t per = tried_size(sure, sure, 0, static_cast<uint32_t>(min_tiles));
+  if (B == 1 || lanes < 0) return parts_of(one, per);  // of the first request alone
   return parts_of(one, per) + (B - 1) * static_cast<int64_t>(parts_of(rest, per));
 }
 """
@@ -571,3 +572,17 @@ def test_parts_stay_within_their_slots_at_any_length(part_arithmetic):
                     for lanes in (0, 1) if batch <= 64 else (0,):
                         parts = part_arithmetic(batch, n, first, target, 1, lanes)
                         assert batch <= parts <= target + batch, (batch, target, n, first, lanes, parts)
+                    # the merge holds the weights of one request's slots
+                    assert part_arithmetic(batch, n, first, target, 1, -1) <= max(1, target)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,code,dtype,lengths", [
+    (1, 1, 80, "int8", "bf16", [262_139]),  # 1024 splits of the general kernel, by four columns and by one
+    (2, 1, 81, "bf16", "bf16", [262_140]),
+    (2, 1, 32, "int8", "bf16", [70_000]),  # 256 parts of the long launch
+    (2, 1, 32, "f16", "f16", [140_000] + [0] * 60 + [17] * 10),  # nearly 512 of one request
+])
+def test_as_many_slots_as_a_request_can_have(gpu, heads, kv, dim, code, dtype, lengths):
+    args = case(len(lengths), heads, kv, dim, 16, lengths, code, dtype, gpu)
+    check(attend_pages(*args), args)
