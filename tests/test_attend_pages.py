@@ -586,3 +586,89 @@ def test_parts_stay_within_their_slots_at_any_length(part_arithmetic):
 def test_as_many_slots_as_a_request_can_have(gpu, heads, kv, dim, code, dtype, lengths):
     args = case(len(lengths), heads, kv, dim, 16, lengths, code, dtype, gpu)
     check(attend_pages(*args), args)
+
+
+def formula_on_the_device(query, pool, tables, lengths):
+    """``formula`` for histories of many tokens: the same sums in 64 bits, on the device; a table's pages
+    may repeat."""
+    codes, scales = (pool.codes, pool.scales) if isinstance(pool, QuantizedPool) else (pool, None)
+    store = codes.float().double() if scales is None else codes.float().double() * scales.double()[..., None]
+    store = store.nan_to_num(0.0)  # the rows that no request may use
+    blocks, _, page, kv, dim = store.shape
+    batch, heads, _ = query.shape
+    parts = [torch.zeros(batch, heads, n, dtype=torch.float64, device=query.device) for n in (dim, dim, 1, 1, 1)]
+    head = torch.arange(kv, device=query.device)[:, None]
+    for b, n in enumerate(lengths.tolist()):
+        token = torch.arange(n, device=query.device)
+        block = tables[b].long().expand(kv, -1)[:, token // page]  # [kv, n]
+        keep = ((block >= 0) & (block < blocks))[:, None]
+        k, v = (store[block.clamp(0, blocks - 1), plane, token % page, head] * keep.transpose(1, 2) for plane in (0, 1))
+        q = query[b].double().view(kv, -1, dim)
+        scores = ((q @ k.transpose(1, 2)) * dim**-0.5).masked_fill(~keep, float("-inf"))
+        p = torch.softmax(scores, -1).nan_to_num(0.0)  # no token at all
+        size = (q.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * dim**-0.5
+        top = scores.masked_fill(~keep, 0.0).abs().amax(-1, keepdim=True)
+        count = keep.sum(-1, keepdim=True).double().expand(top.shape)
+        for part, x in zip(parts, (p @ v, p @ v.abs(), size, top, count)):
+            part[b] = x.reshape(heads, -1)
+    return [x.cpu() for x in parts]
+
+
+def long_waves(tiles, batch, kv, dim, page, code, dtype, device, per_head=False, holes=()):
+    """A batch for which a wave of the long launch has about ``tiles`` tiles (one head a KV head; 128
+    workgroups of two waves for each of four of them): equal parts, two requests' worth of parts at least.
+    Pages repeat; those from ``holes`` are absent.  Blocks 0 and 1 are in no table and NaN."""
+    gen = torch.Generator().manual_seed(tiles + batch + dim + page)
+    tokens = tiles * 2 * 32 * 128 // batch
+    lengths = [tokens - (7 * b) % 29 for b in range(batch)]  # the last tile and half of a page in part
+    blocks, width, lists = 300, -(-tokens // page) + 3, kv if per_head else 1
+    tables = torch.randint(2, blocks, (batch, lists, width), generator=gen)
+    for first, last in holes:
+        tables[:, :, first:last] = torch.tensor([-1, blocks, 2**31 - 1])[torch.arange(last - first) % 3]
+    values = torch.randn(blocks, 2, page, kv, dim, generator=gen)
+    stored, scales = rows_of(values, code)
+    (stored if scales is None else scales)[:2] = float("nan")
+    tables = (tables if per_head else tables[:, 0]).to(torch.int32).to(device)
+    pool = stored.to(device) if scales is None else QuantizedPool(stored.to(device), scales.to(device))
+    query = torch.randn(batch, kv, dim, generator=gen).to(PLAIN[dtype]).to(device)
+    return query, pool, tables, torch.tensor(lengths, dtype=torch.int32, device=device)
+
+
+def check_long(got, args):
+    """``check``'s bound (float16 pools as in ``check_float16``) against the sums on the device."""
+    query, pool = args[0], args[1]
+    want, weight, size, top, count = formula_on_the_device(*args)
+    u, dim, plain = 2.0**-24, query.shape[-1], not isinstance(pool, QuantizedPool)
+    held = 2.0**-24 if query.dtype == torch.float32 else 2.0**-22 if plain and query.dtype == torch.float16 else 2.0**-16
+    weights = (dim + 4) * u * size + 8 * u * top + 4 * u + (count + 16) * u + held
+    tol = torch.finfo(query.dtype).eps / 2 * want.abs() + 2 * weights * weight
+    if query.dtype == torch.float16:
+        tol = tol + 2.0**-25 + count * 2.0**-45 * 9.0  # no |V| of these is above 9
+    error = (got.double().cpu() - want).abs()
+    over = error > tol
+    assert not over.any(), (error[over].max().item(), tol[over].max().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("e4m3", "f16"), ("bf16", "bf16"), ("f16", "f16"),
+                                        ("f32", "f32")])
+@pytest.mark.parametrize("tiles", [31, 32, 33, 64, 70])
+def test_waves_of_more_tiles_than_a_batch_of_table_entries(gpu, tiles, code, dtype):
+    """A wave reads the table for 32 of its tiles at a time: one batch, exactly and in part, two, and
+    a third in part; absent pages in the middle of a batch, over a whole one, at the end."""
+    pages = tiles * 2 * 32 * 128 // 64 // 16  # of a request of 64, whose two parts are tiles * 4 pages each
+    half, third = pages // 2, pages // 3  # 128 pages are a wave's 32 tiles and its neighbour's
+    for batch, holes in ((64, ()), (63, ()), (80, ()),
+                         (64, ((5, 9), (third, third + 9), (pages - 20, pages))),
+                         (64, ((0, half),)), (64, ((half, min(half + 128, pages)),)), (64, ((120, min(260, pages)),))):
+        args = long_waves(tiles, batch, 8, 64, 16, code, dtype, gpu, holes=holes)
+        check_long(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("dim,page", [(64, 48), (64, 12), (128, 16), (96, 32), (256, 16)])
+def test_long_waves_at_other_pages_and_head_dims(gpu, dim, page, code, dtype):
+    for per_head in (False, True):
+        args = long_waves(40, 60, 4, dim, page, code, dtype, gpu, per_head=per_head, holes=((30, 90),))
+        check_long(attend_pages(*args), args)
