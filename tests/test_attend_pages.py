@@ -672,3 +672,30 @@ def test_long_waves_at_other_pages_and_head_dims(gpu, dim, page, code, dtype):
     for per_head in (False, True):
         args = long_waves(40, 60, 4, dim, page, code, dtype, gpu, per_head=per_head, holes=((30, 90),))
         check_long(attend_pages(*args), args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("int8", "bf16"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("dim,wide", [(64, 2), (64, WIDE), (80, 2)])
+def test_what_the_other_requests_hold_does_not_change_one(gpu, dim, wide, code, dtype):
+    """A request's bits depend on the sizes and lengths of its batch, not on what the other requests'
+    queries, tables and rows hold (NaN among them).  In a batch of its own it may be cut into other
+    parts, so there it agrees with the formula."""
+    lengths = [900, 1500, 900, 33]
+    query, pool, tables, lengths = case(4, 14, 2, dim, 16, lengths, code, dtype, gpu, wide=wide)
+    first = attend_pages(query, pool, tables, lengths)
+    assert torch.equal(first, attend_pages(query, pool, tables, lengths))
+    alone = [t[1:2].contiguous() for t in (query, tables, lengths)]
+    alone = (alone[0], pool, *alone[1:])
+    check(attend_pages(*alone), alone)
+    check(first[1:2], alone)
+    others = [0, 2, 3]
+    query, tables = query.clone(), tables.clone()
+    query[others] = -3 * query[others]
+    tables[0] = tables[2].clone()
+    tables[2, 3] = -1
+    block = tables[3, 0].item()  # all of the last request's first page
+    (pool.scales if code in CODES else pool)[block] = float("nan")
+    again = attend_pages(query, pool, tables, lengths)
+    assert torch.equal(again[1], first[1])
+    assert again[3].isnan().all() and not torch.equal(again[0], first[0])
