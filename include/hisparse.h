@@ -422,11 +422,13 @@ int hs_attend_window(const void* query, int64_t q_stride_h, const void* pool, in
  *            past `blocks` is an absent page, whose tokens are masked
  *   lengths  int32 [batch] on the device: tokens of each request (clamped to 0 ..
  *            pages * P); rows past them are never used
- *   out      [batch, heads, head_dim] in query_dtype; 0 for a request without a token
+ *   out      [batch, heads, head_dim] in query_dtype; 0 for a request without a token, and for
+ *            a head all of whose scores are -inf (infinite keys); a score of +inf gives NaN
  * Scores, softmax statistics and sums are fp32.  On the matrix cores a weight enters the
  * second product as a sum of 16-bit parts, to 2^-16 of itself (8-bit pools with a float32
  * query 2^-24; float16 pools 2^-22, and 2^-45 of the largest weight; float32 pools and other
- * head dims fp32).  The workspace
+ * head dims fp32), and weights reach 2^6 before they are divided by their sum: values above
+ * 2^121 may overflow.  The workspace
  * (hs_attend_pages_workspace_bytes of the same sizes; 0: none, null then; 16-byte aligned)
  * may hold anything before a call; calls that share one must run in order.  Nothing is read on
  * the host, so a captured call replays with the tables and lengths of the moment.  head_dim at
@@ -511,7 +513,8 @@ int hs_attend_time_next(void* start_event, void* stop_event);
  * hs_norm_rotary_split: hs_rotary_split with a per-head RMSNorm of q and k before the
  *   rotation (weights q_weight and k_weight [head_dim], `eps` added to the mean square; no
  *   counterpart in the reference, whose heads are not normed).  Computed in fp32 with the
- *   angles position * theta^(-2i/D) reduced in 64 bits, and rounded once.  head_dim <= 512.
+ *   angles position * theta^(-2i/D) reduced in 64 bits, and rounded once (elements above
+ *   2^63 / sqrt(D) overflow the sum of squares, and their head gives zeros).  head_dim <= 512.
  * hs_silu_mul: out[row, j] = silu(g[row, j]) * u[row, j] where a gate_up row
  *   holds g (width) then u (width).
  */

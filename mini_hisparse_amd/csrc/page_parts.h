@@ -23,7 +23,7 @@ __host__ __device__ __forceinline__ int32_t tiles_of(int32_t n) {
 // of PM_TRIES sizes from this one up to the sure one that does is taken, where B is above a quarter
 // of the target (fewer leave three quarters of the CUs busy in any case, and the search costs 1 us).
 // In us without and with the smaller sizes: 64 requests of 16384, 40 query and 8 KV heads of 128
-// in e4m3, 531 and 403; 128 of 4096, 28 and 4 heads in int8, 154 and 115.
+// in e4m3, 526 and 389; 128 of 4096, 28 and 4 heads in int8, 126 and 118.
 constexpr int PM_TRIES = 4;
 
 __host__ __device__ __forceinline__ uint32_t sure_room(int64_t target, int64_t B) {

@@ -287,7 +287,9 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
     Scores, softmax statistics and sums are float32.  Where the matrix cores run (head dims
     32, 64, 96, 128 and, but for float32 pools, 256) a weight enters the product with V to
     2^-16 of itself (float16 pools 2^-22 and 2^-45 of the largest weight, 8-bit pools with a
-    float32 query 2^-24, float32 pools in full).
+    float32 query 2^-24, float32 pools in full).  A NaN in a used row, or a score of +inf, makes
+    its heads' outputs NaN; a token whose score is -inf has no weight, and if no other is left
+    the output is zeros.
     """
     quantized = isinstance(pool, QuantizedPool)
     store = pool.codes if quantized else pool

@@ -699,3 +699,39 @@ def test_what_the_other_requests_hold_does_not_change_one(gpu, dim, wide, code, 
     again = attend_pages(query, pool, tables, lengths)
     assert torch.equal(again[1], first[1])
     assert again[3].isnan().all() and not torch.equal(again[0], first[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,dtype", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("dim,wide", [(64, 2), (64, WIDE), (80, 2), (256, 2)])
+def test_infinite_scores(gpu, dim, wide, code, dtype):
+    """Tokens of score -inf have no weight, as in the formula; a head that has no others gives zeros (the
+    formula has no value there); +inf gives NaN.  Other heads and requests are not touched."""
+    query, pool, tables, lengths = case(2, 4, 2, dim, 16, [700, 700], code, dtype, gpu, wide=wide)
+    plain = not isinstance(pool, QuantizedPool)
+    query[:, :, 0] = query[:, :, 0].abs() + 1
+    want = attend_pages(query, pool, tables, lengths)
+    order = tables.long()[:, :44]
+
+    def with_keys(first, last, value):  # of request 0, KV head 1: pages first .. last
+        store = (pool if plain else pool.scales).clone()
+        for block in order[0, first:last].tolist():
+            if plain:
+                store[block, 0, :, 1, 0] = value
+            else:
+                store[block, 0, :, 1] = value  # a scale: the sign of a score is its code's
+        return store if plain else QuantizedPool(pool.codes, store)
+
+    if plain:
+        some = attend_pages(query, with_keys(3, 30, -float("inf")), tables, lengths)
+        gone = tables[:1, None].repeat(1, 2, 1)
+        gone[:, 1, 3:30] = -1  # the same tokens masked
+        args = (query[:1], pool, gone, lengths[:1])
+        check(some[:1], args)
+        assert torch.equal(some[1], want[1])
+        none = attend_pages(query, with_keys(0, 44, -float("inf")), tables, lengths)
+        assert (none[0, 2:] == 0).all()
+        assert torch.equal(none[0, :2], want[0, :2]) and torch.equal(none[1], want[1])
+    lost = attend_pages(query, with_keys(5, 6, float("inf")), tables, lengths)
+    assert lost[0, 2:].isnan().all()
+    assert torch.equal(lost[0, :2], want[0, :2]) and torch.equal(lost[1], want[1])
