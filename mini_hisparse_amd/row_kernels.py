@@ -282,7 +282,8 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
     page whose tokens are masked; lengths int32 [B], tokens of each request (a row of the
     tables past them is not read).  Tables and lengths are read on the device, so a captured
     call replays with their contents of the moment.  Returns [B, Hq, D] in the query dtype
-    (``out`` when given); zeros for a request without a token.
+    (``out`` when given); zeros for a request without a token.  The launch is chosen from the
+    tables' width: one no wider than the histories need is faster for short ones.
 
     Scores, softmax statistics and sums are float32.  Where the matrix cores run (head dims
     32, 64, 96, 128 and, but for float32 pools, 256) a weight enters the product with V to
