@@ -460,8 +460,8 @@ int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_stride_h, i
  *   k, v   hs_append_quantized: [tokens, Hkv, D] in `dtype`, element strides per token and
  *          head; hs_read_quantized: [n, Hkv, D] contiguous out, code * scale rounded to
  *          `dtype`
- * pool_rows = blocks * P (other values are refused); head_dim at most 512; tokens or n may be 0, and times kv_heads at
- * most 2^25.
+ * pool_rows = blocks * P (refused where it is no multiple of P); head_dim at most 512; tokens or
+ * n may be 0, and times kv_heads at most 2^25.
  */
 int hs_append_quantized(const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, int32_t dtype, const int64_t* rows, int64_t tokens, void* codes,

@@ -360,8 +360,8 @@ __device__ __forceinline__ float lift_at(float m) { return F16 && fabsf(m) < 0x1
 template <int S>
 constexpr int elem_size() { return S == HS_DTYPE_F32 ? 4 : (quantised(S) ? 1 : 2); }
 
-// Parts of a query, and of a weight.  Two parts of a weight lose at most 2^-16 of it, and the output
-// is then rounded to half a step of 2^-8 (bf16) or 2^-11 (float16): 0.2% of bf16 outputs and 1.4% of
+// Parts of a query, and of a weight.  Two parts of a weight lose at most 2^-16 of it, and the output's
+// own rounding is off by up to 2^-8 (bf16) or 2^-11 (float16) of it: 0.2% of bf16 outputs and 1.4% of
 // float16's (8-bit pools) are another neighbour than the 64-bit result rounded, with a third part
 // 0.03% and 0.12%, where the mean distance to it is the rounding's in all of them.  The third part
 // took 16 requests of 4096 tokens, 8 KV heads of 64 in int8, from 22.0 to 23.0 us, 8 of 131072 with
