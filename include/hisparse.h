@@ -48,6 +48,10 @@ extern "C" {
  * 8-bit floats of four significand bits (largest 448, no infinity) */
 #define HS_DTYPE_I8 3
 #define HS_DTYPE_E4M3 4
+/* 4-bit floats (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte, the even element in the low
+ * half.  Every 32 neighbours of a head vector or a weight row share a scale byte: e stands for
+ * 2^(e - 127), 255 for NaN. */
+#define HS_DTYPE_E2M1 6
 
 typedef struct ihipStream_t* hs_stream_t;
 
@@ -416,7 +420,8 @@ int hs_attend_window(const void* query, int64_t q_stride_h, const void* pool, in
  *            contiguous)
  *   pool     [blocks, 2, P, Hkv, D]: float32, float16 or bfloat16 (then query_dtype is
  *            pool_code and scales is null), or the codes of hs_append_quantized with their
- *            scales [blocks, 2, P, Hkv] (any query_dtype)
+ *            scales: float32 [blocks, 2, P, Hkv], or for HS_DTYPE_E2M1 bytes
+ *            [blocks, 2, P, Hkv, D / 32] beside codes [blocks, 2, P, Hkv, D / 2] (any query_dtype)
  *   tables   int32 [batch, pages] (t_stride_k = 0) or [batch, kv_heads, pages]: token t of
  *            a request sits in row t % P of block table[t / P]; an entry below 0 or at or
  *            past `blocks` is an absent page, whose tokens are masked
@@ -425,34 +430,53 @@ int hs_attend_window(const void* query, int64_t q_stride_h, const void* pool, in
  *   out      [batch, heads, head_dim] in query_dtype; 0 for a request without a token, and for
  *            a head all of whose scores are -inf (infinite keys); a score of +inf gives NaN
  * Scores, softmax statistics and sums are fp32.  On the matrix cores a weight enters the
- * second product as a sum of 16-bit parts, to 2^-16 of itself (8-bit pools with a float32
+ * second product as a sum of 16-bit parts, to 2^-16 of itself (8- and 4-bit pools with a float32
  * query 2^-24; float16 pools 2^-22, and 2^-45 of the largest weight; float32 pools and other
  * head dims fp32), and weights reach 2^6 before they are divided by their sum: values above
  * 2^121 may overflow.  The workspace
  * (hs_attend_pages_workspace_bytes of the same sizes; 0: none, null then; 16-byte aligned)
  * may hold anything before a call; calls that share one must run in order.  Nothing is read on
  * the host, so a captured call replays with the tables and lengths of the moment.  head_dim at
- * most 512 (32, 64, 96, 128 and, but for float32 pools, 256 run on the matrix cores), batch and
- * heads at most 65535, pages * page_size below 2^31.
+ * most 512, of HS_DTYPE_E2M1 a multiple of 32 (32, 64, 96, 128 and, but for float32 pools, 256 run on
+ * the matrix cores), batch and heads at most 65535, pages * page_size below 2^31.
+ *
+ * hs_attend_pages_window: token t of a request of n counts only where t >= n - window or
+ * t < sinks (window 0: every token, sinks 0 then); the others' rows are not used, whatever their
+ * pages hold, and whole tiles of 32 of them are not read.  The first kept tokens are attended at
+ * the rotation they were written with.
  */
 int64_t hs_attend_pages_workspace_bytes(int32_t query_dtype, int32_t pool_code, int64_t batch, int64_t heads,
                                         int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t pages);
 int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_stride_h, int32_t query_dtype,
-                    const void* pool, const float* scales, int32_t pool_code, int64_t blocks, int64_t page_size,
+                    const void* pool, const void* scales, int32_t pool_code, int64_t blocks, int64_t page_size,
                     int64_t kv_heads, int64_t head_dim, const int32_t* tables, int64_t t_stride_b,
                     int64_t t_stride_k, int64_t pages, const int32_t* lengths, int64_t batch, int64_t heads,
                     void* out, int64_t o_stride_b, int64_t o_stride_h, void* workspace, int64_t workspace_bytes,
                     hs_stream_t stream);
+int64_t hs_attend_pages_window_workspace_bytes(int32_t query_dtype, int32_t pool_code, int64_t batch, int64_t heads,
+                                               int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t pages,
+                                               int64_t window, int64_t sinks);
+int hs_attend_pages_window(const void* query, int64_t q_stride_b, int64_t q_stride_h, int32_t query_dtype,
+                           const void* pool, const void* scales, int32_t pool_code, int64_t blocks, int64_t page_size,
+                           int64_t kv_heads, int64_t head_dim, const int32_t* tables, int64_t t_stride_b,
+                           int64_t t_stride_k, int64_t pages, const int32_t* lengths, int64_t batch, int64_t heads,
+                           int64_t window, int64_t sinks, void* out, int64_t o_stride_b, int64_t o_stride_h,
+                           void* workspace, int64_t workspace_bytes, hs_stream_t stream);
 
 /* ------------------------------------------------------- quantised KV rows */
 
 /*
- * 8-bit K/V rows of a paged pool; no counterpart in the reference.  The pool is codes
+ * 8- and 4-bit K/V rows of a paged pool; no counterpart in the reference.  The pool is codes
  * [blocks, 2, P, Hkv, D] (code HS_DTYPE_I8 or HS_DTYPE_E4M3) and scales [blocks, 2, P, Hkv]
  * float32.  Per head vector of largest magnitude a: scale = a / top rounded to float32 (top
  * 127 or 448), each code the nearest to the exact quotient by the scale (ties to even);
  * zeros give scale 0; a vector with a NaN or infinity gets scale NaN and codes 0, and so
  * reads back as NaN.
+ * HS_DTYPE_E2M1: codes [blocks, 2, P, Hkv, D / 2], two to a byte, and scale bytes
+ * [blocks, 2, P, Hkv, D / 32].  Per 32 neighbours of largest magnitude a the scale is the smallest
+ * power of two, from 2^-126 on, that is at least a / 7; each code the nearest to the exact
+ * quotient (ties to even, at most 6); 32 neighbours with a NaN or infinity get scale NaN and
+ * codes 0.  D is a multiple of 32.
  *   rows   int64 on the device: physical rows (block * P + offset).  hs_append_quantized
  *          skips a row outside [0, pool_rows); rows of one call must differ (of two equal
  *          ones the codes and the scale may come from different tokens).  hs_read_quantized
@@ -465,9 +489,9 @@ int hs_attend_pages(const void* query, int64_t q_stride_b, int64_t q_stride_h, i
  */
 int hs_append_quantized(const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
                         int64_t v_stride_h, int32_t dtype, const int64_t* rows, int64_t tokens, void* codes,
-                        float* scales, int32_t code, int64_t pool_rows, int64_t page_size, int64_t kv_heads,
+                        void* scales, int32_t code, int64_t pool_rows, int64_t page_size, int64_t kv_heads,
                         int64_t head_dim, hs_stream_t stream);
-int hs_read_quantized(const void* codes, const float* scales, int32_t code, int64_t pool_rows, int64_t page_size,
+int hs_read_quantized(const void* codes, const void* scales, int32_t code, int64_t pool_rows, int64_t page_size,
                       int64_t kv_heads, int64_t head_dim, const int64_t* rows, int64_t n, void* k, void* v,
                       int32_t dtype, hs_stream_t stream);
 

@@ -13,7 +13,7 @@ from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libhisparse_hip.so"
 
-HS_DTYPE_F32, HS_DTYPE_F16, HS_DTYPE_BF16, HS_DTYPE_I8, HS_DTYPE_E4M3 = 0, 1, 2, 3, 4
+HS_DTYPE_F32, HS_DTYPE_F16, HS_DTYPE_BF16, HS_DTYPE_I8, HS_DTYPE_E4M3, HS_DTYPE_E2M1 = 0, 1, 2, 3, 4, 6
 
 
 class HipLibraryError(RuntimeError):
@@ -155,6 +155,15 @@ SIGNATURES = {
          c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
          c_int64, c_void_p],
     ),
+    "hs_attend_pages_window_workspace_bytes": (
+        c_int64, [c_int32, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64],
+    ),
+    "hs_attend_pages_window": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64,
+         c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64,
+         c_void_p, c_int64, c_void_p],
+    ),
     "hs_silu_mul": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p]),
     "hs_uniform_pages": (
         c_int, [c_uint64, c_uint64, POINTER(c_int64), c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p],
@@ -240,7 +249,7 @@ def _element_codes():
     import torch
 
     _DTYPE_CODES.update({torch.float32: HS_DTYPE_F32, torch.float16: HS_DTYPE_F16, torch.bfloat16: HS_DTYPE_BF16,
-                         torch.int8: HS_DTYPE_I8, torch.float8_e4m3fn: HS_DTYPE_E4M3})
+                         torch.int8: HS_DTYPE_I8, torch.float8_e4m3fn: HS_DTYPE_E4M3, torch.float4_e2m1fn_x2: HS_DTYPE_E2M1})
     return _DTYPE_CODES
 
 
@@ -255,7 +264,7 @@ def cache_code(dtype) -> int:
     """Element code of a quantised pool's codes."""
     code = (_DTYPE_CODES or _element_codes()).get(dtype, 0)
     if code < HS_DTYPE_I8:
-        raise ValueError("cache codes must be int8 or float8_e4m3fn")
+        raise ValueError("cache codes must be int8, float8_e4m3fn or float4_e2m1fn_x2")
     return code
 
 

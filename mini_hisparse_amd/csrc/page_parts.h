@@ -17,6 +17,39 @@ __host__ __device__ __forceinline__ int32_t tiles_of(int32_t n) {
   return static_cast<int32_t>((static_cast<uint32_t>(n) + PM_TILE - 1) / PM_TILE);
 }
 
+// A window shows a request's newest `window` tokens and its first `sinks`: those from `lo` on and
+// those below `sinks`.  The whole tiles between them are passed over: of the tiles that are walked,
+// those below `front` are the request's own, the others lie `gap` further on.
+constexpr int32_t NO_WINDOW = 0x7fffffff;  // no request is longer
+
+struct Seen {
+  int32_t lo, front, gap;
+};
+__host__ __device__ __forceinline__ Seen seen_of(int32_t n, int32_t window, int32_t sinks) {
+  const int32_t lo = n > window ? n - window : 0, first = lo / PM_TILE, front = tiles_of(sinks);
+  return Seen{lo, front, first > front ? first - front : 0};
+}
+__host__ __device__ __forceinline__ int32_t seen_tiles(int32_t n, int32_t window, int32_t sinks) {
+  return tiles_of(n) - seen_of(n, window, sinks).gap;
+}
+// The tokens (bits) of the tile from token `base` < lo on that are seen.
+__host__ __device__ __forceinline__ uint32_t seen_mask(int32_t base, int32_t lo, int32_t sinks) {
+  const int32_t before = lo - base, first = sinks - base;
+  return (before < PM_TILE ? 0xffffffffu << before : 0u) |
+         (first <= 0 ? 0u : (first < PM_TILE ? (1u << first) - 1u : 0xffffffffu));
+}
+// The most tokens, and tiles, that any request of up to `tokens` has to see (its window may begin
+// inside a tile).
+__host__ __device__ __forceinline__ int64_t most_seen(int64_t tokens, int32_t window, int32_t sinks) {
+  const int64_t seen = static_cast<int64_t>(window) + sinks;
+  return seen < tokens ? seen : tokens;
+}
+__host__ __device__ __forceinline__ int64_t most_seen_tiles(int64_t tokens, int32_t window, int32_t sinks) {
+  const int64_t all = (tokens + PM_TILE - 1) / PM_TILE;
+  const int64_t seen = (static_cast<int64_t>(window) + PM_TILE - 2) / PM_TILE + 1 + tiles_of(sinks);
+  return seen < all ? seen : all;
+}
+
 // Parts are of `per` tiles, and an empty request has one.  All requests together are to need at
 // most `target` workgroups: with per = sum n_b / (target - B) they surely do (sum ceil(n_b / per)
 // <= sum n_b / per + B), but with sum n_b / target they may, as equal lengths often do.  The first

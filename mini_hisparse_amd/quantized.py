@@ -1,8 +1,11 @@
-"""8-bit K/V rows: a quantised paged pool, written and read by the gfx950 kernels.
+"""8- and 4-bit K/V rows: a quantised paged pool, written and read by the gfx950 kernels.
 
 A :class:`QuantizedPool` has the layout of a plain pool, ``codes`` [blocks, 2, P, Hkv, D]
 (int8 or float8_e4m3fn) beside ``scales`` [blocks, 2, P, Hkv] float32, one scale per head
-vector; a row takes ``2 Hkv (D + 4)`` bytes.  :func:`append_quantized` quantises rows as
+vector; a row takes ``2 Hkv (D + 4)`` bytes.  In 4 bits, ``codes`` [blocks, 2, P, Hkv, D / 2]
+(float4_e2m1fn_x2: two values a byte, the even one in the low half) stand beside ``scales``
+[blocks, 2, P, Hkv, D / 32] (float8_e8m0fnu), a power of two for every 32 neighbours; a row
+takes ``2 Hkv (D / 2 + D / 32)`` bytes.  :func:`append_quantized` quantises rows as
 they are written (a prompt's or one token of each request), :func:`read_quantized` widens
 rows again, and ``row_kernels.attend_pages`` attends over the codes themselves.  Rows are
 named by physical row (block * P + offset), as everywhere in this package; a call takes up
@@ -18,25 +21,35 @@ import torch
 
 from . import _lib
 
+FP4_GROUP = 32  # neighbours that share a scale of 4-bit codes
+
 
 @dataclass(frozen=True, eq=False)
 class QuantizedPool:
     """Codes and scales of one pool; ``blocks``, ``page_size``, ``kv_heads``, ``head_dim`` and
     ``rows`` (blocks * page_size) are read off them."""
 
-    codes: torch.Tensor  # [blocks, 2, P, Hkv, D] int8 or float8_e4m3fn
-    scales: torch.Tensor  # [blocks, 2, P, Hkv] float32
+    codes: torch.Tensor  # [blocks, 2, P, Hkv, D] int8 or float8_e4m3fn, or [.., D / 2] float4_e2m1fn_x2
+    scales: torch.Tensor  # [blocks, 2, P, Hkv] float32, or for 4-bit codes [.., D / 32] float8_e8m0fnu
 
     def __post_init__(self):
         codes, scales = self.codes, self.scales
         code = _lib.cache_code(codes.dtype)
         if codes.dim() != 5 or codes.shape[1] != 2 or 0 in codes.shape or not codes.is_contiguous():
             raise ValueError("codes must be contiguous [blocks, 2, page_size, kv_heads, head_dim]")
-        if scales.shape != codes.shape[:-1] or scales.dtype != torch.float32 or not scales.is_contiguous():
+        four = code == _lib.HS_DTYPE_E2M1
+        if four:
+            if codes.shape[4] % (FP4_GROUP // 2):
+                raise ValueError("4-bit pools need a head_dim of a multiple of 32")
+            if scales.shape != (*codes.shape[:-1], codes.shape[4] * 2 // FP4_GROUP) \
+                    or scales.dtype != torch.float8_e8m0fnu or not scales.is_contiguous():
+                raise ValueError("scales must be contiguous float8_e8m0fnu [blocks, 2, page_size, kv_heads, head_dim / 32]")
+        elif scales.shape != codes.shape[:-1] or scales.dtype != torch.float32 or not scales.is_contiguous():
             raise ValueError("scales must be contiguous float32 [blocks, 2, page_size, kv_heads]")
         if scales.device != codes.device:
             raise ValueError("codes and scales must be on one device")
         blocks, _, page_size, kv_heads, head_dim = codes.shape
+        head_dim = 2 * head_dim if four else head_dim
         for name, value in (("blocks", blocks), ("page_size", page_size), ("kv_heads", kv_heads),
                             ("head_dim", head_dim), ("rows", blocks * page_size), ("code", code),
                             ("device", codes.device), ("vector", (kv_heads, head_dim))):
@@ -46,12 +59,20 @@ class QuantizedPool:
     def empty(cls, blocks, page_size, kv_heads, head_dim, dtype=torch.int8, device="cuda"):
         """A pool of zeros: every row reads back as zero until it is written."""
         shape = (blocks, 2, page_size, kv_heads, head_dim)
+        if dtype == torch.float4_e2m1fn_x2:
+            if head_dim % FP4_GROUP:
+                raise ValueError("4-bit pools need a head_dim of a multiple of 32")
+            codes, scales = (torch.zeros((*shape[:-1], n), dtype=torch.uint8, device=device)
+                             for n in (head_dim // 2, head_dim // FP4_GROUP))
+            return cls(codes.view(dtype), scales.view(torch.float8_e8m0fnu))
         codes = torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype)
         return cls(codes, torch.zeros(shape[:-1], device=device))
 
     @property
     def row_bytes(self):
         """Bytes of one token row: codes and scales of K and V of every KV head."""
+        if self.code == _lib.HS_DTYPE_E2M1:
+            return 2 * self.kv_heads * (self.head_dim // 2 + self.head_dim // FP4_GROUP)
         return 2 * self.kv_heads * (self.head_dim + 4)
 
 
@@ -89,7 +110,7 @@ def append_quantized(k, v, rows, pool):
 
 def read_quantized(pool, rows, dtype=torch.bfloat16, out=None):
     """K and V [n, Hkv, D] in ``dtype`` of the physical rows ``rows`` (int64 [n], device):
-    code * scale, rounded once.  A row outside the pool (-1) gives zeros.  ``out``: a (k, v)
+    code * scale, rounded once (exact from 4 bits, but where the dtype cannot hold it).  A row outside the pool (-1) gives zeros.  ``out``: a (k, v)
     pair to write instead."""
     code = _lib.dtype_code(dtype)
     _check_rows(rows, pool, "read_quantized")

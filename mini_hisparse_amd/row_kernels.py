@@ -272,7 +272,7 @@ def attend_window(query, pool, slots, lengths, mask, config):
     return m, l, acc
 
 
-def attend_pages(query, pool, tables, lengths, *, out=None):
+def attend_pages(query, pool, tables, lengths, *, window=None, sinks=0, out=None):
     """Attention of one new token per request over page tables (hs_attend_pages).
 
     query [B, Hq, D]; ``pool`` a plain pool [blocks, 2, P, Hkv, D] in the query dtype, or a
@@ -285,9 +285,14 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
     (``out`` when given); zeros for a request without a token.  The launch is chosen from the
     tables' width: one no wider than the histories need is faster for short ones.
 
+    ``window``: of a request of n tokens only the newest ``window`` (t >= n - window) and the
+    first ``sinks`` (t < sinks) count.  The others' rows are not used, whatever their pages
+    hold or whether they are there, and whole tiles of them are not read: the launch is
+    chosen, and takes the time, of histories of about ``window + sinks`` tokens.
+
     Scores, softmax statistics and sums are float32.  Where the matrix cores run (head dims
     32, 64, 96, 128 and, but for float32 pools, 256) a weight enters the product with V to
-    2^-16 of itself (float16 pools 2^-22 and 2^-45 of the largest weight, 8-bit pools with a
+    2^-16 of itself (float16 pools 2^-22 and 2^-45 of the largest weight, 8- and 4-bit pools with a
     float32 query 2^-24, float32 pools in full).  A NaN in a used row, or a score of +inf, makes
     its heads' outputs NaN; a token whose score is -inf has no weight, and if no other is left
     the output is zeros.
@@ -299,6 +304,8 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
         raise ValueError("attend_pages takes query [B, Hq, D] and a pool [blocks, 2, page_size, kv_heads, head_dim]")
     batch, heads, dim = shape
     blocks, _, page_size, kv_heads, head_dim = s_shape
+    if quantized:
+        head_dim = pool.head_dim
     if dim != head_dim or heads % kv_heads or dim > 512:
         raise ValueError("query and pool differ in head_dim (at most 512), or query heads are no multiple of KV heads")
     code = _lib.dtype_code(query.dtype)
@@ -322,6 +329,16 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
     if out is not None and (out.shape != shape or out.dtype != query.dtype or out.device != device
                             or not out.is_contiguous()):
         raise ValueError("attend_pages: out must be contiguous, of the query's shape, dtype and device")
+    if window is None:
+        if sinks:
+            raise ValueError("attend_pages: first tokens that stay (sinks) go with a window")
+        seen = 0
+    else:
+        seen = window
+        if window < 1 or sinks < 0:
+            raise ValueError("attend_pages: a window holds at least one token, and sinks are not negative")
+        if window >= 2**63 or sinks >= 2**63:
+            raise ValueError("attend_pages: window and sinks are counts of tokens below 2^63")
     if device.type != "cuda":
         raise ValueError("attend_pages needs ROCm device tensors (HIP kernels only)")
     q_stride = query.stride()
@@ -329,21 +346,21 @@ def attend_pages(query, pool, tables, lengths, *, out=None):
         query = query.contiguous()
         q_stride = query.stride()
     result = query.new_empty(shape) if out is None else out
-    nbytes = _pages_workspace_bytes(code, pool_code, batch, heads, kv_heads, dim, page_size, pages)
+    nbytes = _pages_workspace_bytes(code, pool_code, batch, heads, kv_heads, dim, page_size, pages, seen, sinks)
     with _lib.on_device(device):
         # a workspace of this call's own: calls on other streams and captured graphs share none
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        status = _lib.load().hs_attend_pages(
+        status = _lib.load().hs_attend_pages_window(
             query.data_ptr(), q_stride[0], q_stride[1], code, store.data_ptr(), scales, pool_code, blocks, page_size,
             kv_heads, dim, tables.data_ptr(), t_stride[0], t_stride[1] if per_head else 0, pages, lengths.data_ptr(),
-            batch, heads, result.data_ptr(), heads * dim, dim, workspace.data_ptr() if nbytes else None, nbytes,
+            batch, heads, seen, sinks, result.data_ptr(), heads * dim, dim, workspace.data_ptr() if nbytes else None, nbytes,
             _lib.stream_handle(device),
         )
     if status:
-        _lib.check(status, "hs_attend_pages")
+        _lib.check(status, "hs_attend_pages_window")
     return result
 
 
 @functools.lru_cache(maxsize=1024)
 def _pages_workspace_bytes(*sizes):
-    return _lib.load().hs_attend_pages_workspace_bytes(*sizes)
+    return _lib.load().hs_attend_pages_window_workspace_bytes(*sizes)
