@@ -496,6 +496,19 @@ int hs_read_quantized(const void* codes, const void* scales, int32_t code, int64
                       int32_t dtype, hs_stream_t stream);
 
 /*
+ * hs_norm_rotary_split with K and V written to a paged pool on the way: q [rows, heads, head_dim] comes
+ * out, row i's K (normed and rotated as q is) and V go to physical row to_rows[i] (int64 on the
+ * device; a row outside [0, pool_rows) is skipped, the others of one call must differ).  pool and
+ * scales as for hs_append_quantized, or a plain pool [blocks, 2, P, Hkv, D] of `dtype` (pool_code
+ * dtype, scales null).  Quantised rows are those of the fp32 values.  q_weight and k_weight both
+ * null: no norm.  rows may be 0; head_dim at most 512, even, for HS_DTYPE_E2M1 a multiple of 32.
+ */
+int hs_norm_rotary_append(const void* qkv, int64_t qkv_stride, const void* q_weight, const void* k_weight, float eps,
+                          void* q, const int64_t* positions, const int64_t* to_rows, int64_t rows, int64_t heads,
+                          double theta, int32_t dtype, void* pool, void* scales, int32_t pool_code, int64_t pool_rows,
+                          int64_t page_size, int64_t kv_heads, int64_t head_dim, hs_stream_t stream);
+
+/*
  * Diagnostic (no reference counterpart): read, without computing, n segment
  * pairs of a device region -- segment i at byte offset offsets[i] (device
  * array) and its partner plane_bytes further, segment_bytes each -- with

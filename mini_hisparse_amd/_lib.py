@@ -136,6 +136,11 @@ SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
          c_int64, c_int64, c_double, c_int32, c_void_p],
     ),
+    "hs_norm_rotary_append": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_double,
+         c_int32, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_void_p],
+    ),
     "hs_append_quantized": (
         c_int,
         [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p,

@@ -23,10 +23,10 @@
 #include <math.h>
 
 #include "hs_common.h"
+#include "norm_rotary.h"
 
 namespace hs {
 
-constexpr int DN_T = 256;
 
 // One workgroup per row.  `delta` may be null (no residual add); `x_out` may
 // alias `x`.  A row of at most NR_REG * DN_T elements is held in registers: every
@@ -172,175 +172,6 @@ __global__ __launch_bounds__(DN_T) void rotary_split_kernel(const void* qkv, int
   }
 }
 
-// Per-head RMS norm of q and k, then the rotary embedding, with the split of a packed
-// q|k|v row: for a q or k head vector x with norm weight w,
-//
-//   n_d = x_d rsqrt(mean(x^2) + eps) w_d,
-//   (y_i, y_{i+D/2}) = (n_i cos a - n_{i+D/2} sin a, n_{i+D/2} cos a + n_i sin a),
-//   a = position * theta^(-2i/D),
-//
-// in fp32, rounded once.  The angle is reduced to a part of one turn in 64 bits: at
-// position 10^5 an fp32 angle is off by up to 4e-3, more than a bf16 step of the result.
-// A head vector is held by `lanes` lanes of NE pairs each, so both halves of a pair meet in
-// one lane and the norm's sum is a butterfly within the lanes.  A workgroup takes `brows` rows:
-// its threads first fill the rows' cos/sin table in LDS (one 64-bit reduction per row and pair,
-// shared by all heads), then walk the rows' heads, the next head's loads in flight.
-// Bound by its bytes: 16384 rows of 28 query and 2 x 4 KV heads of 128 in bf16 move 302 MB in
-// 58 us, 5.2 TB/s, where a copy of 256 MiB runs at 5.35.  A decode batch is bound by its chain of
-// loads, table and stores: 16 rows of these heads take 3.9 us, one row of 14 and 2 x 2 heads of
-// 64 takes 2.8.
-constexpr int NH_TAB = 512;  // cos/sin pairs of a workgroup's table
-
-struct NormRotaryArgs {
-  const void *qkv, *wq, *wk;
-  void *q, *k, *v;
-  const int64_t* positions;
-  int64_t qkv_stride, rows, heads, kv_heads;
-  double log2_theta;
-  float eps;
-  int D, lanes_log2, brows;
-};
-
-// Elements of half a head vector that a lane holds, as loaded: NE neighbours (VEC), or one of
-// every `lanes` (then as floats).
-template <int DT, int NE, bool VEC>
-struct HalfVector {
-  static constexpr int WORDS = VEC && DT != HS_DTYPE_F32 ? NE / 2 : NE;
-  uint32_t w[WORDS];
-
-  __device__ __forceinline__ void load(const void* base, int64_t at, int lane, int lanes, int half) {
-    if constexpr (VEC) {
-      const char* p = static_cast<const char*>(base) + (at + (lane * NE < half ? lane * NE : 0)) * (DT == HS_DTYPE_F32 ? 4 : 2);
-      if constexpr (WORDS == 4) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = v[i];
-      } else {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(p);
-        w[0] = v[0];
-        w[1] = v[1];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const int i = lane + lanes * e;
-        w[e] = __float_as_uint(i < half ? load_elem<DT>(base, at + i) : 0.f);
-      }
-    }
-  }
-  __device__ __forceinline__ void store(void* base, int64_t at, int lane, int lanes, int half) const {
-    if constexpr (VEC) {
-      if (lane * NE >= half) return;
-      char* p = static_cast<char*>(base) + (at + lane * NE) * (DT == HS_DTYPE_F32 ? 4 : 2);
-      if constexpr (WORDS == 4) *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
-      else *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
-    } else {
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const int i = lane + lanes * e;
-        if (i < half) store_elem<DT>(base, at + i, __uint_as_float(w[e]));
-      }
-    }
-  }
-  __device__ __forceinline__ void floats(float (&x)[NE], bool in) const {  // zeros past the vector's end
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      if constexpr (WORDS == NE) {
-        x[e] = __uint_as_float(w[e]);
-      } else {
-        const unsigned short b = static_cast<unsigned short>(w[e >> 1] >> (16 * (e & 1)));
-        x[e] = DT == HS_DTYPE_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
-      }
-      if constexpr (VEC) x[e] = in ? x[e] : 0.f;
-    }
-  }
-  __device__ __forceinline__ void round_from(const float (&x)[NE]) {
-#pragma unroll
-    for (int e = 0; e < WORDS; ++e) {
-      if constexpr (WORDS == NE) w[e] = __float_as_uint(x[e]);
-      else w[e] = pack16<DT == HS_DTYPE_F16>(x[2 * e], x[2 * e + 1]);
-    }
-  }
-};
-
-template <int DT, int NE, bool VEC>
-__global__ __launch_bounds__(DN_T) void norm_rotary_split_kernel(NormRotaryArgs a) {
-  using Half = HalfVector<DT, NE, VEC>;
-  __shared__ __attribute__((aligned(16))) float s_cos[NH_TAB], s_sin[NH_TAB];
-  const int half = a.D / 2, lanes = 1 << a.lanes_log2;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.brows;
-  const int nrows = static_cast<int>(a.rows - row0 < a.brows ? a.rows - row0 : a.brows);
-  const int H = static_cast<int>(a.heads), K = static_cast<int>(a.kv_heads), total = H + 2 * K;
-  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> a.lanes_log2, groups = DN_T >> a.lanes_log2;
-  const bool in = !VEC || lane * NE < half;
-  // this group's heads: h = first, first + step, ... of every row in turn; the next head's loads
-  // go out before the current one is worked on
-  const int step = static_cast<int>(gridDim.y) * groups;
-  int r = 0, h = static_cast<int>(blockIdx.y) * groups + group;
-  auto settle = [&]() {
-    while (h >= total && r < nrows) {
-      h -= total;
-      ++r;
-    }
-  };
-  Half lo, hi, wq[2], wk[2];
-  auto fetch = [&](Half& x, Half& y) {
-    const int64_t src = (row0 + r) * a.qkv_stride + static_cast<int64_t>(h) * a.D;
-    x.load(a.qkv, src, lane, lanes, half);
-    y.load(a.qkv, src + half, lane, lanes, half);
-  };
-  settle();
-  if (r < nrows) fetch(lo, hi);
-  for (int i = 0; i < 2; ++i) {
-    wq[i].load(a.wq, i * half, lane, lanes, half);
-    wk[i].load(a.wk, i * half, lane, lanes, half);
-  }
-  for (int t = threadIdx.x; t < nrows * half; t += DN_T) {
-    const int tr = t / half, i = t - tr * half;
-    // turns = position * theta^(-2i/D) / 2 pi
-    const double turns = static_cast<double>(a.positions[row0 + tr]) *
-                         (exp2(-(2.0 * i / a.D) * a.log2_theta) * 0.15915494309189535);
-    float s, c;
-    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
-    s_cos[t] = c;
-    s_sin[t] = s;
-  }
-  __syncthreads();
-  while (r < nrows) {
-    const int cr = r, ch = h;
-    Half cur[2] = {lo, hi};
-    h += step;
-    settle();
-    if (r < nrows) fetch(lo, hi);
-    const int64_t row = row0 + cr;
-    void* dst = ch < H ? a.q : (ch < H + K ? a.k : a.v);
-    const int64_t to = (ch < H ? row * H + ch : (ch < H + K ? row * K + ch - H : row * K + ch - H - K)) * a.D;
-    if (ch < H + K) {  // one condition for all lanes of the head
-      float x[NE], y[NE], u[NE], v[NE], sq = 0.f;
-      cur[0].floats(x, in);
-      cur[1].floats(y, in);
-#pragma unroll
-      for (int e = 0; e < NE; ++e) sq += x[e] * x[e] + y[e] * y[e];
-      sq = group_reduce(sq, lanes, [](float p, float q) { return p + q; });
-      const float norm = rsqrtf(sq / static_cast<float>(a.D) + a.eps);
-      (ch < H ? wq[0] : wk[0]).floats(u, in);
-      (ch < H ? wq[1] : wk[1]).floats(v, in);
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const int i = VEC ? lane * NE + e : lane + lanes * e;
-        const int at = i < half ? cr * half + i : 0;
-        const float p = x[e] * norm * u[e], q = y[e] * norm * v[e], c = s_cos[at], s = s_sin[at];
-        x[e] = p * c - q * s;
-        y[e] = q * c + p * s;
-      }
-      cur[0].round_from(x);
-      cur[1].round_from(y);
-    }
-    cur[0].store(dst, to, lane, lanes, half);
-    cur[1].store(dst, to + half, lane, lanes, half);
-  }
-}
-
 // out[row, j] = silu(gate[row, j]) * up[row, j] with gate = gate_up[row, :width],
 // up = gate_up[row, width:].
 template <int DT>
@@ -405,34 +236,14 @@ extern "C" int hs_norm_rotary_split(const void* qkv, int64_t qkv_stride, const v
   HS_CHECK_ARG(qkv_stride >= (heads + 2 * kv_heads) * head_dim, "q|k|v row stride below its width");
   HS_CHECK_ARG(qkv && q_weight && k_weight && q && k && v && positions, "null normed rotary pointer");
   HS_CHECK_ARG(theta > 0.0 && isfinite(theta) && eps >= 0.f, "theta must be positive and eps not negative");
-  const int half = static_cast<int>(head_dim / 2);
   const uintptr_t all = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_weight) |
                         reinterpret_cast<uintptr_t>(k_weight) | reinterpret_cast<uintptr_t>(q) |
                         reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
-  // pairs of a lane: a load of 16 bytes where the head dim and the addresses allow it, else of 8
-  // (16-bit types), else element by element over a whole wave
-  int ne = 0;
-  for (const int n : {16 / elem_bytes(dtype), 4})
-    if (ne == 0 && half % n == 0 && qkv_stride % n == 0 && all % (n * elem_bytes(dtype)) == 0) ne = n;
+  const int ne = norm_rotary_pairs(dtype, head_dim / 2, qkv_stride, all, 0, 0);
   NormRotaryArgs a{qkv, q_weight, k_weight, q, k, v, positions, qkv_stride, rows, heads, kv_heads, log2(theta), eps,
                    static_cast<int>(head_dim), 6, 1};
-  if (ne) {
-    a.lanes_log2 = 0;
-    while ((ne << a.lanes_log2) < half) ++a.lanes_log2;
-  }
-  const int64_t groups = DN_T >> a.lanes_log2, total = heads + 2 * kv_heads;
-  // Rows per workgroup: as many as give every thread one cos/sin pair, once that still
-  // leaves two workgroups per CU; fewer rows go one to a workgroup, their heads spread.
-  const int64_t fill = DN_T / half > 1 ? DN_T / half : 1;
-  a.brows = rows >= 512 * fill ? static_cast<int>(fill) : 1;
-  int64_t spread = 1;
-  if (rows < 512) {
-    spread = (total + groups - 1) / groups;
-    const int64_t most = (512 + rows - 1) / rows;
-    if (spread > most) spread = most;
-  }
-  HS_CHECK_ARG((rows + a.brows - 1) / a.brows < (int64_t{1} << 32) / DN_T, "too many rows in one call");
-  const dim3 grid(static_cast<unsigned>((rows + a.brows - 1) / a.brows), static_cast<unsigned>(spread));
+  const dim3 grid = norm_rotary_grid(a, ne);
+  HS_CHECK_ARG(grid.x < (int64_t{1} << 32) / DN_T, "too many rows in one call");
 #define HS_NORM_ROTARY(DT, NE, VEC) \
   hipLaunchKernelGGL((norm_rotary_split_kernel<DT, NE, VEC>), grid, dim3(DN_T), 0, stream, a)
   if (dtype == HS_DTYPE_F32) {

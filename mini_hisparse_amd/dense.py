@@ -10,7 +10,8 @@ RMSNorm (with the residual add before it), the rotary embedding of q and k
 implements (model.py:53-57 RMSNorm, the rotary and MLP of this package's
 ``model.py``; the reference's model.py:183-226).  One launch each for B rows.
 ``norm_rotary_split`` (``hs_norm_rotary_split``) is ``rotary_split`` with a per-head
-RMSNorm of q and k before the rotation.
+RMSNorm of q and k before the rotation, ``norm_rotary_append`` (``hs_norm_rotary_append``)
+the same with K and V written to a paged pool on the way.
 """
 
 from __future__ import annotations
@@ -18,6 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .quantized import QuantizedPool
 
 
 def _stream(tensor):
@@ -390,6 +392,79 @@ def prepare_norm_rotary_split(qkv, q_weight, k_weight, eps, positions, heads, kv
     return Launch(_lib.load().hs_norm_rotary_split,
                   _norm_rotary_args(qkv, q_weight, k_weight, eps, positions, heads, kv_heads, head_dim, theta, *out),
                   "hs_norm_rotary_split")
+
+
+def _norm_rotary_append_check(qkv, q_weight, k_weight, positions, rows, pool, heads, out):
+    """The pool's (code, scales or None, rows, page size, KV heads, head dim)."""
+    shape, stride, dtype, device = qkv.shape, qkv.stride(), qkv.dtype, qkv.device
+    code = _lib.dtype_code(dtype)
+    if isinstance(pool, QuantizedPool):
+        held = (pool.codes, pool.scales, pool.code, pool.rows, pool.page_size, pool.kv_heads, pool.head_dim)
+    elif pool.dim() != 5 or pool.shape[1] != 2 or 0 in pool.shape or pool.dtype != dtype or not pool.is_contiguous():
+        raise ValueError("norm_rotary_append: a plain pool must be contiguous [blocks, 2, page_size, kv_heads, "
+                         "head_dim] in the dtype of qkv")
+    else:
+        held = (pool, None, code, pool.shape[0] * pool.shape[2], *pool.shape[2:])
+    kv_heads, head_dim = held[5:]
+    if heads < 1 or head_dim % 2 or head_dim > 512:
+        raise ValueError("norm_rotary_append takes query heads and a pool of an even head_dim of at most 512")
+    if len(shape) != 2 or shape[1] != (heads + 2 * kv_heads) * head_dim or stride[1] != 1 \
+            or stride[0] < shape[1] and shape[0] > 1:
+        raise ValueError("qkv must be [rows, (heads + 2 kv_heads) head_dim] with unit inner stride, its rows apart")
+    for name, x in (("positions", positions), ("rows", rows)):
+        if x.dtype != torch.int64 or x.shape != shape[:1] or x.device != device or not x.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int64 [rows] on the device of qkv")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("norm_rotary_append takes both norm weights or none")
+    for name, x in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if x is not None and (x.shape != (head_dim,) or x.dtype != dtype or x.device != device or not x.is_contiguous()):
+            raise ValueError(f"{name} must be [head_dim] contiguous in the dtype and on the device of qkv")
+    if held[0].device != device:
+        raise ValueError("norm_rotary_append: the pool must be on the device of qkv")
+    _check_out(out, (shape[0], heads, head_dim), qkv, "norm_rotary_append")
+    if device.type != "cuda":
+        raise ValueError("norm_rotary_append needs ROCm device tensors (HIP kernels only)")
+    return held
+
+
+def _norm_rotary_append_args(qkv, q_weight, k_weight, eps, positions, rows, heads, theta, held, q):
+    store, scales, code, pool_rows, page_size, kv_heads, head_dim = held
+    count, width = qkv.shape
+    stride = qkv.stride(0)
+    return (qkv.data_ptr(), stride if stride > width else width, _lib.ptr(q_weight), _lib.ptr(k_weight), eps,
+            q.data_ptr(), positions.data_ptr(), rows.data_ptr(), count, heads, theta, _lib.dtype_code(qkv.dtype),
+            store.data_ptr(), _lib.ptr(scales), code, pool_rows, page_size, kv_heads, head_dim)
+
+
+def norm_rotary_append(qkv, q_weight, k_weight, eps, positions, rows, pool, heads, theta, out=None):
+    """:func:`norm_rotary_split` with K and V written to a paged pool on the way: returns q
+    [rows, heads, head_dim]; token i's K and V go to physical row ``rows[i]`` (int64, device;
+    one outside the pool, -1, is skipped; the others must differ).  ``pool``: a plain pool
+    [blocks, 2, P, Hkv, D] in the dtype of ``qkv`` or a
+    :class:`~mini_hisparse_amd.quantized.QuantizedPool`, which names the KV heads and the head
+    dim; quantised rows are those of the float32 values, which are rounded once.
+    ``q_weight`` and ``k_weight`` None: heads are rotated without a norm (``eps`` is unused)."""
+    held = _norm_rotary_append_check(qkv, q_weight, k_weight, positions, rows, pool, heads, out)
+    device = qkv.device
+    q = qkv.new_empty((qkv.shape[0], heads, held[6])) if out is None else out
+    with _lib.on_device(device):
+        status = _lib.load().hs_norm_rotary_append(
+            *_norm_rotary_append_args(qkv, q_weight, k_weight, eps, positions, rows, heads, theta, held, q),
+            _lib.stream_handle(device))
+    if status:
+        _lib.check(status, "hs_norm_rotary_append")
+    return q
+
+
+def prepare_norm_rotary_append(qkv, q_weight, k_weight, eps, positions, rows, pool, heads, theta, out):
+    """:func:`norm_rotary_append` into ``out``, bound once (``positions`` and ``rows`` are read
+    when the launch runs)."""
+    held = _norm_rotary_append_check(qkv, q_weight, k_weight, positions, rows, pool, heads, out)
+    if out is None:
+        raise ValueError("prepare_norm_rotary_append writes into a given out")
+    return Launch(_lib.load().hs_norm_rotary_append,
+                  _norm_rotary_append_args(qkv, q_weight, k_weight, eps, positions, rows, heads, theta, held, out),
+                  "hs_norm_rotary_append")
 
 
 def _silu_check(gate_up, out):
