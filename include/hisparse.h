@@ -629,6 +629,21 @@ int hs_skinny_gemm_argmax_tiled(const void* x, int64_t x_stride, const void* wei
                                 const void* bias, int64_t* tokens, int64_t rows, int32_t dtype, void* workspace,
                                 int64_t workspace_bytes, hs_stream_t stream);
 
+/*
+ * The projection with 4-bit weights: W[n, k] = code * 2^(e - 127), e2m1 codes with a scale byte e for
+ * every 32 neighbours of a row (HS_DTYPE_E2M1), for 1 <= rows <= 16, x and out bf16 or f16, fp32
+ * sums rounded once (with the bias).  weight_tiles: ceil(n/16) * ceil(k/128) blocks of 1 KB, block
+ * (t, s) at t * ceil(k/128) + s: 64 runs of 16 bytes, run 16 j + c the 32 codes of row 16t + c from
+ * k = 128s + 32j on (the even one in the low half of a byte).  weight_scales: for each t and each
+ * four blocks, 64 dwords, dword 16 j + c the scale bytes of that run in those four blocks, the
+ * first lowest.  Rows past n, k past the last and blocks past ceil(k/128) are zero bytes.  k a
+ * multiple of 32 below 2^30; x rows and weight_tiles 16-byte aligned.  No workspace; a row's sums
+ * do not depend on the other token rows.  No reference counterpart.
+ */
+int hs_skinny_gemm_fp4(const void* x, int64_t x_stride, const void* weight_tiles, const void* weight_scales, int64_t n,
+                       int64_t k, const void* bias, void* out, int64_t out_stride, int64_t rows, int32_t dtype,
+                       hs_stream_t stream);
+
 #pragma GCC visibility pop
 
 #ifdef __cplusplus

@@ -187,6 +187,10 @@ SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p,
          c_int64, c_void_p],
     ),
+    "hs_skinny_gemm_fp4": (
+        c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32,
+                c_void_p],
+    ),
     "hs_skinny_gemm_argmax_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
     "hs_skinny_gemm_argmax_tiled": (
         c_int,

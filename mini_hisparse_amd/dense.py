@@ -1,7 +1,8 @@
 """Dense stages of a decoder layer's decode step (HIP kernels).
 
 ``linear`` wraps ``hs_skinny_gemm``, the projection of up to 16 token rows
-(an HBM stream of the weight on MFMA tiles).  ``add_rms_norm``,
+(an HBM stream of the weight on MFMA tiles), ``linear_quantized``
+``hs_skinny_gemm_fp4``, the same with a weight in 4 bits.  ``add_rms_norm``,
 ``rotary_split`` and ``silu_mul`` wrap ``hs_add_rms_norm``,
 ``hs_rotary_split`` and ``hs_silu_mul``: the
 RMSNorm (with the residual add before it), the rotary embedding of q and k
@@ -16,10 +17,12 @@ the same with K and V written to a paged pool on the way.
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from . import _lib
-from .quantized import QuantizedPool
+from .quantized import FP4_GROUP, QuantizedPool
 
 
 def _stream(tensor):
@@ -169,6 +172,125 @@ def prepare_linear_tiled(x, tiles, n, bias, out, workspace):
         raise ValueError("prepare_linear_tiled writes into a given out")
     ws = _workspace(x.device, None, gemm_workspace_bytes(x.shape[0], n, x.shape[1]), workspace)
     return _linear_tiled_launch(x, tiles, n, bias, out, ws)
+
+
+@dataclass(frozen=True, eq=False)
+class QuantizedWeight:
+    """A projection's weight [n, k] in 4 bits, laid out for :func:`linear_quantized`: e2m1 codes
+    (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) with a power of two for every 32 neighbours of a row,
+    4.25 bits a weight.  From :func:`quantize_weight`, or :meth:`pack` of codes and scales that
+    exist already."""
+
+    tiles: torch.Tensor  # uint8 [ceil(n / 16), ceil(k / 128), 64, 16]
+    scales: torch.Tensor  # uint8 [ceil(n / 16), ceil(k / 512), 64, 4]
+    n: int
+    k: int
+
+    def __post_init__(self):
+        steps = -(-self.k // 128)
+        tall = -(-self.n // 16)
+        if self.n < 1 or self.k < 1 or self.k % FP4_GROUP:
+            raise ValueError("a 4-bit weight has n rows of k, a multiple of 32")
+        for x, shape in ((self.tiles, (tall, steps, 64, 16)), (self.scales, (tall, -(-steps // 4), 64, 4))):
+            if x.dtype != torch.uint8 or x.shape != shape or not x.is_contiguous():
+                raise ValueError(f"a 4-bit weight of {self.n} x {self.k} needs contiguous uint8 {shape}")
+        if self.tiles.device != self.scales.device:
+            raise ValueError("codes and scales must be on one device")
+
+    @classmethod
+    def pack(cls, codes, scales):
+        """``codes`` [n, k / 2] (float4_e2m1fn_x2 or its bytes: two a byte, the even one in the low
+        half) with ``scales`` [n, k / 32] (float8_e8m0fnu or its bytes) in the kernel's layout."""
+        if codes.dtype == torch.float4_e2m1fn_x2:
+            codes = codes.view(torch.uint8)
+        if scales.dtype == torch.float8_e8m0fnu:
+            scales = scales.view(torch.uint8)
+        if codes.dtype != torch.uint8 or codes.dim() != 2 or 0 in codes.shape or codes.shape[1] % (FP4_GROUP // 2):
+            raise ValueError("codes must be float4_e2m1fn_x2 or uint8 [n, k / 2], k a multiple of 32")
+        n, k = codes.shape[0], 2 * codes.shape[1]
+        if scales.dtype != torch.uint8 or scales.shape != (n, k // FP4_GROUP):
+            raise ValueError("scales must be float8_e8m0fnu or uint8 [n, k / 32]")
+        if scales.device != codes.device:
+            raise ValueError("codes and scales must be on one device")
+        tall, steps = -(-n // 16), -(-k // 128)
+        groups = -(-steps // 4)
+        pad = torch.nn.functional.pad
+        tiles = pad(codes, (0, 64 * steps - k // 2, 0, 16 * tall - n)).view(tall, 16, steps, 4, 16)
+        bytes_ = pad(scales, (0, 16 * groups - k // FP4_GROUP, 0, 16 * tall - n)).view(tall, 16, groups, 4, 4)
+        return cls(tiles.permute(0, 2, 3, 1, 4).reshape(tall, steps, 64, 16).contiguous(),
+                   bytes_.permute(0, 2, 4, 1, 3).reshape(tall, groups, 64, 4).contiguous(), n, k)
+
+
+def quantize_weight(weight):
+    """``weight`` [n, k] (float32, float16 or bfloat16; k a multiple of 32) in 4 bits, as
+    ``quantized.append_quantized`` rounds: per 32 neighbours the smallest power of two, from
+    2^-126 on, that takes the largest magnitude to at most 7, and the nearest codes, ties to
+    even, at most 6."""
+    _lib.dtype_code(weight.dtype)
+    if weight.dim() != 2 or 0 in weight.shape or weight.shape[1] % FP4_GROUP:
+        raise ValueError("quantize_weight takes [n, k], k a multiple of 32")
+    n, k = weight.shape
+    codes = torch.empty((n, k // 2), dtype=torch.uint8, device=weight.device)
+    scales = torch.empty((n, k // FP4_GROUP), dtype=torch.uint8, device=weight.device)
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], device=weight.device)
+    step = max(1, (1 << 26) // k)
+    for i in range(0, n, step):
+        x = weight[i : i + step].float().unflatten(1, (-1, FP4_GROUP))
+        top = x.abs().amax(-1)
+        finite = top.isfinite()
+        part, power = torch.frexp(torch.where(finite, top, 0.0))
+        power = torch.where(top > 0, power - 3 + (part > 0.875).int(), -126).clamp(min=-126)
+        x = torch.where(finite[..., None], torch.ldexp(x, -power[..., None]), 0.0)
+        # a border's own value goes to the even of the two codes beside it
+        low, high = (torch.bucketize(x.abs(), borders, right=r) for r in (False, True))
+        code = (torch.where(low % 2 == 0, low, high) | x.signbit().int() << 3).flatten(1).to(torch.uint8)
+        codes[i : i + step] = code[:, 0::2] | code[:, 1::2] << 4
+        scales[i : i + step] = torch.where(finite, power + 127, 255).to(torch.uint8)
+    return QuantizedWeight.pack(codes, scales)
+
+
+def _linear_quantized_check(x, weight, bias, out):
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if len(shape) != 2 or not 1 <= shape[0] <= 16 or shape[1] != weight.k \
+            or dtype not in (torch.bfloat16, torch.float16) or x.stride(1) != 1 and shape[1] > 1 \
+            or shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < shape[1]) or x.data_ptr() % 16:
+        raise ValueError("linear_quantized takes 1-16 rows of a bf16/f16 x [rows, k], rows 16-byte aligned")
+    if bias is not None and (bias.shape != (weight.n,) or bias.dtype != dtype or not bias.is_contiguous()
+                             or bias.device != device):
+        raise ValueError("bias must be [n] contiguous in the dtype and on the device of x")
+    if weight.tiles.device != device:
+        raise ValueError("linear_quantized: x and the weight must be on one device")
+    _check_out(out, (shape[0], weight.n), x, "linear_quantized")
+    if device.type != "cuda":
+        raise ValueError("linear_quantized needs ROCm device tensors (HIP kernels only)")
+
+
+def _linear_quantized_args(x, weight, bias, y):
+    rows, k = x.shape
+    return (x.data_ptr(), x.stride(0) if rows > 1 else k, weight.tiles.data_ptr(), weight.scales.data_ptr(), weight.n, k,
+            _lib.ptr(bias), y.data_ptr(), y.stride(0) if rows > 1 else weight.n, rows, _lib.dtype_code(x.dtype))
+
+
+def linear_quantized(x, weight, bias=None, out=None):
+    """``x @ W.T + bias`` for ``x`` [rows <= 16, k] and a :class:`QuantizedWeight`.  The weights
+    are taken exactly, sums are float32 and rounded once with the bias; a row's result does not
+    depend on the other rows.  No workspace, one launch."""
+    _linear_quantized_check(x, weight, bias, out)
+    y = x.new_empty((x.shape[0], weight.n)) if out is None else out
+    device = x.device
+    with _lib.on_device(device):
+        status = _lib.load().hs_skinny_gemm_fp4(*_linear_quantized_args(x, weight, bias, y), _lib.stream_handle(device))
+    if status:
+        _lib.check(status, "hs_skinny_gemm_fp4")
+    return y
+
+
+def prepare_linear_quantized(x, weight, bias, out):
+    """:func:`linear_quantized` into ``out``, bound once."""
+    _linear_quantized_check(x, weight, bias, out)
+    if out is None:
+        raise ValueError("prepare_linear_quantized writes into a given out")
+    return Launch(_lib.load().hs_skinny_gemm_fp4, _linear_quantized_args(x, weight, bias, out), "hs_skinny_gemm_fp4")
 
 
 def argmax_workspace_bytes(rows, n, k):

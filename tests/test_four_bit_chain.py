@@ -1,19 +1,21 @@
-"""The operators of a decode step in 4 bits as they are used together: normed rotary embedding into a
-4-bit cache, attention over it whole and through a window; eager, and captured once and replayed."""
+"""The operators of a decode step in 4 bits as they are used together: 4-bit projections, normed rotary
+embedding into a 4-bit cache, attention over it whole and through a window; eager, and captured
+once and replayed."""
 
 import pytest
 import torch
 
-from mini_hisparse_amd.dense import norm_rotary_append
+from mini_hisparse_amd.dense import linear_quantized, norm_rotary_append, quantize_weight
 from mini_hisparse_amd.quantized import QuantizedPool
 from mini_hisparse_amd.row_kernels import attend_pages
 
 from page_cases import FP4, check as check_attention
+from test_linear_quantized import check as check_linear, unpack
 from test_norm_rotary import check as check_norm, formula as norm_formula
 from test_rotary_append import check_keys, planes
 
 HEADS, KV, DIM, PAGE, EPS, THETA = 14, 2, 64, 16, 1e-6, 1e6
-WINDOW, SINKS = 40, 4
+WINDOW, SINKS, HIDDEN = 40, 4, 288
 
 
 class Batch:
@@ -112,3 +114,50 @@ def test_captured_steps(gpu, prompts):
         for x, y in zip(planes(captured.pool), planes(eager.pool)):
             assert torch.equal(x, y)
     assert not torch.equal(planes(captured.pool)[0], kept[0])
+
+
+class Layer(Batch):
+    """A layer's attention with 4-bit projections around it."""
+
+    def __init__(self, prompts, room, dtype, device):
+        super().__init__(prompts, room, dtype, device)
+        draw = lambda *shape: (torch.randn(*shape, generator=self.gen) * shape[-1] ** -0.5).to(dtype).to(device)  # noqa: E731
+        self.into, self.out = (quantize_weight(draw(n, k)) for n, k in
+                               (((HEADS + 2 * KV) * DIM, HIDDEN), (HIDDEN, HEADS * DIM)))
+        self.bias = draw((HEADS + 2 * KV) * DIM)
+
+    def hidden(self, rows):
+        return torch.randn(rows, HIDDEN, generator=self.gen).to(self.dtype).to(self.device)
+
+    def decode(self, x):
+        qkv = linear_quantized(x, self.into, self.bias)
+        near = self.step(qkv)[-1]
+        return qkv, near, linear_quantized(near.flatten(1), self.out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_layer_with_its_projections(gpu, dtype):
+    """Each projection is its product's, and the captured layer follows the eager one."""
+    prompts = [200, 1, 33, 64]
+    eager, captured = (Layer(prompts, 30, dtype, gpu) for _ in range(2))
+    for layer in (eager, captured):
+        for b, n in enumerate(prompts):
+            layer.prefill(b, n)
+    x = captured.hidden(len(prompts))
+    eager.hidden(len(prompts))
+    lengths = captured.lengths.clone()
+    captured.decode(x)  # outside the graph first, its length undone
+    captured.lengths.copy_(lengths)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = captured.decode(x)[-1]
+    for _ in range(12):
+        fresh = captured.hidden(len(prompts))
+        assert torch.equal(fresh, eager.hidden(len(prompts)))
+        qkv, near, want = eager.decode(fresh)
+        check_linear(qkv, fresh, *unpack(eager.into), eager.bias)
+        check_linear(want, near.flatten(1), *unpack(eager.out), None)
+        x.copy_(fresh)
+        graph.replay()
+        assert torch.equal(y, want)
