@@ -184,16 +184,23 @@ static bool pages_mfma_shape(int64_t bits, int64_t Hkv, int64_t D) {
   return (D == 32 || D == 64 || D == 96 || D == 128 || (D == 256 && bits < 32)) && Hkv * D * bits < (int64_t{1} << 30);
 }
 
+// 4-bit pools whose KV heads share their tables go two KV heads a unit where the products' 16 columns
+// hold both's query heads.
+static bool pages_pair_shape(int pool_code, int64_t Hq, int64_t Hkv, int64_t D) {
+  return pool_code == HS_DTYPE_E2M1 && (D == 32 || D == 64 || D == 128) && Hkv % 2 == 0 && Hq / Hkv <= 8;
+}
+
 // `whole`: the general kernel takes a request in one split (the workspace was sized for a kernel
 // that needs none).  `most`: tokens that the tables can name.
-static PagesPlan plan_pages(bool mfma, bool whole, int64_t bits, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t most,
-                            int32_t window, int32_t sinks) {
+static PagesPlan plan_pages(bool mfma, bool pair, bool whole, int64_t bits, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                            int64_t most, int32_t window, int32_t sinks) {
   PagesPlan p{};
   const int64_t g = Hq / Hkv;
   p.mfma = mfma;
   if (mfma) {
+    p.pair = pair;
     p.head_chunks = static_cast<int>((g + 15) / 16);
-    p.units = static_cast<int>(Hkv * p.head_chunks);
+    p.units = static_cast<int>(pair ? Hkv / 2 : Hkv * p.head_chunks);
     const int64_t tiles = most_seen_tiles(most, window, sinks);
     // Short: as many parts of a request as give every CU a workgroup, 8 at most, of a tile for each
     // of its waves at least.  Taken while a wave has four tiles at most: us by this launch and by
@@ -205,9 +212,9 @@ static PagesPlan plan_pages(bool mfma, bool whole, int64_t bits, int64_t B, int6
     // 16 and 32 words: 12.9 16.2 and 12.6 12.6).
     // A unit of at most 128 KiB stays one part (14 query and 2 KV heads of 64 in int8, 64 requests
     // of 1024 tokens: 10.4 in one part, 12.7 in two).
-    const int64_t W = mfma_waves(D), rows = g < 16 ? g : 16;
+    const int64_t W = mfma_waves(D), rows = pair ? 2 * g : (g < 16 ? g : 16), held = pair ? 2 * D : D;
     int64_t parts = 256 / (B * p.units);
-    parts = parts < 1 || tiles * 2 * PM_TILE * D * bits <= 128 * 1024 * 8 ? 1 : (parts > PM_PARTS ? PM_PARTS : parts);
+    parts = parts < 1 || tiles * 2 * PM_TILE * held * bits <= 128 * 1024 * 8 ? 1 : (parts > PM_PARTS ? PM_PARTS : parts);
     p.min_tiles = (tiles + parts - 1) / parts;
     if (p.min_tiles < W) p.min_tiles = W;
     p.slots = (tiles + p.min_tiles - 1) / p.min_tiles;
@@ -292,14 +299,17 @@ extern "C" int64_t hs_attend_pages_window_workspace_bytes(int32_t query_dtype, i
   const int64_t bits = elem_bits(pool_code), tokens = pages * page_size;
   const int32_t newest = window_of(window), first = sinks_of(sinks);
   const bool shape = pages_mfma_shape(bits, kv_heads, head_dim);
-  auto need_of = [&](bool mfma, bool whole) {
-    return pages_workspace(plan_pages(mfma, whole, bits, batch, heads, kv_heads, head_dim, tokens, newest, first), batch,
-                           heads, head_dim);
+  auto need_of = [&](bool mfma, bool pair, bool whole) {
+    return pages_workspace(plan_pages(mfma, pair, whole, bits, batch, heads, kv_heads, head_dim, tokens, newest, first),
+                           batch, heads, head_dim);
   };
-  const int64_t need = need_of(shape, false);
+  int64_t need = need_of(shape, false, false);
   if (!shape) return need;
-  const int64_t other = need_of(false, need == 0);  // a pool that is not aligned goes to the general kernel
-  return need > other ? need : other;
+  // a pool that is not aligned goes to the general kernel, and only tables that KV heads share to pairs
+  const int64_t other = need_of(false, false, need == 0);
+  if (other > need) need = other;
+  const int64_t paired = pages_pair_shape(pool_code, heads, kv_heads, head_dim) ? need_of(true, true, false) : 0;
+  return paired > need ? paired : need;
 }
 
 extern "C" int64_t hs_attend_pages_workspace_bytes(int32_t query_dtype, int32_t pool_code, int64_t batch,
@@ -344,10 +354,11 @@ extern "C" int hs_attend_pages_window(const void* query, int64_t q_stride_b, int
   // (4-bit scales of 256 of the head dim are loaded eight at a time)
   const bool mfma = shape && reinterpret_cast<uintptr_t>(pool) % 16 == 0 &&
                     (pool_code != HS_DTYPE_E2M1 || reinterpret_cast<uintptr_t>(scales) % 8 == 0);
-  PagesPlan p = plan_pages(shape, false, bits, batch, heads, kv_heads, head_dim, tokens, newest, first);
+  const bool pair = mfma && t_stride_k == 0 && pages_pair_shape(pool_code, heads, kv_heads, head_dim);
+  PagesPlan p = plan_pages(shape, pair, false, bits, batch, heads, kv_heads, head_dim, tokens, newest, first);
   if (shape && !mfma)
-    p = plan_pages(false, pages_workspace(p, batch, heads, head_dim) == 0, bits, batch, heads, kv_heads, head_dim, tokens,
-                   newest, first);
+    p = plan_pages(false, false, pages_workspace(p, batch, heads, head_dim) == 0, bits, batch, heads, kv_heads, head_dim,
+                   tokens, newest, first);
   HS_CHECK_ARG((p.mfma ? p.target : p.splits) <= PJ_SLOTS, "page attention plan with too many parts of a request");
   const int64_t need = pages_workspace(p, batch, heads, head_dim);
   HS_CHECK_ARG(need == 0 || (workspace != nullptr && workspace_bytes >= need &&

@@ -521,13 +521,22 @@ __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& o
 // load together; a part alone writes the output, several are joined by the last to arrive.
 // Else the schedule of share_of over workgroups of up to four units (a page's rows are
 // contiguous over the KV heads), joined by pages_merge_kernel.
-template <int S, int QD, int D, bool UNIFORM, bool SHORT>
+// PAIR (4-bit pools, one table for all KV heads, at most 8 query heads a KV head): a unit is two
+// neighbouring KV heads, whose vectors are one of 2D, with the first one's query heads in columns 0 ..
+// 7 of the products and the second one's in 8 .. 15.  Scores are taken from either's product; of V's
+// the quarter in which rows and columns are of one head counts, half of the lanes' sums.  So a wave
+// reads whole lines of the cache (a head's row is 64 bytes at D = 128: two waves that each read one
+// half of a line take it from memory twice where they drift apart), and one exponential a lane
+// serves two heads.
+template <int S, int QD, int D, bool UNIFORM, bool SHORT, bool PAIR = false>
 __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArgs a) {
+  static_assert(!PAIR || (fp4(S) && D <= 128 && D != 96), "pairs of 4-bit head vectors of 32, 64 or 128");
+  constexpr int KVS = PAIR ? 2 : 1, DD = KVS * D;  // KV heads of a unit; their vectors' elements
   constexpr int W = mfma_waves(D), T = 64 * W;
   constexpr bool F16 = S == HS_DTYPE_F16, F32 = S == HS_DTYPE_F32;
   constexpr int BITS = elem_bits(S), VECTOR = D * BITS / 8;  // of an element; bytes of a head vector
   constexpr int KK = F32 ? D / 4 : D / 32;   // products over the head dim
-  constexpr int E = D / 16;                  // V elements of a lane and token
+  constexpr int E = DD / 16;                 // V elements of a lane and token
   constexpr int NQ = query_parts<S, QD>(), NP = weight_parts<S, QD>();
   constexpr int KROW = VECTOR / 4;           // K bytes of a lane and row
   constexpr int KL = KROW < 16 ? KROW & -KROW : (KROW % 16 ? 8 : 16);  // a K load
@@ -537,7 +546,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
   constexpr int VL = VB < 16 ? VB : 16;      // a V load
   constexpr int VB1 = (E - E0) * BITS / 8;   // bytes of the second part, from dim 16 E0
   constexpr int VW0 = VB < 4 ? 1 : VB / 4, VW = VW0 + (VB1 + 3) / 4;
-  constexpr int GS = D / FP4_GROUP;          // 4-bit pools: scales of a head vector
+  constexpr int GS1 = D / FP4_GROUP, GS = KVS * GS1;  // 4-bit pools: scales of a head vector, and of a unit's
   constexpr int SD = D + 4;                  // row stride of the waves' sums in LDS: no bank conflicts
   extern __shared__ __attribute__((aligned(16))) float smem[];
   __shared__ float s_m[W][16], s_l[W][16];
@@ -561,8 +570,8 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
   const int unit = SHORT ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * a.waves_units + wave % a.waves_units;
   const int sub = SHORT ? wave : wave / a.waves_units;
   const int subs = SHORT ? W : a.subs;
-  const int kv = unit / a.head_chunks, h0 = unit % a.head_chunks * 16;
-  const int heads = static_cast<int>(a.g - h0 < 16 ? a.g - h0 : 16);
+  const int kv = PAIR ? 2 * unit : unit / a.head_chunks, h0 = PAIR ? 0 : unit % a.head_chunks * 16;
+  const int heads = PAIR ? static_cast<int>(2 * a.g) : static_cast<int>(a.g - h0 < 16 ? a.g - h0 : 16);
   const int32_t* table = a.tables + b * a.t_sb + kv * a.t_sk;
   const uint32_t P = static_cast<uint32_t>(a.P), pages = static_cast<uint32_t>(a.pages);
   const char* pool = static_cast<const char*>(a.pool);
@@ -630,8 +639,9 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
     return F32 ? 16 * (kk >> 2) + 4 * j + (kk & 3)
                : (BITS == 8 && KL == 16 ? 64 * (kk >> 1) + 16 * j + 8 * (kk & 1) : 32 * kk + 8 * j);
   };
-  const bool live = c < heads;
-  const int64_t q_at = b * a.q_sb + (kv * a.g + h0 + (live ? c : 0)) * a.q_sh;
+  const bool live = PAIR ? (c & 7) < a.g : c < heads;
+  const int64_t own = kv * a.g + h0 + (PAIR ? (c >> 3) * a.g + (c & 7) : c);  // this column's query head
+  const int64_t q_at = b * a.q_sb + (live ? own : kv * a.g + h0) * a.q_sh;
   constexpr int QE = F32 ? 1 : 8;
   constexpr int QW = QD == HS_DTYPE_F32 ? QE : 4;  // words of a product's elements
   uint32_t qw[KK][QW];
@@ -662,10 +672,10 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
 
   // A tile's registers: scales, K and V.  Loads of the next tile go out as soon as the registers
   // of this one are consumed.
-  uint32_t kw[2][KN * KL / 4], vw[8][VW];
+  uint32_t kw[2][KVS * KN * KL / 4], vw[8][VW];
   float sc = 0.f;
   // 4-bit pools: the scale bytes of a lane's K loads, and all those of one token's V
-  uint32_t kb[2][fp4(S) ? KN : 1], vb[fp4(S) && GS > 4 ? 2 : 1];
+  uint32_t kb[2][fp4(S) ? KVS * KN : 1], vb[fp4(S) && GS > 4 ? 2 : 1];
   // token of the scale this lane holds (lanes 0-7 of a group: keys, 8-15: values)
   const int s_token = 4 * j + (c & 3), s_half = (c >> 2) & 1;
   float qs[F32 ? KK : 1];
@@ -709,28 +719,45 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
       f32x4 t = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (PAIR) {
+        f32x4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        if constexpr (F32) {
-          t = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[rt][kk]), qs[kk], t, 0, 0, 0);
-        } else {
-          u32x4 kf;
-          if constexpr (fp4(S)) {
-            widen_fp4_bf16x8(kw[rt][kk], __uint_as_float(kb[rt][kk / (KL / 4)] << 23), kf);
-          } else if constexpr (quantised(S)) {
+        for (int kk = 0; kk < KK; ++kk) {
+          u32x4 kf, kg;
+          widen_fp4_bf16x8(kw[rt][kk], __uint_as_float(kb[rt][0] << 23), kf);
+          widen_fp4_bf16x8(kw[rt][KK + kk], __uint_as_float(kb[rt][1] << 23), kg);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float x[4];
-              decode4<S>(kw[rt][2 * kk + h], x);
-              kf[2 * h] = pair_bf16(x[0], x[1]);
-              kf[2 * h + 1] = pair_bf16(x[2], x[3]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) kf[i] = kw[rt][4 * kk + i];
+          for (int q = 0; q < NQ; ++q) {
+            t = mfma_16x16x32<false>(kf, qf[q][kk], t);
+            u = mfma_16x16x32<false>(kg, qf[q][kk], u);
           }
+        }
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) t = mfma_16x16x32<F16>(kf, qf[q][kk], t);
+        for (int i = 0; i < 4; ++i) t[i] = c < 8 ? t[i] : u[i];
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          if constexpr (F32) {
+            t = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[rt][kk]), qs[kk], t, 0, 0, 0);
+          } else {
+            u32x4 kf;
+            if constexpr (fp4(S)) {
+              widen_fp4_bf16x8(kw[rt][kk], __uint_as_float(kb[rt][kk / (KL / 4)] << 23), kf);
+            } else if constexpr (quantised(S)) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float x[4];
+                decode4<S>(kw[rt][2 * kk + h], x);
+                kf[2 * h] = pair_bf16(x[0], x[1]);
+                kf[2 * h + 1] = pair_bf16(x[2], x[3]);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) kf[i] = kw[rt][4 * kk + i];
+            }
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) t = mfma_16x16x32<F16>(kf, qf[q][kk], t);
+          }
         }
       }
 #pragma unroll
@@ -925,7 +952,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
     // A load is a base every lane shares and a 32-bit offset of the lane's own.
     const uint32_t k_lane = c * row_bytes + j * KL;
     const uint32_t s_lane = static_cast<uint32_t>(s_token) * static_cast<uint32_t>(a.Hkv);
-    const uint32_t kb_lane = static_cast<uint32_t>(c) * static_cast<uint32_t>(a.Hkv) * GS + KL * j / 16;
+    const uint32_t kb_lane = static_cast<uint32_t>(c) * static_cast<uint32_t>(a.Hkv) * GS1 + KL * j / 16;
     uint32_t v_lane[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v_lane[e] = (4 * j + e) * row_bytes;
@@ -939,11 +966,11 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
       for (int rt = 0; rt < 2; ++rt) {
         const char* p = pool + (rt ? off1 : off0) * VECTOR;
 #pragma unroll
-        for (int i = 0; i < KN; ++i) load_words<KL>(p + k_lane + 4 * KL * i, &kw[rt][i * (KL / 4)]);
+        for (int i = 0; i < KVS * KN; ++i) load_words<KL>(p + k_lane + 4 * KL * i, &kw[rt][i * (KL / 4)]);
         if constexpr (fp4(S)) {
-          const unsigned char* b = a.scale_bytes + (rt ? off1 : off0) * GS;
+          const unsigned char* b = a.scale_bytes + (rt ? off1 : off0) * GS1;
 #pragma unroll
-          for (int i = 0; i < KN; ++i) kb[rt][i] = b[kb_lane + KL * i / 4];
+          for (int i = 0; i < KVS * KN; ++i) kb[rt][i] = b[kb_lane + (PAIR ? GS1 * i : KL * i / 4)];
         }
       }
     };
@@ -956,7 +983,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
         if constexpr (VB1 > 0) load_words<VB1>(p + (v_lane[e & 3] + v_col1), &vw[e][VW0]);
       }
       if constexpr (fp4(S))
-        load_scales<GS>(a.scale_bytes + ((s_half ? off1 : off0) + a.P * a.Hkv + s_lane) * GS, vb);
+        load_scales<GS>(a.scale_bytes + ((s_half ? off1 : off0) + a.P * a.Hkv + s_lane) * GS1, vb);
     };
     if (advance()) {
       load_k();
@@ -989,10 +1016,10 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
         const int64_t from = row_of(16 * rt + c);
         const char* p = pool + from * VECTOR + j * KL;
 #pragma unroll
-        for (int i = 0; i < KN; ++i) load_words<KL>(p + 4 * KL * i, &kw[rt][i * (KL / 4)]);
+        for (int i = 0; i < KVS * KN; ++i) load_words<KL>(p + 4 * KL * i, &kw[rt][i * (KL / 4)]);
         if constexpr (fp4(S)) {
 #pragma unroll
-          for (int i = 0; i < KN; ++i) kb[rt][i] = a.scale_bytes[from * GS + KL * j / 16 + KL * i / 4];
+          for (int i = 0; i < KVS * KN; ++i) kb[rt][i] = a.scale_bytes[from * GS1 + KL * j / 16 + (PAIR ? GS1 * i : KL * i / 4)];
         }
       }
     };
@@ -1004,7 +1031,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
         for (int i = 0; i < VB / VL; ++i) load_words<VL>(p + c * VB + VL * i, &vw[e][i * 4]);
         if constexpr (VB1 > 0) load_words<VB1>(p + 16 * VB + c * VB1, &vw[e][VW0]);
       }
-      if constexpr (fp4(S)) load_scales<GS>(a.scale_bytes + (row_of(16 * s_half + s_token) + a.P * a.Hkv) * GS, vb);
+      if constexpr (fp4(S)) load_scales<GS>(a.scale_bytes + (row_of(16 * s_half + s_token) + a.P * a.Hkv) * GS1, vb);
     };
     if (at_tile < tile1) {
       int32_t left = (tile1 - at_tile + subs - 1) / subs;
@@ -1021,16 +1048,21 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
     }
   }
 
-  auto dim_of = [](int v_lane, int e) { return e < E0 ? E0 * v_lane + e : 16 * E0 + (E - E0) * v_lane + e - E0; };
+  // (of a pair, the lanes whose rows are of their column's head)
+  const bool mine = live && (!PAIR || (j < 2) == (c < 8));
+  auto dim_of = [](int v_lane, int e) {
+    if constexpr (PAIR) return E * (v_lane & 7) + e;
+    return e < E0 ? E0 * v_lane + e : 16 * E0 + (E - E0) * v_lane + e - E0;
+  };
   m_run -= lift_at<F16>(m_run);  // the scale that the sums are at
   // the totals of a head over the four groups, then the waves of a unit, then the partial
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
   if (l_run != l_run) m_run = 0.f;  // NaN scores set no maximum: keep the partial in the merge
   if (!SHORT && a.subs == 1) {
-    if (live) {
-      const int64_t at = sh.slot * a.Hq + kv * a.g + h0 + c;
-      if (j == 0) {
+    if (mine) {
+      const int64_t at = sh.slot * a.Hq + own;
+      if (j == 0 || (PAIR && j == 2)) {
         a.part_m[at] = m_run;
         a.part_l[at] = l_run;
       }
@@ -1042,9 +1074,9 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
     }
     return;
   }
-  const int rows = static_cast<int>(a.g < 16 ? a.g : 16);
-  if (live) {
-    if (j == 0) {
+  const int rows = PAIR ? 16 : static_cast<int>(a.g < 16 ? a.g : 16);
+  if (mine) {
+    if (j == 0 || (PAIR && j == 2)) {
       s_m[wave][c] = m_run;
       s_l[wave][c] = l_run;
     }
@@ -1062,8 +1094,8 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
     const int d = i % QUADS * 4, hu = i / QUADS;
     const int u = SHORT ? 0 : hu / rows, h = SHORT ? hu : hu % rows;
     const int un = SHORT ? unit : static_cast<int>(blockIdx.y) * a.waves_units + u;
-    const int first = un % a.head_chunks * 16;
-    if (first + h >= a.g) continue;
+    const int first = PAIR ? 0 : un % a.head_chunks * 16;
+    if (PAIR ? (h & 7) >= a.g : first + h >= a.g) continue;
     float M = -INFINITY, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -1079,7 +1111,8 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
         O += f * *reinterpret_cast<const f32x4*>(smem + (at * rows + h) * SD + d);
       }
     }
-    const int64_t head = static_cast<int64_t>(un / a.head_chunks) * a.g + first + h;
+    const int64_t head = PAIR ? (2 * static_cast<int64_t>(un) + (h >> 3)) * a.g + (h & 7)
+                              : static_cast<int64_t>(un / a.head_chunks) * a.g + first + h;
     if constexpr (SHORT) {
       if (sh.parts == 1) {
         store_quad<QD>(a.out, b * a.o_sb + head * a.o_sh + d, L != 0.f ? O * (1.f / L) : f32x4{0.f, 0.f, 0.f, 0.f}, a.o_vec);
@@ -1179,7 +1212,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
 // ---- launches -------------------------------------------------------------------
 
 struct PagesPlan {
-  bool mfma, brief;
+  bool mfma, brief, pair;
   int G, head_chunks;
   int64_t splits, chunk;                 // general kernel
   int units, waves_units, subs;          // MFMA kernel
@@ -1188,7 +1221,7 @@ struct PagesPlan {
 
 template <int S, int QD>
 static void launch_mfma_pages(const PagesPlan& p, const PagesArgs& a, hipStream_t s) {
-  const int64_t waves = p.brief ? mfma_waves(a.D) : p.waves_units * p.subs, heads = a.g < 16 ? a.g : 16;
+  const int64_t waves = p.brief ? mfma_waves(a.D) : p.waves_units * p.subs, heads = p.pair || a.g > 16 ? 16 : a.g;
   const dim3 grid = p.brief ? dim3(static_cast<unsigned>(p.slots), static_cast<unsigned>(p.units), static_cast<unsigned>(a.B))
                             : dim3(static_cast<unsigned>(p.slots), static_cast<unsigned>(p.units / p.waves_units));
   const dim3 block(static_cast<unsigned>(64 * waves));
@@ -1196,8 +1229,15 @@ static void launch_mfma_pages(const PagesPlan& p, const PagesArgs& a, hipStream_
   int64_t bytes = !p.brief && p.subs == 1 ? 0 : waves * heads * (a.D + 4) * 4;
   if (p.brief && bytes < PM_PARTS * 16 * 4) bytes = PM_PARTS * 16 * 4;
   const unsigned smem = static_cast<unsigned>(bytes);
-#define HS_PAGES_RUN(DIM, U, SHORT) \
-  hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT>), grid, block, smem, s, a)
+#define HS_PAGES_RUN(DIM, U, SHORT)                                                                   \
+  do {                                                                                                \
+    if constexpr (fp4(S) && DIM <= 128 && DIM != 96) {                                                \
+      if (p.pair) hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT, true>), grid, block, smem, s, a); \
+      else hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT>), grid, block, smem, s, a);    \
+    } else {                                                                                          \
+      hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT>), grid, block, smem, s, a);         \
+    }                                                                                                 \
+  } while (0)
 #define HS_PAGES_D(DIM)                                         \
   do {                                                          \
     if (a.P % 16 == 0 && p.brief) HS_PAGES_RUN(DIM, true, true); \
