@@ -124,15 +124,148 @@ __global__ __launch_bounds__(64 * NW) void fp4_gemm_kernel(Fp4GemmArgs a) {
   }
 }
 
+// The form for many rows of a K that eight waves hold in one round each (K <= 4096): one workgroup a CU
+// keeps its waves' parts of x in registers and walks its share of the row tiles two at a time, the
+// next two's loads out before this two's products.  The waves' sums meet in one of two LDS
+// buffers, so that one barrier a turn, which waits for no load, is enough.
+constexpr int F4_WAVES = 8;
+
+template <int DT, bool NT>
+__global__ __launch_bounds__(64 * F4_WAVES) void fp4_gemm_walk_kernel(Fp4GemmArgs a) {
+  constexpr int U = F4_UNROLL, PARTS = DT == HS_DTYPE_F16 ? 2 : 1;
+  __shared__ float red[2][F4_WAVES][32][17];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int c = lane & 15, j = lane >> 4;
+  const int64_t lo = a.T * blockIdx.x / gridDim.x, hi = a.T * (blockIdx.x + 1) / gridDim.x;
+  const int busy = a.groups < F4_WAVES ? a.groups : F4_WAVES;  // waves with a part of K
+  const int K = static_cast<int>(a.K), first = wave * U;
+  // one turn's end: the waves' sums are in LDS, and the next turns' loads stay in flight
+  auto finish = [&](int buffer, int64_t t) {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int r = threadIdx.x & 31, m = threadIdx.x >> 5;
+    const int64_t n = t * 16 + r;
+    if (m < a.M && n < hi * 16 && n < a.N) {
+      float v = red[buffer][0][r][m];
+      for (int q = 1; q < busy; ++q) v += red[buffer][q][r][m];
+      if (a.bias) v += load_elem<DT>(a.bias, n);
+      store_elem<DT>(a.out, m * a.out_stride + n, v);
+    }
+  };
+  if (wave >= busy) {
+    for (int64_t t = lo, buffer = 0; t < hi; t += 2, buffer ^= 1) finish(static_cast<int>(buffer), t);
+    return;
+  }
+  struct Pair {
+    u32x4 w[2][U];
+    uint32_t sc[2];
+  };
+  auto load = [&](Pair& p, int64_t t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t tile = t + i < hi ? t + i : hi - 1;  // past the share: read again, dropped
+      p.sc[i] = a.scales[(tile * a.groups + wave) * 64 + lane];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // past the last block: read again, where x is 0
+        const int step = first + u < a.steps ? first + u : a.steps - 1;
+        const u32x4* at = reinterpret_cast<const u32x4*>(a.tiles + (tile * a.steps + step) * 1024 + lane * 16);
+        p.w[i][u] = NT ? __builtin_nontemporal_load(at) : *at;
+      }
+    }
+  };
+  u32x4 x[PARTS][U][4], raw[U][4];
+  const unsigned short* row = a.x + (c < a.M ? c : a.M - 1) * a.x_stride;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int k = F4_STEP * (first + u) + 32 * j;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[u][i] = *reinterpret_cast<const u32x4*>(row + (k < K ? k : 0) + 8 * i);
+  }
+  Pair one, two, three;
+  load(one, lo);
+  load(two, lo + 2);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const bool in = F4_STEP * (first + u) + 32 * j < K;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32x4 v = in ? raw[u][i] : u32x4{0u, 0u, 0u, 0u};
+      if constexpr (DT == HS_DTYPE_F16) {
+        u32x4 part[2];
+        split_f16x8(v, part);
+        x[0][u][i] = part[0];
+        x[1][u][i] = part[1];
+      } else {
+        x[0][u][i] = v;
+        // x is waited for here: a wait inside the loop would be one for younger loads too
+        asm volatile("" : "+v"(x[0][u][i]));
+      }
+    }
+  }
+  auto turn = [&](const Pair& p, int buffer, int64_t t) {
+    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float scale = __uint_as_float(__builtin_amdgcn_alignbit(p.sc[i], p.sc[i], (8 * u + 9) & 31));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          u32x4 wide;
+          widen_fp4_bf16x8(p.w[i][u][q], scale, wide);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) acc[i] = fp4_mfma(wide, x[part][u][q], acc[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[buffer][wave][16 * i + 4 * j + e][c] = acc[i][e];
+    finish(buffer, t);
+  };
+  if constexpr (DT == HS_DTYPE_F16) {  // x takes twice the registers
+    for (int64_t t = lo; t < hi; t += 4) {
+      turn(one, 0, t);
+      load(one, t + 4);
+      if (t + 2 >= hi) break;
+      turn(two, 1, t + 2);
+      load(two, t + 6);
+    }
+  } else {
+    int buffer = 0;
+    for (int64_t t = lo; t < hi; t += 6) {
+      load(three, t + 4);
+      turn(one, buffer, t);
+      if (t + 2 >= hi) break;
+      load(one, t + 6);
+      turn(two, buffer ^ 1, t + 2);
+      if (t + 4 >= hi) break;
+      load(two, t + 8);
+      turn(three, buffer, t + 4);
+      buffer ^= 1;
+    }
+  }
+}
+
 struct Fp4GemmPlan {
   int tiles, waves;
-  bool stream;
+  bool stream, walk;
 };
 
+// Row tiles and waves of a workgroup (not by the token rows, so that a row's sums are the same in every
+// batch).  Tiles share the reads of x, which at 16 token rows are four times a tile's own bytes, but
+// a CU should have a workgroup.  us for 1 and for 16 token rows, one, two and four tiles in 8 waves:
+// 3584 x 3584 3.95 4.41 5.33 and 5.8 6.3 7.6; 4608 x 3584 5.2 4.5 5.4 and 9.0 6.4 7.7; 8192 x 2048
+// 4.2 4.0 4.7 and 6.4 5.0 5.8; 12288 x 4096 8.1 8.6 7.5 and 14.1 12.9 9.8.  Where several workgroups
+// run on a CU in any case, those of four waves: four tiles of 55296 x 5120 in 8 waves 30.1 and 40.5,
+// in 4 26.3 and 35.9.  The walk: 37888 x 3584 15.8 and 17.9, four tiles in four waves 14.7 and 19.4;
+// 152064 x 3584 with 4 rows in float16 49.9 and 57.2; but 12288 x 4096 9.7 and 11.7, and where only
+// two of its waves have a part of K, 151936 x 896, 19.5 and 21.4 (17.7 and 23.1 in four tiles).
 static Fp4GemmPlan plan_fp4_gemm(int64_t T, int64_t groups) {
   Fp4GemmPlan p{};
-  p.tiles = T >= 2048 ? 4 : (T >= 1024 ? 2 : 1);
-  p.waves = p.tiles == 4 || groups <= 4 ? 4 : 8;
+  p.tiles = T > 512 ? 4 : (T > 256 ? 2 : 1);
+  p.waves = T > 1024 ? 4 : 8;
+  p.walk = T > 1024 && groups >= 4 && groups <= F4_WAVES;
   // a weight is read once per step: above the 4 MB of an XCD's L2 nothing of it is left for the next
   p.stream = T * groups * 4096 > (4 << 20);
   return p;
@@ -147,9 +280,15 @@ static void launch_fp4_gemm(const Fp4GemmPlan& p, const Fp4GemmArgs& a, hipStrea
 
 template <int DT>
 static void launch_fp4_gemm(const Fp4GemmPlan& p, const Fp4GemmArgs& a, hipStream_t s) {
-  if (p.tiles == 4) launch_fp4_gemm<DT, 4, 4>(p, a, s);
-  else if (p.tiles == 2) p.waves == 8 ? launch_fp4_gemm<DT, 2, 8>(p, a, s) : launch_fp4_gemm<DT, 2, 4>(p, a, s);
-  else p.waves == 8 ? launch_fp4_gemm<DT, 1, 8>(p, a, s) : launch_fp4_gemm<DT, 1, 4>(p, a, s);
+  if (p.walk) {
+    const dim3 grid(256), block(64 * F4_WAVES);  // one a CU; the plan gives each several tiles
+    if (p.stream) hipLaunchKernelGGL((fp4_gemm_walk_kernel<DT, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((fp4_gemm_walk_kernel<DT, false>), grid, block, 0, s, a);
+    return;
+  }
+  if (p.tiles == 4) p.waves == 8 ? launch_fp4_gemm<DT, 4, 8>(p, a, s) : launch_fp4_gemm<DT, 4, 4>(p, a, s);
+  else if (p.tiles == 2) launch_fp4_gemm<DT, 2, 8>(p, a, s);
+  else launch_fp4_gemm<DT, 1, 8>(p, a, s);
 }
 
 }  // namespace hs
