@@ -212,13 +212,20 @@ static PagesPlan plan_pages(bool mfma, bool pair, bool whole, int64_t bits, int6
     // 16 and 32 words: 12.9 16.2 and 12.6 12.6).
     // A unit of at most 128 KiB stays one part (14 query and 2 KV heads of 64 in int8, 64 requests
     // of 1024 tokens: 10.4 in one part, 12.7 in two).
-    const int64_t W = mfma_waves(D), rows = pair ? 2 * g : (g < 16 ? g : 16), held = pair ? 2 * D : D;
+    // For windows and 4-bit pools both limits are a little wider: two tiles more, as a window begins and
+    // its first tokens end inside a tile (16 windows of 4096, 28 and 4 heads of 128 in int8, 20.2 here and
+    // 22.4 long), and one part of up to 288 KiB of head dims up to 64 (one window of 1024, 14 and 2
+    // heads of 64 in bf16, 9.6 in one and 11.1 in eight; but of 28 and 4 heads of 128 in int8 11.3 and
+    // 11.0, 1060 tokens of 40 and 8 heads of 128 in 4 bits 15.5 and 13.4).
+    const bool wider = bits == 4 || most_seen(most, window, sinks) < most;
+    const int64_t W = mfma_waves(D), slack = wider ? 2 : 0, kib = wider && D <= 64 && tiles <= 4 * W + slack ? 288 : 128;
+    const int64_t rows = pair ? 2 * g : (g < 16 ? g : 16), held = pair ? 2 * D : D;
     int64_t parts = 256 / (B * p.units);
-    parts = parts < 1 || tiles * 2 * PM_TILE * held * bits <= 128 * 1024 * 8 ? 1 : (parts > PM_PARTS ? PM_PARTS : parts);
+    parts = parts < 1 || tiles * 2 * PM_TILE * held * bits <= kib * 1024 * 8 ? 1 : (parts > PM_PARTS ? PM_PARTS : parts);
     p.min_tiles = (tiles + parts - 1) / parts;
     if (p.min_tiles < W) p.min_tiles = W;
     p.slots = (tiles + p.min_tiles - 1) / p.min_tiles;
-    p.brief = p.min_tiles <= 4 * W && p.units <= 65535 && (p.slots == 1 || p.slots * rows * D < 16 * 64 * W);
+    p.brief = p.min_tiles <= 4 * W + slack && p.units <= 65535 && (p.slots == 1 || p.slots * rows * D < 16 * 64 * W);
     if (p.brief) return p;
     // Long: one workgroup a CU, over up to four units.  us at 4 histories of 32768
     // tokens, 14 query and 2 KV heads of 64 in bf16, for 256, 512 and 768 workgroups 20.4 21.4
