@@ -1,6 +1,8 @@
 // The normed (or plain) rotary split of norm_rotary.h with K and V written to a paged pool on the way:
 // q comes out, and no K or V is stored in between.  The pool is plain, of qkv's type, or quantised
 // (quantized.hip), and then its codes are those of the fp32 values, which are rounded once.
+// Bound by its bytes, or a short call by its chain of loads, table and stores: 16383 rows of 28 query
+// and 4 KV heads of 128 in bf16 into int8, 285 MB, take 59 us, 4.8 TB/s; 16 rows into bf16 4 us.
 #include "norm_rotary.h"
 
 namespace hs {
