@@ -636,8 +636,8 @@ int hs_skinny_gemm_argmax_tiled(const void* x, int64_t x_stride, const void* wei
  * (t, s) at t * ceil(k/128) + s: 64 runs of 16 bytes, run 16 j + c the 32 codes of row 16t + c from
  * k = 128s + 32j on (the even one in the low half of a byte).  weight_scales: for each t and each
  * four blocks, 64 dwords, dword 16 j + c the scale bytes of that run in those four blocks, the
- * first lowest.  Rows past n, k past the last and blocks past ceil(k/128) are zero bytes.  k a
- * multiple of 32 below 2^30; x rows and weight_tiles 16-byte aligned.  No workspace; a row's sums
+ * first lowest.  Rows past n, k past the last and blocks past ceil(k/128) are zero bytes.  n at most
+ * 2^28, k a multiple of 32 below 2^30; x rows and weight_tiles 16-byte aligned.  No workspace; a row's sums
  * do not depend on the other token rows.  No reference counterpart.
  */
 int hs_skinny_gemm_fp4(const void* x, int64_t x_stride, const void* weight_tiles, const void* weight_scales, int64_t n,

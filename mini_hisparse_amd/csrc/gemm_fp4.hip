@@ -33,14 +33,15 @@ __device__ __forceinline__ f32x4 fp4_mfma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Eight float16 as the sum of two bf16 (8 and then at most 3 significand bits: exact).
+// Eight float16 as the sum of two bf16 (8 and then at most 3 significand bits: exact; an infinity keeps
+// a finite second part, which an infinity less itself would not be).
 __device__ __forceinline__ void split_f16x8(u32x4 v, u32x4 (&part)[2]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float lo = f16_bits_to_f32(static_cast<unsigned short>(v[i])), hi = f16_bits_to_f32(static_cast<unsigned short>(v[i] >> 16));
     part[0][i] = pack16<false>(lo, hi);
-    lo -= __uint_as_float(part[0][i] << 16);
-    hi -= __uint_as_float(part[0][i] & 0xffff0000u);
+    lo = __builtin_amdgcn_fmed3f(lo - __uint_as_float(part[0][i] << 16), -65504.f, 65504.f);
+    hi = __builtin_amdgcn_fmed3f(hi - __uint_as_float(part[0][i] & 0xffff0000u), -65504.f, 65504.f);
     part[1][i] = pack16<false>(lo, hi);
   }
 }
@@ -300,8 +301,9 @@ extern "C" int hs_skinny_gemm_fp4(const void* x, int64_t x_stride, const void* t
                                   hipStream_t stream) {
   HS_CHECK_ARG(dtype == HS_DTYPE_BF16 || dtype == HS_DTYPE_F16, "4-bit projections take bf16 or f16 rows: dtype code %d", dtype);
   HS_CHECK_ARG(rows >= 1 && rows <= 16, "4-bit projections take 1 to 16 rows");
-  HS_CHECK_ARG(n >= 1 && n <= 0x7fffffff && k >= 32 && k % 32 == 0 && k < (int64_t{1} << 30),
-               "4-bit projections need n of 1 to 2^31 - 1 and k a multiple of 32 below 2^30");
+  // (n: the grid's threads stay below 2^32)
+  HS_CHECK_ARG(n >= 1 && n <= (int64_t{1} << 28) && k >= 32 && k % 32 == 0 && k < (int64_t{1} << 30),
+               "4-bit projections need n of 1 to 2^28 and k a multiple of 32 below 2^30");
   HS_CHECK_ARG(x && tiles && scales && out, "null 4-bit projection pointer");
   HS_CHECK_ARG(x_stride % 8 == 0 && (rows == 1 || x_stride >= k) && out_stride >= (rows == 1 ? 0 : n),
                "row strides below the width, or x rows not 16-byte aligned");

@@ -286,7 +286,8 @@ def attend_pages(query, pool, tables, lengths, *, window=None, sinks=0, out=None
     tables' width: one no wider than the histories need is faster for short ones.
 
     ``window``: of a request of n tokens only the newest ``window`` (t >= n - window) and the
-    first ``sinks`` (t < sinks) count.  The others' rows are not used, whatever their pages
+    first ``sinks`` (t < sinks) count, t being the position in the request's table (each KV
+    head's own where tables differ).  The others' rows are not used, whatever their pages
     hold or whether they are there, and whole tiles of them are not read: the launch is
     chosen, and takes the time, of histories of about ``window + sinks`` tokens.
 

@@ -55,7 +55,9 @@ def check(got, x, codes, scales, bias):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,k", [(1, 32), (16, 128), (17, 96), (1152, 896), (896, 896), (100, 4864), (33, 160), (5, 2080),
-                                 (640, 512), (24_000, 512), (40_000, 256), (33_000, 160), (16_400, 672), (16, 27_648)])
+                                 (640, 512), (24_000, 512), (40_000, 256), (33_000, 160), (16_400, 672), (16, 27_648),
+                                 (5000, 640), (9000, 288), (16_500, 1568), (16_401, 4096), (17_000, 3616),
+                                 (16_385, 4128)])
 def test_matches_the_product(gpu, dtype, n, k):
     codes, scales, weight = random_weight(n, k, gpu)
     gen = torch.Generator().manual_seed(1)
@@ -69,7 +71,7 @@ def test_matches_the_product(gpu, dtype, n, k):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_every_number_of_rows_alike(gpu, dtype):
     """A row's bits do not depend on the rows beside it."""
-    for n, k in ((1152, 896), (17_000, 288)):
+    for n, k in ((1152, 896), (5000, 640), (17_000, 288), (16_400, 2080)):
         codes, scales, weight = random_weight(n, k, gpu)
         x = torch.randn(16, k, device=gpu).to(dtype)
         full = linear_quantized(x, weight)
@@ -98,16 +100,22 @@ def test_scales_of_every_size(gpu, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_nan_and_infinity_reach_their_rows_alone(gpu, dtype):
-    codes, scales, _ = random_weight(40, 160, "cpu")
-    scales[7, 3] = 255
-    weight = QuantizedWeight.pack(codes.to(gpu), scales.to(gpu))
-    x = torch.randn(4, 160).to(dtype)
-    x[2, 159] = float("nan")
-    x[3, 0] = float("inf")
-    y = linear_quantized(x.to(gpu), weight).cpu()
-    assert y[:, 7].isnan().all() and y[2].isnan().all()
-    good = [n for n in range(40) if n != 7]
-    assert y[:2][:, good].isfinite().all() and not y[3, good].isfinite().any()
+    for n, k in ((40, 160), (16_400, 1568)):
+        codes, scales, _ = random_weight(n, k, "cpu")
+        scales[7, 3] = 255
+        weight = QuantizedWeight.pack(codes.to(gpu), scales.to(gpu))
+        x = torch.randn(4, k).to(dtype)
+        x[2, k - 1] = float("nan")
+        x[3, 0] = float("inf")
+        y = linear_quantized(x.to(gpu), weight).cpu()
+        assert y[:, 7].isnan().all() and y[2].isnan().all()
+        good = torch.arange(n) != 7
+        assert y[:2][:, good].isfinite().all()
+        # an infinity times its weight: NaN for a weight of 0, as in the plain product
+        first = widen_fp4(codes, scales)[:, 0]
+        want = torch.where(first == 0, float("nan"), first.sign() * float("inf"))[good]
+        assert torch.equal(y[3, good].isnan(), want.isnan())
+        assert torch.equal(y[3, good].nan_to_num(0.0, 1.0, -1.0).double(), want.nan_to_num(0.0, 1.0, -1.0))
 
 
 @pytest.mark.gpu
@@ -220,7 +228,7 @@ def test_entry_point_refusals_without_a_gpu():
         return lib.hs_skinny_gemm_fp4(x, stride, tiles, scales, n, k, None, out, out_stride, rows, dtype, None)
 
     for bad in (dict(x=None), dict(tiles=None), dict(scales=None), dict(out=None), dict(stride=60), dict(stride=56),
-                dict(n=0), dict(n=2**31), dict(k=0), dict(k=48), dict(k=2**30, stride=2**30), dict(out_stride=15),
+                dict(n=0), dict(n=2**28 + 1, out_stride=2**29), dict(k=0), dict(k=48), dict(k=2**30, stride=2**30), dict(out_stride=15),
                 dict(rows=0), dict(rows=17), dict(dtype=0), dict(dtype=3), dict(x=at + 2), dict(tiles=at + 8),
                 dict(scales=at + 2)):
         assert call(**bad) == -1, bad
