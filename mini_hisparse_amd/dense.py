@@ -174,6 +174,9 @@ def prepare_linear_tiled(x, tiles, n, bias, out, workspace):
     return _linear_tiled_launch(x, tiles, n, bias, out, ws)
 
 
+_LINEAR_DTYPES = (torch.bfloat16, torch.float16)
+
+
 @dataclass(frozen=True, eq=False)
 class QuantizedWeight:
     """A projection's weight [n, k] in 4 bits, laid out for :func:`linear_quantized`: e2m1 codes
@@ -196,6 +199,7 @@ class QuantizedWeight:
                 raise ValueError(f"a 4-bit weight of {self.n} x {self.k} needs contiguous uint8 {shape}")
         if self.tiles.device != self.scales.device:
             raise ValueError("codes and scales must be on one device")
+        object.__setattr__(self, "device", self.tiles.device)  # a plain attribute: every call reads it
 
     @classmethod
     def pack(cls, codes, scales):
@@ -250,24 +254,26 @@ def quantize_weight(weight):
 
 
 def _linear_quantized_check(x, weight, bias, out):
-    shape, dtype, device = x.shape, x.dtype, x.device
+    shape, stride, dtype, device = x.shape, x.stride(), x.dtype, x.device
     if len(shape) != 2 or not 1 <= shape[0] <= 16 or shape[1] != weight.k \
-            or dtype not in (torch.bfloat16, torch.float16) or x.stride(1) != 1 and shape[1] > 1 \
-            or shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < shape[1]) or x.data_ptr() % 16:
+            or dtype not in _LINEAR_DTYPES or stride[1] != 1 \
+            or shape[0] > 1 and (stride[0] % 8 or stride[0] < shape[1]) or x.data_ptr() % 16:
         raise ValueError("linear_quantized takes 1-16 rows of a bf16/f16 x [rows, k], rows 16-byte aligned")
     if bias is not None and (bias.shape != (weight.n,) or bias.dtype != dtype or not bias.is_contiguous()
                              or bias.device != device):
         raise ValueError("bias must be [n] contiguous in the dtype and on the device of x")
-    if weight.tiles.device != device:
+    if weight.device != device:
         raise ValueError("linear_quantized: x and the weight must be on one device")
-    _check_out(out, (shape[0], weight.n), x, "linear_quantized")
+    if out is not None:
+        _check_out(out, (shape[0], weight.n), x, "linear_quantized")
     if device.type != "cuda":
         raise ValueError("linear_quantized needs ROCm device tensors (HIP kernels only)")
 
 
 def _linear_quantized_args(x, weight, bias, y):
     rows, k = x.shape
-    return (x.data_ptr(), x.stride(0) if rows > 1 else k, weight.tiles.data_ptr(), weight.scales.data_ptr(), weight.n, k,
+    return (x.data_ptr(), x.stride(0) if rows > 1 else k, weight.tiles.data_ptr(),
+            weight.scales.data_ptr(), weight.n, k,
             _lib.ptr(bias), y.data_ptr(), y.stride(0) if rows > 1 else weight.n, rows, _lib.dtype_code(x.dtype))
 
 
@@ -517,33 +523,47 @@ def prepare_norm_rotary_split(qkv, q_weight, k_weight, eps, positions, heads, kv
 
 
 def _norm_rotary_append_check(qkv, q_weight, k_weight, positions, rows, pool, heads, out):
-    """The pool's (code, scales or None, rows, page size, KV heads, head dim)."""
+    """The pool's (codes or values, scales or None, code, rows, page size, KV heads, head dim)."""
     shape, stride, dtype, device = qkv.shape, qkv.stride(), qkv.dtype, qkv.device
-    code = _lib.dtype_code(dtype)
     if isinstance(pool, QuantizedPool):
-        held = (pool.codes, pool.scales, pool.code, pool.rows, pool.page_size, pool.kv_heads, pool.head_dim)
-    elif pool.dim() != 5 or pool.shape[1] != 2 or 0 in pool.shape or pool.dtype != dtype or not pool.is_contiguous():
-        raise ValueError("norm_rotary_append: a plain pool must be contiguous [blocks, 2, page_size, kv_heads, "
-                         "head_dim] in the dtype of qkv")
+        _lib.dtype_code(dtype)
+        kv_heads, head_dim = pool.vector
+        held = (pool.codes, pool.scales, pool.code, pool.rows, pool.page_size, kv_heads, head_dim)
+        pool_device = pool.device
     else:
-        held = (pool, None, code, pool.shape[0] * pool.shape[2], *pool.shape[2:])
-    kv_heads, head_dim = held[5:]
+        p_shape = pool.shape
+        if len(p_shape) != 5 or p_shape[1] != 2 or 0 in p_shape or pool.dtype != dtype or not pool.is_contiguous():
+            raise ValueError("norm_rotary_append: a plain pool must be contiguous [blocks, 2, page_size, kv_heads, "
+                             "head_dim] in the dtype of qkv")
+        blocks, _, page_size, kv_heads, head_dim = p_shape
+        held = (pool, None, _lib.dtype_code(dtype), blocks * page_size, page_size, kv_heads, head_dim)
+        pool_device = pool.device
     if heads < 1 or head_dim % 2 or head_dim > 512:
         raise ValueError("norm_rotary_append takes query heads and a pool of an even head_dim of at most 512")
     if len(shape) != 2 or shape[1] != (heads + 2 * kv_heads) * head_dim or stride[1] != 1 \
             or stride[0] < shape[1] and shape[0] > 1:
         raise ValueError("qkv must be [rows, (heads + 2 kv_heads) head_dim] with unit inner stride, its rows apart")
-    for name, x in (("positions", positions), ("rows", rows)):
-        if x.dtype != torch.int64 or x.shape != shape[:1] or x.device != device or not x.is_contiguous():
-            raise ValueError(f"{name} must be contiguous int64 [rows] on the device of qkv")
-    if (q_weight is None) != (k_weight is None):
-        raise ValueError("norm_rotary_append takes both norm weights or none")
-    for name, x in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if x is not None and (x.shape != (head_dim,) or x.dtype != dtype or x.device != device or not x.is_contiguous()):
-            raise ValueError(f"{name} must be [head_dim] contiguous in the dtype and on the device of qkv")
-    if held[0].device != device:
+    count = shape[:1]
+    if positions.dtype != torch.int64 or positions.shape != count or positions.device != device \
+            or not positions.is_contiguous():
+        raise ValueError("positions must be contiguous int64 [rows] on the device of qkv")
+    if rows.dtype != torch.int64 or rows.shape != count or rows.device != device or not rows.is_contiguous():
+        raise ValueError("rows must be contiguous int64 [rows] on the device of qkv")
+    if q_weight is None or k_weight is None:
+        if q_weight is not k_weight:
+            raise ValueError("norm_rotary_append takes both norm weights or none")
+    else:
+        width = (head_dim,)
+        if q_weight.shape != width or q_weight.dtype != dtype or q_weight.device != device \
+                or not q_weight.is_contiguous():
+            raise ValueError("q_weight must be [head_dim] contiguous in the dtype and on the device of qkv")
+        if k_weight.shape != width or k_weight.dtype != dtype or k_weight.device != device \
+                or not k_weight.is_contiguous():
+            raise ValueError("k_weight must be [head_dim] contiguous in the dtype and on the device of qkv")
+    if pool_device != device:
         raise ValueError("norm_rotary_append: the pool must be on the device of qkv")
-    _check_out(out, (shape[0], heads, head_dim), qkv, "norm_rotary_append")
+    if out is not None:
+        _check_out(out, (shape[0], heads, head_dim), qkv, "norm_rotary_append")
     if device.type != "cuda":
         raise ValueError("norm_rotary_append needs ROCm device tensors (HIP kernels only)")
     return held
