@@ -161,3 +161,29 @@ def test_a_layer_with_its_projections(gpu, dtype):
         x.copy_(fresh)
         graph.replay()
         assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(gpu):
+    """Layers of their own on two streams, launched in turn with no wait between them, give what each
+    gives alone (parts joined in the launch, and by a second one)."""
+    for prompts in ([2500, 3, 900], [9000, 40, 7000, 1]):
+        alone, beside = ([Layer(prompts, 30, torch.bfloat16, gpu) for _ in range(2)] for _ in range(2))
+        inputs = []
+        for pair in (alone, beside):
+            for layer in pair:
+                for b, n in enumerate(prompts):
+                    layer.prefill(b, n)
+        for layer in alone:
+            inputs.append([layer.hidden(len(prompts)) for _ in range(10)])
+        want = [[layer.decode(x)[-1] for x in xs] for layer, xs in zip(alone, inputs)]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(torch.device(gpu)) for _ in beside]
+        got = [[], []]
+        for i in range(10):
+            for k, (layer, stream) in enumerate(zip(beside, streams)):
+                with torch.cuda.stream(stream):
+                    got[k].append(layer.decode(inputs[k][i])[-1])
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
