@@ -289,8 +289,9 @@ static int check_window(int64_t window, int64_t sinks) {
   HS_CHECK_ARG(window > 0 || sinks == 0, "first tokens that stay go with a window");
   return HS_OK;
 }
-static int32_t window_of(int64_t window) {
-  return window == 0 || window >= NO_WINDOW ? NO_WINDOW : static_cast<int32_t>(window);
+// (a window of every token that the tables can name is none)
+static int32_t window_of(int64_t window, int64_t tokens) {
+  return window == 0 || window >= tokens ? NO_WINDOW : static_cast<int32_t>(window);
 }
 static int32_t sinks_of(int64_t sinks) { return clamp_length(sinks, NO_WINDOW); }
 
@@ -304,7 +305,7 @@ extern "C" int64_t hs_attend_pages_window_workspace_bytes(int32_t query_dtype, i
                                                           int64_t sinks) {
   if (check_pages(batch, heads, kv_heads, head_dim, page_size, pages) || check_window(window, sinks)) return 256;
   const int64_t bits = elem_bits(pool_code), tokens = pages * page_size;
-  const int32_t newest = window_of(window), first = sinks_of(sinks);
+  const int32_t newest = window_of(window, tokens), first = sinks_of(sinks);
   const bool shape = pages_mfma_shape(bits, kv_heads, head_dim);
   auto need_of = [&](bool mfma, bool pair, bool whole) {
     return pages_workspace(plan_pages(mfma, pair, whole, bits, batch, heads, kv_heads, head_dim, tokens, newest, first),
@@ -356,7 +357,7 @@ extern "C" int hs_attend_pages_window(const void* query, int64_t q_stride_b, int
   HS_CHECK_ARG(quantised_pool == (scales != nullptr), "scales go with a quantised pool, and only with one");
   HS_CHECK_ARG(blocks >= 1 && blocks <= 0x7fffffff, "a pool has 1 to 2^31 - 1 blocks");
   const int64_t bits = elem_bits(pool_code), tokens = pages * page_size;
-  const int32_t newest = window_of(window), first = sinks_of(sinks);
+  const int32_t newest = window_of(window, tokens), first = sinks_of(sinks);
   const bool shape = pages_mfma_shape(bits, kv_heads, head_dim);
   // (4-bit scales of 256 of the head dim are loaded eight at a time)
   const bool mfma = shape && reinterpret_cast<uintptr_t>(pool) % 16 == 0 &&
@@ -428,13 +429,17 @@ extern "C" int hs_attend_pages_window(const void* query, int64_t q_stride_b, int
       hipLaunchKernelGGL(pages_schedule_kernel, dim3(1), dim3(PS_T), 0, stream, a, p.slots);
       HS_CHECK_LAUNCH("page attention schedule");
     }
-    switch (pool_code) {
-      case HS_DTYPE_F32: launch_mfma_pages<HS_DTYPE_F32, HS_DTYPE_F32>(p, a, stream); break;
-      case HS_DTYPE_F16: launch_mfma_pages<HS_DTYPE_F16, HS_DTYPE_F16>(p, a, stream); break;
-      case HS_DTYPE_BF16: launch_mfma_pages<HS_DTYPE_BF16, HS_DTYPE_BF16>(p, a, stream); break;
-      case HS_DTYPE_I8: launch_mfma_codes<HS_DTYPE_I8>(p, a, stream); break;
-      case HS_DTYPE_E2M1: launch_fp4_pages(p, a, true, stream); break;
-      default: launch_mfma_codes<HS_DTYPE_E4M3>(p, a, stream); break;
+    if (newest != NO_WINDOW) {
+      launch_window_pages(pool_code, p, a, stream);
+    } else {
+      switch (pool_code) {
+        case HS_DTYPE_F32: launch_mfma_pool<HS_DTYPE_F32, false>(p, a, stream); break;
+        case HS_DTYPE_F16: launch_mfma_pool<HS_DTYPE_F16, false>(p, a, stream); break;
+        case HS_DTYPE_BF16: launch_mfma_pool<HS_DTYPE_BF16, false>(p, a, stream); break;
+        case HS_DTYPE_I8: launch_mfma_pool<HS_DTYPE_I8, false>(p, a, stream); break;
+        case HS_DTYPE_E2M1: launch_fp4_pages(p, a, true, stream); break;
+        default: launch_mfma_pool<HS_DTYPE_E4M3, false>(p, a, stream); break;
+      }
     }
   } else {
     const bool vec = head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(pool) % (bits / 2) == 0;

@@ -5,7 +5,7 @@
 namespace hs {
 
 void launch_fp4_pages(const PagesPlan& p, const PagesArgs& a, bool vec, hipStream_t s) {
-  if (p.mfma) launch_mfma_codes<HS_DTYPE_E2M1>(p, a, s);
+  if (p.mfma) launch_mfma_pool<HS_DTYPE_E2M1, false>(p, a, s);
   else launch_general<HS_DTYPE_E2M1>(p, a, vec, s);
 }
 

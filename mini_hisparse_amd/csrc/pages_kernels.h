@@ -373,6 +373,13 @@ __global__ __launch_bounds__(PG_T) void pages_general_kernel(PagesArgs a) {
 
 // Waves of a workgroup: half as many for 256 of the head dim, with twice the registers each.
 constexpr int mfma_waves(int64_t D) { return D > 128 ? 4 : 8; }
+// Waves a SIMD that the register allocator is held to (1: it decides).  float16 queries of 64 of the head
+// dim in the short launch stand at the border between one workgroup a CU and two (126 to 130 registers)
+// and fit below it without a spill (us with it and without, 14 and 2 heads on e4m3, 256 requests of
+// 1024 tokens 22.9 and 24.3, 1024 of 256 26.4 and 32.5); a pair's 157 do not.
+constexpr int mfma_least(int QD, int64_t D, bool SHORT, bool PAIR) {
+  return QD == HS_DTYPE_F16 && D == 64 && SHORT && !PAIR ? 4 : 1;
+}
 constexpr int PM_PARTS = 8;  // parts of a short request
 constexpr int PM_LANES = 64;  // requests whose schedule a wave derives by itself
 constexpr float PM_SLACK = 6.f;
@@ -482,10 +489,11 @@ __device__ __forceinline__ T scan_lanes(T v) {
 
 // The request and part of workgroup w, of up to PM_LANES requests: every wave derives the same
 // schedule from the lengths, one request a lane.
+template <bool WINDOW>
 __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& out) {
   const int lane = threadIdx.x & 63;
   const int32_t n = lane < a.B ? clamp_length(a.lengths[lane], a.pages * a.P) : 0;
-  const int32_t tiles = seen_tiles(n, a.window, a.sinks);
+  const int32_t tiles = WINDOW ? seen_tiles(n, a.window, a.sinks) : tiles_of(n);
   const float total =
       __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scan_lanes(static_cast<float>(tiles))), 63));
   const uint32_t target = static_cast<uint32_t>(a.target), min_tiles = static_cast<uint32_t>(a.min_tiles);
@@ -530,8 +538,13 @@ __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& o
 // serves two heads.  us with one head a unit and with two: 8 requests of 131072 tokens, 28 and 4
 // heads of 128, 112 (the loads alone 111) and 106; 16 of 65536 .. 20521, 40 and 8 heads, float16
 // queries, 166 and 137; one of 1999, 14 and 2 heads of 64, 14.1 and 11.2.
-template <int S, int QD, int D, bool UNIFORM, bool SHORT, bool PAIR = false>
-__global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArgs a) {
+// WINDOW: whole histories have kernels without its arithmetic, which takes up to ten registers and
+// with them one of two workgroups a CU where a kernel stands at the border.  us with it and without,
+// 14 query and 2 KV heads of 64, whole histories: float16, 512 requests of 1024 tokens 47.3 and 42.8,
+// 1024 of 256 37.5 and 30.2; float16 queries on e4m3, 256 of 1 .. 4096 41.4 and 40.4 (96 of 4096 each,
+// 40 and 8 heads, are as fast again as before with two workgroups a CU, 121, and were 112 with one).
+template <int S, int QD, int D, bool UNIFORM, bool SHORT, bool WINDOW, bool PAIR = false>
+__global__ __launch_bounds__(64 * mfma_waves(D), mfma_least(QD, D, SHORT, PAIR)) void pages_mfma_kernel(PagesArgs a) {
   static_assert(!PAIR || (fp4(S) && D <= 128 && D != 96), "pairs of 4-bit head vectors of 32, 64 or 128");
   constexpr int KVS = PAIR ? 2 : 1, DD = KVS * D;  // KV heads of a unit; their vectors' elements
   constexpr int W = mfma_waves(D), T = 64 * W;
@@ -564,7 +577,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
       if (t.b < 0) return;
       sh = Share{t.b, static_cast<int32_t>(blockIdx.x), t.part, t.parts, t.n};
     } else {
-      if (!share_of(a, static_cast<int32_t>(blockIdx.x), sh)) return;  // the same for every wave
+      if (!share_of<WINDOW>(a, static_cast<int32_t>(blockIdx.x), sh)) return;  // the same for every wave
       if (sh.part == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.ranges[sh.b] = SlotRange{sh.slot, sh.parts};
     }
   }
@@ -600,7 +613,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
   Seen view{0, 0, 0};
   auto measure = [&]() {  // waits for the length
     n = __builtin_amdgcn_readfirstlane(length < 0 ? 0 : (length > limit ? static_cast<int32_t>(limit) : length));
-    view = seen_of(n, a.window, a.sinks);
+    if constexpr (WINDOW) view = seen_of(n, a.window, a.sinks);
     tiles = tiles_of(n) - view.gap;
     if constexpr (SHORT) sh.parts = tiles > share ? (tiles + share - 1) / share : 1;
   };
@@ -608,10 +621,10 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
     measure();
     share = (tiles + sh.parts - 1) / sh.parts;
     tile0 = sh.part * share;
-  } else if (a.window != NO_WINDOW) {
+  } else if constexpr (WINDOW) {
     measure();  // which table entries come first depends on the length then
   }
-  auto tile_at = [&](int32_t tile) { return tile + (tile >= view.front ? view.gap : 0); };
+  auto tile_at = [&](int32_t tile) { return WINDOW && tile >= view.front ? tile + view.gap : tile; };
 
   // UNIFORM: pages of a multiple of 16 rows, so a tile's two halves lie in one page each.  A wave
   // reads the table for 32 of its tiles at once (lane l: half l), keeps the halves' first rows
@@ -642,8 +655,9 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
                : (BITS == 8 && KL == 16 ? 64 * (kk >> 1) + 16 * j + 8 * (kk & 1) : 32 * kk + 8 * j);
   };
   const bool live = PAIR ? (c & 7) < a.g : c < heads;
-  const int64_t own = kv * a.g + h0 + (PAIR ? (c >> 3) * a.g + (c & 7) : c);  // this column's query head
-  const int64_t q_at = b * a.q_sb + (live ? own : kv * a.g + h0) * a.q_sh;
+  // (this column's query head past the unit's first; not held through the loop: two registers)
+  auto column = [&](int v) { return PAIR ? (v >> 3) * a.g + (v & 7) : v; };
+  const int64_t q_at = b * a.q_sb + (kv * a.g + h0 + column(live ? c : 0)) * a.q_sh;
   constexpr int QE = F32 ? 1 : 8;
   constexpr int QW = QD == HS_DTYPE_F32 ? QE : 4;  // words of a product's elements
   uint32_t qw[KK][QW];
@@ -663,7 +677,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
       }
     }
   }
-  if (SHORT && a.window == NO_WINDOW) measure();
+  if constexpr (SHORT && !WINDOW) measure();
   const int32_t tile1 = tile0 + share < tiles ? tile0 + share : tiles;
   if (SHORT && sh.part > 0 && tile0 >= tiles) return;  // past the request's tiles: the whole workgroup
 
@@ -937,7 +951,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
       const int at = __ffsll(static_cast<unsigned long long>(some)) - 1;
       const int32_t base = 32 * tile_at(tile0 + sub + (batch + (at >> 1)) * subs), left = n - base;
       valid = left >= PM_TILE ? 0xffffffffu : (1u << left) - 1u;
-      if (base < view.lo) valid &= seen_mask(base, view.lo, a.sinks);
+      if (WINDOW && base < view.lo) valid &= seen_mask(base, view.lo, a.sinks);
       const uint32_t has = static_cast<uint32_t>(present >> at) & 3u;
       if (!(has & 1u)) valid &= 0xffff0000u;
       if (!(has & 2u)) valid &= 0x0000ffffu;
@@ -1004,7 +1018,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
     auto advance = [&]() {
       const uint32_t t = token_of(at_tile);
       const bool ok = at_tile < tile1 && t < static_cast<uint32_t>(n) && entry >= 0 && entry < a.blocks &&
-                      (t >= static_cast<uint32_t>(view.lo) || t < static_cast<uint32_t>(a.sinks));
+                      (!WINDOW || t >= static_cast<uint32_t>(view.lo) || t < static_cast<uint32_t>(a.sinks));
       row = ok ? (static_cast<int64_t>(entry) * 2 * P + within) * a.Hkv + kv : 0;
       valid = static_cast<uint32_t>(__ballot(ok));
       at_tile += subs;
@@ -1063,7 +1077,7 @@ __global__ __launch_bounds__(64 * mfma_waves(D)) void pages_mfma_kernel(PagesArg
   if (l_run != l_run) m_run = 0.f;  // NaN scores set no maximum: keep the partial in the merge
   if (!SHORT && a.subs == 1) {
     if (mine) {
-      const int64_t at = sh.slot * a.Hq + own;
+      const int64_t at = sh.slot * a.Hq + kv * a.g + h0 + column(c);
       if (j == 0 || (PAIR && j == 2)) {
         a.part_m[at] = m_run;
         a.part_l[at] = l_run;
@@ -1221,7 +1235,7 @@ struct PagesPlan {
   int64_t target, min_tiles, slots;
 };
 
-template <int S, int QD>
+template <int S, int QD, bool WINDOW>
 static void launch_mfma_pages(const PagesPlan& p, const PagesArgs& a, hipStream_t s) {
   const int64_t waves = p.brief ? mfma_waves(a.D) : p.waves_units * p.subs, heads = p.pair || a.g > 16 ? 16 : a.g;
   const dim3 grid = p.brief ? dim3(static_cast<unsigned>(p.slots), static_cast<unsigned>(p.units), static_cast<unsigned>(a.B))
@@ -1234,10 +1248,10 @@ static void launch_mfma_pages(const PagesPlan& p, const PagesArgs& a, hipStream_
 #define HS_PAGES_RUN(DIM, U, SHORT)                                                                   \
   do {                                                                                                \
     if constexpr (fp4(S) && DIM <= 128 && DIM != 96) {                                                \
-      if (p.pair) hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT, true>), grid, block, smem, s, a); \
-      else hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT>), grid, block, smem, s, a);    \
+      if (p.pair) hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT, WINDOW, true>), grid, block, smem, s, a); \
+      else hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT, WINDOW>), grid, block, smem, s, a); \
     } else {                                                                                          \
-      hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT>), grid, block, smem, s, a);         \
+      hipLaunchKernelGGL((pages_mfma_kernel<S, QD, DIM, U, SHORT, WINDOW>), grid, block, smem, s, a); \
     }                                                                                                 \
   } while (0)
 #define HS_PAGES_D(DIM)                                         \
@@ -1256,11 +1270,16 @@ static void launch_mfma_pages(const PagesPlan& p, const PagesArgs& a, hipStream_
 #undef HS_PAGES_RUN
 }
 
-template <int S>
-static void launch_mfma_codes(const PagesPlan& p, const PagesArgs& a, hipStream_t s) {
-  if (a.q_dtype == HS_DTYPE_BF16) launch_mfma_pages<S, HS_DTYPE_BF16>(p, a, s);
-  else if (a.q_dtype == HS_DTYPE_F16) launch_mfma_pages<S, HS_DTYPE_F16>(p, a, s);
-  else launch_mfma_pages<S, HS_DTYPE_F32>(p, a, s);
+// The matrix-core launch over a pool of element code S; WINDOW where a.window is one.
+template <int S, bool WINDOW>
+static void launch_mfma_pool(const PagesPlan& p, const PagesArgs& a, hipStream_t s) {
+  if constexpr (quantised(S) || fp4(S)) {  // any query type
+    if (a.q_dtype == HS_DTYPE_BF16) launch_mfma_pages<S, HS_DTYPE_BF16, WINDOW>(p, a, s);
+    else if (a.q_dtype == HS_DTYPE_F16) launch_mfma_pages<S, HS_DTYPE_F16, WINDOW>(p, a, s);
+    else launch_mfma_pages<S, HS_DTYPE_F32, WINDOW>(p, a, s);
+  } else {
+    launch_mfma_pages<S, S, WINDOW>(p, a, s);
+  }
 }
 
 template <int S>
@@ -1282,7 +1301,10 @@ static void launch_general(const PagesPlan& p, const PagesArgs& a, bool vec, hip
 #undef HS_PAGES_RUN
 }
 
-// 4-bit pools (pages_fp4.hip): the launch that the plan names; `vec`, for the vector-unit kernel.
+// The launches of other files: whole histories in 4 bits (pages_fp4.hip; `vec`, for the vector-unit
+// kernel), and windows, for which the vector-unit kernel has no forms of its own (pages_window.hip).
 void launch_fp4_pages(const PagesPlan& p, const PagesArgs& a, bool vec, hipStream_t s);
+void launch_window_pages(int pool_code, const PagesPlan& p, const PagesArgs& a, hipStream_t s);
+void launch_fp4_window_pages(const PagesPlan& p, const PagesArgs& a, hipStream_t s);
 
 }  // namespace hs
