@@ -22,7 +22,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .quantized import FP4_GROUP, QuantizedPool
+from .quantized import FP4_CODES, FP4_GROUP, FP4_SCALES, QuantizedPool
 
 
 def _stream(tensor):
@@ -205,9 +205,9 @@ class QuantizedWeight:
     def pack(cls, codes, scales):
         """``codes`` [n, k / 2] (float4_e2m1fn_x2 or its bytes: two a byte, the even one in the low
         half) with ``scales`` [n, k / 32] (float8_e8m0fnu or its bytes) in the kernel's layout."""
-        if codes.dtype == torch.float4_e2m1fn_x2:
+        if codes.dtype == FP4_CODES:
             codes = codes.view(torch.uint8)
-        if scales.dtype == torch.float8_e8m0fnu:
+        if scales.dtype == FP4_SCALES:
             scales = scales.view(torch.uint8)
         if codes.dtype != torch.uint8 or codes.dim() != 2 or 0 in codes.shape or codes.shape[1] % (FP4_GROUP // 2):
             raise ValueError("codes must be float4_e2m1fn_x2 or uint8 [n, k / 2], k a multiple of 32")

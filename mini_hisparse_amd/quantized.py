@@ -22,6 +22,9 @@ import torch
 from . import _lib
 
 FP4_GROUP = 32  # neighbours that share a scale of 4-bit codes
+# the dtypes of 4-bit codes and their scales; None in builds of torch that lack them
+FP4_CODES = getattr(torch, "float4_e2m1fn_x2", None)
+FP4_SCALES = getattr(torch, "float8_e8m0fnu", None)
 
 
 @dataclass(frozen=True, eq=False)
@@ -42,7 +45,7 @@ class QuantizedPool:
             if codes.shape[4] % (FP4_GROUP // 2):
                 raise ValueError("4-bit pools need a head_dim of a multiple of 32")
             if scales.shape != (*codes.shape[:-1], codes.shape[4] * 2 // FP4_GROUP) \
-                    or scales.dtype != torch.float8_e8m0fnu or not scales.is_contiguous():
+                    or scales.dtype != FP4_SCALES or not scales.is_contiguous():
                 raise ValueError("scales must be contiguous float8_e8m0fnu [blocks, 2, page_size, kv_heads, head_dim / 32]")
         elif scales.shape != codes.shape[:-1] or scales.dtype != torch.float32 or not scales.is_contiguous():
             raise ValueError("scales must be contiguous float32 [blocks, 2, page_size, kv_heads]")
@@ -59,12 +62,12 @@ class QuantizedPool:
     def empty(cls, blocks, page_size, kv_heads, head_dim, dtype=torch.int8, device="cuda"):
         """A pool of zeros: every row reads back as zero until it is written."""
         shape = (blocks, 2, page_size, kv_heads, head_dim)
-        if dtype == torch.float4_e2m1fn_x2:
+        if dtype is not None and dtype == FP4_CODES:
             if head_dim % FP4_GROUP:
                 raise ValueError("4-bit pools need a head_dim of a multiple of 32")
             codes, scales = (torch.zeros((*shape[:-1], n), dtype=torch.uint8, device=device)
                              for n in (head_dim // 2, head_dim // FP4_GROUP))
-            return cls(codes.view(dtype), scales.view(torch.float8_e8m0fnu))
+            return cls(codes.view(dtype), scales.view(FP4_SCALES))
         codes = torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype)
         return cls(codes, torch.zeros(shape[:-1], device=device))
 
