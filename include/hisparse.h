@@ -501,7 +501,8 @@ int hs_read_quantized(const void* codes, const void* scales, int32_t code, int64
  * device; a row outside [0, pool_rows) is skipped, the others of one call must differ).  pool and
  * scales as for hs_append_quantized, or a plain pool [blocks, 2, P, Hkv, D] of `dtype` (pool_code
  * dtype, scales null).  Quantised rows are those of the fp32 values.  q_weight and k_weight both
- * null: no norm.  rows may be 0; head_dim at most 512, even, for HS_DTYPE_E2M1 a multiple of 32.
+ * null: no norm, and eps is not looked at.  rows may be 0; head_dim at most 512, even, for
+ * HS_DTYPE_E2M1 a multiple of 32.
  */
 int hs_norm_rotary_append(const void* qkv, int64_t qkv_stride, const void* q_weight, const void* k_weight, float eps,
                           void* q, const int64_t* positions, const int64_t* to_rows, int64_t rows, int64_t heads,

@@ -40,7 +40,7 @@ extern "C" int hs_norm_rotary_append(const void* qkv, int64_t qkv_stride, const 
   HS_CHECK_ARG(pool != nullptr && quantised == (scales != nullptr), "scales go with a quantised pool, and only with one");
   HS_CHECK_ARG(!valid_code(pool_code) || reinterpret_cast<uintptr_t>(scales) % 4 == 0, "scales must be 4-byte aligned");
   HS_CHECK_ARG((q_weight == nullptr) == (k_weight == nullptr), "both norm weights, or none");
-  HS_CHECK_ARG(theta > 0.0 && isfinite(theta) && eps >= 0.f, "theta must be positive and eps not negative");
+  HS_CHECK_ARG(theta > 0.0 && isfinite(theta) && (eps >= 0.f || !q_weight), "theta must be positive and eps not negative");
   if (rows == 0) return HS_OK;
   HS_CHECK_ARG(qkv && q && positions && to_rows, "null normed rotary append pointer");
   uintptr_t all = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_weight) |

@@ -573,8 +573,8 @@ def _norm_rotary_append_args(qkv, q_weight, k_weight, eps, positions, rows, head
     store, scales, code, pool_rows, page_size, kv_heads, head_dim = held
     count, width = qkv.shape
     stride = qkv.stride(0)
-    return (qkv.data_ptr(), stride if stride > width else width, _lib.ptr(q_weight), _lib.ptr(k_weight), eps,
-            q.data_ptr(), positions.data_ptr(), rows.data_ptr(), count, heads, theta, _lib.dtype_code(qkv.dtype),
+    return (qkv.data_ptr(), stride if stride > width else width, _lib.ptr(q_weight), _lib.ptr(k_weight),
+            0.0 if q_weight is None else eps, q.data_ptr(), positions.data_ptr(), rows.data_ptr(), count, heads, theta, _lib.dtype_code(qkv.dtype),
             store.data_ptr(), _lib.ptr(scales), code, pool_rows, page_size, kv_heads, head_dim)
 
 
