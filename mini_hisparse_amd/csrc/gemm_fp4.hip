@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * NW) void fp4_gemm_kernel(Fp4GemmArgs a) {
 // buffers, so that one barrier a turn, which waits for no load, is enough.
 constexpr int F4_WAVES = 8;
 
-template <int DT, bool NT>
+template <int DT>
 __global__ __launch_bounds__(64 * F4_WAVES) void fp4_gemm_walk_kernel(Fp4GemmArgs a) {
   constexpr int U = F4_UNROLL, PARTS = DT == HS_DTYPE_F16 ? 2 : 1;
   __shared__ float red[2][F4_WAVES][32][17];
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * F4_WAVES) void fp4_gemm_walk_kernel(Fp4GemmArg
       for (int u = 0; u < U; ++u) {  // past the last block: read again, where x is 0
         const int step = first + u < a.steps ? first + u : a.steps - 1;
         const u32x4* at = reinterpret_cast<const u32x4*>(a.tiles + (tile * a.steps + step) * 1024 + lane * 16);
-        p.w[i][u] = NT ? __builtin_nontemporal_load(at) : *at;
+        p.w[i][u] = __builtin_nontemporal_load(at);
       }
     }
   };
@@ -268,6 +268,7 @@ static Fp4GemmPlan plan_fp4_gemm(int64_t T, int64_t groups) {
   p.waves = T > 1024 ? 4 : 8;
   p.walk = T > 1024 && groups >= 4 && groups <= F4_WAVES;
   // a weight is read once per step: above the 4 MB of an XCD's L2 nothing of it is left for the next
+  // (more than 1024 row tiles are always above: the forms for them have no other loads)
   p.stream = T * groups * 4096 > (4 << 20);
   return p;
 }
@@ -275,16 +276,20 @@ static Fp4GemmPlan plan_fp4_gemm(int64_t T, int64_t groups) {
 template <int DT, int GT, int NW>
 static void launch_fp4_gemm(const Fp4GemmPlan& p, const Fp4GemmArgs& a, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((a.T + GT - 1) / GT));
-  if (p.stream) hipLaunchKernelGGL((fp4_gemm_kernel<DT, GT, NW, true>), grid, dim3(64 * NW), 0, s, a);
-  else hipLaunchKernelGGL((fp4_gemm_kernel<DT, GT, NW, false>), grid, dim3(64 * NW), 0, s, a);
+  if constexpr (NW == 8) {
+    if (!p.stream) {
+      hipLaunchKernelGGL((fp4_gemm_kernel<DT, GT, NW, false>), grid, dim3(64 * NW), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((fp4_gemm_kernel<DT, GT, NW, true>), grid, dim3(64 * NW), 0, s, a);
 }
 
 template <int DT>
 static void launch_fp4_gemm(const Fp4GemmPlan& p, const Fp4GemmArgs& a, hipStream_t s) {
   if (p.walk) {
-    const dim3 grid(256), block(64 * F4_WAVES);  // one a CU; the plan gives each several tiles
-    if (p.stream) hipLaunchKernelGGL((fp4_gemm_walk_kernel<DT, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((fp4_gemm_walk_kernel<DT, false>), grid, block, 0, s, a);
+    // one workgroup a CU; the plan gives each several tiles
+    hipLaunchKernelGGL((fp4_gemm_walk_kernel<DT>), dim3(256), dim3(64 * F4_WAVES), 0, s, a);
     return;
   }
   if (p.tiles == 4) p.waves == 8 ? launch_fp4_gemm<DT, 4, 8>(p, a, s) : launch_fp4_gemm<DT, 4, 4>(p, a, s);
