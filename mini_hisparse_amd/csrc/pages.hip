@@ -184,7 +184,7 @@ static bool pages_mfma_shape(int64_t bits, int64_t Hkv, int64_t D) {
   return (D == 32 || D == 64 || D == 96 || D == 128 || (D == 256 && bits < 32)) && Hkv * D * bits < (int64_t{1} << 30);
 }
 
-// 4-bit pools whose KV heads share their tables go two KV heads a unit where the products' 16 columns
+// 4-bit pools whose KV heads share their tables may go two KV heads a unit where the products' 16 columns
 // hold both's query heads.
 static bool pages_pair_shape(int pool_code, int64_t Hq, int64_t Hkv, int64_t D) {
   return pool_code == HS_DTYPE_E2M1 && (D == 32 || D == 64 || D == 128) && Hkv % 2 == 0 && Hq / Hkv <= 8;
@@ -216,7 +216,9 @@ static PagesPlan plan_pages(bool mfma, bool pair, bool whole, int64_t bits, int6
     // its first tokens end inside a tile (16 windows of 4096, 28 and 4 heads of 128 in int8, 20.2 here and
     // 22.4 long), and one part of up to 288 KiB of head dims up to 64 (one window of 1024, 14 and 2
     // heads of 64 in bf16, 9.6 in one and 11.1 in eight; but of 28 and 4 heads of 128 in int8 11.3 and
-    // 11.0, 1060 tokens of 40 and 8 heads of 128 in 4 bits 15.5 and 13.4).
+    // 11.0, 1060 tokens of 40 and 8 heads of 128 in 4 bits 15.5 and 13.4).  Whole 4-bit histories
+    // with and without the two, 64 and 256 of 1056 tokens: 14 and 2 heads of 64 8.1 10.4 and 10.6 26.7,
+    // 40 and 8 of 128 18.5 69.8 and 29.1 85.7, but 8 and 8 of 64 15.2 51.3 and 19.3 47.8.
     const bool wider = bits == 4 || most_seen(most, window, sinks) < most;
     const int64_t W = mfma_waves(D), slack = wider ? 2 : 0, kib = wider && D <= 64 && tiles <= 4 * W + slack ? 288 : 128;
     const int64_t rows = pair ? 2 * g : (g < 16 ? g : 16), held = pair ? 2 * D : D;
@@ -263,6 +265,19 @@ static PagesPlan plan_pages(bool mfma, bool pair, bool whole, int64_t bits, int6
   if (p.splits < 1) p.splits = 1;
   p.slots = B * p.splits;
   return p;
+}
+
+// Whether a call whose KV heads could go in pairs goes one head a unit, by the plan for that: where the
+// short launch then has at most a workgroup for every CU, pairs only halve their number, and a wave has
+// both heads' work one after the other.  us in pairs and one by one, bf16 queries: 14 and 2 heads of 64,
+// 1 request of 1000 tokens 8.6 7.5, 16 of 1 .. 4000 11.7 10.4, 256 of 1 .. 1000 (512 workgroups)
+// 9.3 11.9; 28 and 4 heads of 128, 16 of 1 .. 1000 13.8 8.7, 64 of 1 .. 1000 15.7 10.8, 256 of
+// 1 .. 1000 26.4 31.0; 40 and 8 heads, 1 of 4000 15.5 13.0, 64 of 1 .. 1000 16.0 20.4.  Not where the parts
+// of a request are above four tiles a wave: 16 windows of 4096, 28 and 4 heads of 128, 17.8 and 19.9.
+// (The long launch goes in pairs; some single requests would be faster one by one: of 16000 tokens,
+// 40 and 8 heads of 128, 20.4 14.8; 28 and 4 heads 15.3 16.0; 64 of 1 .. 16000 tokens 66 73.)
+static bool one_by_one(const PagesPlan& p, int64_t B, int64_t D) {
+  return p.brief && B * p.units * p.slots <= 256 && (p.slots == 1 || p.min_tiles <= 4 * mfma_waves(D));
 }
 
 // Partials (m, l, o) of every slot and query head, the requests' slot ranges and the schedule.
@@ -362,8 +377,9 @@ extern "C" int hs_attend_pages_window(const void* query, int64_t q_stride_b, int
   // (4-bit scales of 256 of the head dim are loaded eight at a time)
   const bool mfma = shape && reinterpret_cast<uintptr_t>(pool) % 16 == 0 &&
                     (pool_code != HS_DTYPE_E2M1 || reinterpret_cast<uintptr_t>(scales) % 8 == 0);
-  const bool pair = mfma && t_stride_k == 0 && pages_pair_shape(pool_code, heads, kv_heads, head_dim);
-  PagesPlan p = plan_pages(shape, pair, false, bits, batch, heads, kv_heads, head_dim, tokens, newest, first);
+  PagesPlan p = plan_pages(shape, false, false, bits, batch, heads, kv_heads, head_dim, tokens, newest, first);
+  if (mfma && t_stride_k == 0 && pages_pair_shape(pool_code, heads, kv_heads, head_dim) && !one_by_one(p, batch, head_dim))
+    p = plan_pages(true, true, false, bits, batch, heads, kv_heads, head_dim, tokens, newest, first);
   if (shape && !mfma)
     p = plan_pages(false, false, pages_workspace(p, batch, heads, head_dim) == 0, bits, batch, heads, kv_heads, head_dim,
                    tokens, newest, first);

@@ -537,7 +537,7 @@ __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& o
 // half of a line take it from memory twice where they drift apart), and one exponential a lane
 // serves two heads.  us with one head a unit and with two: 8 requests of 131072 tokens, 28 and 4
 // heads of 128, 112 (the loads alone 111) and 106; 16 of 65536 .. 20521, 40 and 8 heads, float16
-// queries, 166 and 137; one of 1999, 14 and 2 heads of 64, 14.1 and 11.2.
+// queries, 166 and 137.  (Small calls go one by one: pages.hip, one_by_one.)
 // WINDOW: whole histories have kernels without its arithmetic, which takes up to ten registers and
 // with them one of two workgroups a CU where a kernel stands at the border.  us with it and without,
 // 14 query and 2 KV heads of 64, whole histories: float16, 512 requests of 1024 tokens 47.3 and 42.8,
