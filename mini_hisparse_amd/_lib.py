@@ -257,10 +257,11 @@ _DTYPE_CODES = {}  # torch dtype -> element code, filled at the first use (torch
 def _element_codes():
     import torch
 
-    _DTYPE_CODES.update({torch.float32: HS_DTYPE_F32, torch.float16: HS_DTYPE_F16, torch.bfloat16: HS_DTYPE_BF16,
-                         torch.int8: HS_DTYPE_I8, torch.float8_e4m3fn: HS_DTYPE_E4M3})
+    codes = {torch.float32: HS_DTYPE_F32, torch.float16: HS_DTYPE_F16, torch.bfloat16: HS_DTYPE_BF16,
+             torch.int8: HS_DTYPE_I8, torch.float8_e4m3fn: HS_DTYPE_E4M3}
     if hasattr(torch, "float4_e2m1fn_x2"):  # older builds of torch do everything but 4-bit pools
-        _DTYPE_CODES[torch.float4_e2m1fn_x2] = HS_DTYPE_E2M1
+        codes[torch.float4_e2m1fn_x2] = HS_DTYPE_E2M1
+    _DTYPE_CODES.update(codes)  # at once: another thread finds none of them or all
     return _DTYPE_CODES
 
 
