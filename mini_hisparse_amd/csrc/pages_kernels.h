@@ -541,8 +541,8 @@ __device__ __forceinline__ bool share_of(const PagesArgs& a, int32_t w, Share& o
 // WINDOW: whole histories have kernels without its arithmetic, which takes up to ten registers and
 // with them one of two workgroups a CU where a kernel stands at the border.  us with it and without,
 // 14 query and 2 KV heads of 64, whole histories: float16, 512 requests of 1024 tokens 47.3 and 42.8,
-// 1024 of 256 37.5 and 30.2; float16 queries on e4m3, 256 of 1 .. 4096 41.4 and 40.4 (96 of 4096 each,
-// 40 and 8 heads, are as fast again as before with two workgroups a CU, 121, and were 112 with one).
+// 1024 of 256 37.5 and 30.2; float16 queries on e4m3, 256 of 1 .. 4096 41.4 and 40.4 (but 96 of 4096
+// each, 40 and 8 heads, 112 with one workgroup a CU and 121 with two).
 template <int S, int QD, int D, bool UNIFORM, bool SHORT, bool WINDOW, bool PAIR = false>
 __global__ __launch_bounds__(64 * mfma_waves(D), mfma_least(QD, D, SHORT, PAIR)) void pages_mfma_kernel(PagesArgs a) {
   static_assert(!PAIR || (fp4(S) && D <= 128 && D != 96), "pairs of 4-bit head vectors of 32, 64 or 128");
